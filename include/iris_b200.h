@@ -468,6 +468,109 @@ int iris_softmax_exp_terms(uint32_t first, uint32_t count, uint64_t* out);
  * Synchronous; clears the library's fault word before and after. */
 int iris_wait_probe(int kind, int release);
 
+/* ---------------------------------------------------------------------------
+ * 6. Serving many requests: a paged K/V cache, packed prompts and drafted
+ *    trees. No counterpart in the reference, which decodes one sequence a
+ *    token at a time; the arithmetic is that loop's (Q16.16 rows, Q32.32 sums,
+ *    attention_softmax ops.rs:233-276), so a packed or drafted row equals the
+ *    row of its tokens decoded one by one, bit for bit. Device pointers
+ *    throughout; every call is asynchronous on `stream` (cudaStream_t as
+ *    void*), allocates nothing and may be captured. Refused arguments return
+ *    IRIS_EINVAL with nothing launched. Rows are int32, 16-byte aligned, their
+ *    strides in values and multiples of 4.
+ *
+ *    Pools: k_pages / v_pages hold [pages][page_size][kv_dim] values; request
+ *    r's token at index t lies in row table[r][t / page_size] * page_size +
+ *    t % page_size. A table entry that names no page of the pool hides its
+ *    tokens (nothing is read or written there).
+ * ------------------------------------------------------------------------- */
+/* The bookkeeping of one step on the device. Request r has held[r] tokens in
+ * the cache and brings fresh[r] more; table ([requests][width]) names the pages
+ * of the held ones. New pages come from free_pages in order, request by
+ * request, and are written into the table. Out: offsets (requests + 1: the
+ * packed rows of each request), slots (the pool row of each packed token, -1
+ * where it has none), positions (its index in its request) and counts:
+ * {tokens, pages taken, tokens past `tokens`, IRIS_PLAN_* faults}. Rows past
+ * the last token have slot -1 and position 0. With parents (each node's parent
+ * among its request's nodes, an earlier one, or -1): masks, bit j of a node's
+ * word saying whether it sees node j (itself and its ancestors), and the
+ * position counts a node's ancestors only; a node past 64, or one that hangs on
+ * a parent that is no earlier node, sees nothing (mask 0). At most 16,384
+ * requests. parents and masks are given together or not at all. */
+int iris_page_plan(const int32_t* d_held, const int32_t* d_fresh, uint32_t requests, uint32_t page_size,
+                   int32_t* d_table, uint32_t width, const int32_t* d_free, uint32_t n_free,
+                   const int32_t* d_parents, uint32_t tokens, int32_t* d_offsets, int64_t* d_slots,
+                   int32_t* d_positions, int64_t* d_masks, int32_t* d_counts, void* stream);
+#define IRIS_PLAN_POOL 1   /* the free list is too short: the last tokens have no slot */
+#define IRIS_PLAN_WIDTH 2  /* a request needs more pages than its table is wide */
+#define IRIS_PLAN_TOKENS 4 /* more fresh tokens than `tokens` */
+#define IRIS_PLAN_LENGTH 8 /* a negative length (taken as 0), or lengths past 2^31 */
+/* K and V rows ([tokens][kv_dim], strides apart) into their slots' pool rows;
+ * a slot outside [0, pool_rows) skips its row. kv_dim a multiple of 4. */
+int iris_page_append(const int32_t* d_k, const int32_t* d_v, uint64_t k_stride, uint64_t v_stride, uint32_t tokens,
+                     uint32_t kv_dim, const int64_t* d_slots, int32_t* d_k_pages, int32_t* d_v_pages,
+                     uint64_t pool_rows, void* stream);
+/* Causal attention of packed prompts: row i of request r (rows offsets[r] ..
+ * offsets[r + 1] - 1, offsets[0] = 0, offsets[requests] = tokens) attends over
+ * its request's rows up to i, the last `window` of them where window is not 0.
+ * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]
+ * (a fused q|k|v row's parts may be passed with its stride). longest: no
+ * request is longer. scale_q32: the score scale (mistral.rs:148-160), 0 for
+ * unscaled scores (gemma-dense). head_dim a multiple of 4, at most 256. */
+typedef struct {
+  const int32_t *q, *k, *v;
+  const int32_t* offsets;
+  int32_t* out;
+  uint64_t q_stride, k_stride, v_stride, out_stride;
+  uint32_t requests, tokens, longest;
+  uint32_t heads, kv_heads, head_dim;
+  uint32_t window, scale_q32;
+} IrisPromptAttention;
+/* Bytes of device scratch (16-byte aligned) the call needs, 0 for refused
+ * arguments; a smaller workspace is refused with IRIS_ESCRATCH. Its contents
+ * mean nothing between calls. */
+uint64_t iris_prompt_attention_workspace(const IrisPromptAttention* a);
+int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_t workspace_bytes, void* stream);
+/* Attention of drafted trees over the paged cache (K/V of the nodes appended
+ * already): request r's nodes are the packed rows offsets[r] .. offsets[r + 1]
+ * - 1, at most `nodes` <= 64 of them; a node sees the held[r] cached tokens
+ * and the nodes of its mask. With a window, only keys at positions above its own less the window
+ * (positions: of the nodes, required then). A node that sees no key gives
+ * zeros. longest: no request has more cached tokens and nodes together; at
+ * most width * page_size. One node a request whose mask is 1 is plain decoding. */
+typedef struct {
+  const int32_t* q;
+  const int32_t *k_pages, *v_pages;
+  const int32_t* table;
+  const int32_t* held;
+  const int32_t* offsets;
+  const int64_t* masks;
+  const int32_t* positions; /* may be NULL without a window */
+  int32_t* out;
+  uint64_t q_stride, out_stride, pages;
+  uint32_t requests, rows, width, page_size, nodes, longest;
+  uint32_t heads, kv_heads, head_dim;
+  uint32_t window, scale_q32;
+} IrisTreeAttention;
+uint64_t iris_tree_attention_workspace(const IrisTreeAttention* a);
+int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t workspace_bytes, void* stream);
+/* The drafted tokens that greedy decoding accepts: from a request's node 0
+ * (its last committed token) to the lowest child whose token is the pick at
+ * the current node (picks: the model's selection after each node), until there
+ * is none. Out: path ([requests][path_width], the nodes, -1 after the last),
+ * accepted (their number, 0 without nodes), next (the pick at the last one, -1
+ * without nodes) and held_out = held + accepted. With pools (NULL to leave
+ * them alone) the accepted nodes' K/V rows of each of `layers` layers
+ * (layer_stride values apart) move to indices held, held + 1, ... of the
+ * request, so that held_out tokens are cached. path_width <= 64: nodes past it
+ * are not looked at. A parent that is no earlier node is no parent. */
+int iris_tree_accept(const int32_t* d_tokens, const int32_t* d_parents, const int32_t* d_picks,
+                     const int32_t* d_offsets, uint32_t requests, uint32_t rows, const int32_t* d_held,
+                     uint32_t path_width, int32_t* d_path, int32_t* d_accepted, int32_t* d_next, int32_t* d_held_out,
+                     const int32_t* d_table, uint32_t width, uint32_t page_size, int32_t* d_k_pages,
+                     int32_t* d_v_pages, uint32_t layers, uint64_t layer_stride, uint64_t pages, uint32_t kv_dim,
+                     void* stream);
+
 /* Message for any status this library returns. */
 const char* iris_error(int code);
 

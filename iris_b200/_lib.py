@@ -17,6 +17,7 @@ LIB_PATH = PKG / "libiris_b200.so"
 IRIS_EINVAL, IRIS_ESCALE, IRIS_ERANGE, IRIS_ESTATE, IRIS_EWINDOW, IRIS_ESTALL = 10001, 10002, 10003, 10004, 10005, 10006
 IRIS_ESCRATCH = 10007
 NOALLOC_PLANES_BYTES = 16 << 20
+PLAN_POOL, PLAN_WIDTH, PLAN_TOKENS, PLAN_LENGTH = 1, 2, 4, 8
 PATH_AUTO, PATH_GEMV, PATH_GEMM, PATH_TC, PATH_TC3, PATH_GEMV1 = 0, 1, 2, 3, 4, 5
 GEMM_AUTO, GEMM_MMA = 0, 1
 ATTN_AUTO, ATTN_SPLIT, ATTN_CLUSTER = 0, 1, 2
@@ -59,6 +60,23 @@ class GemmaShape(C.Structure):
                 ("sliding_window", u32p), ("rope_base", i64p), ("rotary_dim", u32p),
                 ("rope_freq_base_dim", u32p), ("kv_donor_layer", i32p), ("layer_scalar", i32p),
                 ("tied_head", C.c_uint32)]
+
+
+class PromptAttention(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("offsets", vp), ("out", vp),
+                ("q_stride", C.c_uint64), ("k_stride", C.c_uint64), ("v_stride", C.c_uint64),
+                ("out_stride", C.c_uint64), ("requests", C.c_uint32), ("tokens", C.c_uint32),
+                ("longest", C.c_uint32), ("heads", C.c_uint32), ("kv_heads", C.c_uint32),
+                ("head_dim", C.c_uint32), ("window", C.c_uint32), ("scale_q32", C.c_uint32)]
+
+
+class TreeAttention(C.Structure):
+    _fields_ = [("q", vp), ("k_pages", vp), ("v_pages", vp), ("table", vp), ("held", vp), ("offsets", vp),
+                ("masks", vp), ("positions", vp), ("out", vp), ("q_stride", C.c_uint64),
+                ("out_stride", C.c_uint64), ("pages", C.c_uint64), ("requests", C.c_uint32), ("rows", C.c_uint32),
+                ("width", C.c_uint32), ("page_size", C.c_uint32), ("nodes", C.c_uint32), ("longest", C.c_uint32),
+                ("heads", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("window", C.c_uint32), ("scale_q32", C.c_uint32)]
 
 
 # name -> (restype, argtypes); every symbol include/iris_b200.h declares.
@@ -137,6 +155,17 @@ SIGNATURES = {
     "iris_host_free": (None, [vp]),
     "iris_synth_q8": (C.c_int, [C.c_uint64, C.c_uint32, C.c_int32, C.c_uint32, C.c_uint32, C.c_int, u8p]),
     "iris_synth_values": (C.c_int, [C.c_uint64, C.c_uint32, C.c_int32, C.c_uint64, C.c_uint32, i32p]),
+    "iris_page_plan": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, C.c_uint32, vp, C.c_uint32,
+                                 vp, vp, vp, vp, vp, vp]),
+    "iris_page_append": (C.c_int, [vp, vp, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, vp, vp, vp, C.c_uint64,
+                                   vp]),
+    "iris_prompt_attention_workspace": (C.c_uint64, [C.POINTER(PromptAttention)]),
+    "iris_prompt_attention": (C.c_int, [C.POINTER(PromptAttention), vp, C.c_uint64, vp]),
+    "iris_tree_attention_workspace": (C.c_uint64, [C.POINTER(TreeAttention)]),
+    "iris_tree_attention": (C.c_int, [C.POINTER(TreeAttention), vp, C.c_uint64, vp]),
+    "iris_tree_accept": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp, vp, vp, vp,
+                                   C.c_uint32, C.c_uint32, vp, vp, C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint32,
+                                   vp]),
     "iris_error": (C.c_char_p, [C.c_int]),
 }
 

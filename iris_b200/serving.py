@@ -1,0 +1,225 @@
+"""Serving many requests over one paged K/V cache: a step's block tables and
+slot map, packed prompts, drafted trees and their acceptance.
+
+The operators take CUDA tensors (int32 Q16.16 rows, as every activation of the
+library) and run in libiris_b200.so on torch's current stream, asynchronously
+and without host synchronisation; outputs and scratch come from torch's
+allocator. Their arithmetic is the decode loop's, so a token verified in a
+drafted tree, or a prompt row packed among others, has the values that
+decoding it alone gives, bit for bit. include/iris_b200.h (section 6) states
+each operator's contract; a refused argument raises IrisError (or ValueError
+where a tensor has the wrong type, shape or device).
+
+One step of a drafted decode:
+
+    plan = page_plan(held, fresh, table, free_pages, page_size, tokens, parents=parents)
+    ... q, k, v rows of the drafted tokens at plan.positions ...
+    page_append(k, v, plan.slots, k_pages, v_pages)            # each layer
+    ctx = tree_attention(q, k_pages, v_pages, plan.table, held, plan.offsets, plan.masks, ...)
+    ... picks = the model's first-maximum token after each node ...
+    done = tree_accept(tokens, parents, picks, plan.offsets, held, plan.table, nodes,
+                       k_pages=all_k, v_pages=all_v)           # all layers at once
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from ._lib import check, lib
+
+TREE_NODES = 64  # drafted nodes a request
+
+
+class PagePlan(NamedTuple):
+    """The bookkeeping of a step (page_plan). faults() waits for the device."""
+    offsets: torch.Tensor    # [requests + 1] packed rows of each request
+    slots: torch.Tensor      # [tokens] int64 pool rows, -1: none
+    positions: torch.Tensor  # [tokens]
+    table: torch.Tensor      # [requests][width], the one passed in
+    counts: torch.Tensor     # {tokens, pages taken, tokens left out, faults}
+    masks: Optional[torch.Tensor]  # [tokens] int64, with parents
+
+    def faults(self) -> int:
+        """PLAN_* bits of this plan (0: every token has its slot)."""
+        return int(self.counts[3])
+
+
+class Accepted(NamedTuple):
+    path: torch.Tensor      # [requests][path_width] accepted nodes, -1 after the last
+    accepted: torch.Tensor  # [requests]
+    next: torch.Tensor      # [requests] the token after the last accepted one
+    held: torch.Tensor      # [requests] cached tokens now
+
+
+def _need(x: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
+    """The address of a tensor whose last axis is dense; its other axes may have strides."""
+    if x.dtype != dtype or x.dim() != dim or not x.is_cuda or (x.numel() and x.stride(-1) != 1):
+        raise ValueError(f"{name}: a CUDA tensor of {dtype} with {dim} axes, the last one dense, is needed; "
+                         f"got {x.dtype} {tuple(x.shape)} on {x.device} with strides {x.stride()}")
+    return x.data_ptr()
+
+
+def _dense(x: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
+    if not x.is_contiguous():
+        raise ValueError(f"{name}: a contiguous tensor is needed; got strides {x.stride()}")
+    return _need(x, name, dtype, dim)
+
+
+def _same(count: int, want: int, name: str) -> None:
+    if count != want:
+        raise ValueError(f"{name}: {count} entries, expected {want}")
+
+
+def _stream(x: torch.Tensor) -> int:
+    if x.device.index != torch.cuda.current_device():
+        raise ValueError(f"tensors are on {x.device}, but cuda:{torch.cuda.current_device()} is the current device")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, page_size: int,
+              tokens: int, parents: Optional[torch.Tensor] = None) -> PagePlan:
+    """Block tables and slot map of a step: request r has held[r] cached tokens
+    and brings fresh[r]. New pages are taken from free_pages in order and
+    written into `table` [requests][width]. `tokens`: rows of the outputs (at
+    least the fresh tokens). With `parents` (each drafted node's parent in its
+    request, -1 for a root) the plan has the nodes' visibility masks and their
+    positions count ancestors only."""
+    requests = held.numel()
+    ph, pf = _dense(held, "held"), _dense(fresh, "fresh")
+    pt, pp = _dense(table, "table", dim=2), _dense(free_pages, "free_pages")
+    _same(fresh.numel(), requests, "fresh")
+    _same(table.shape[0], requests, "table")
+    dev = held.device
+    offsets = torch.empty(requests + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
+    positions = torch.empty(tokens, dtype=torch.int32, device=dev)
+    counts = torch.empty(4, dtype=torch.int32, device=dev)
+    masks, pm, pa = None, None, None
+    if parents is not None:
+        if parents.numel() < tokens:
+            raise ValueError(f"parents: {parents.numel()} entries, expected {tokens}")
+        pa = _dense(parents, "parents")
+        masks = torch.empty(tokens, dtype=torch.int64, device=dev)
+        pm = masks.data_ptr()
+    check(lib().iris_page_plan(ph, pf, requests, page_size, pt, table.shape[1], pp, free_pages.numel(), pa, tokens,
+                               offsets.data_ptr(), slots.data_ptr(), positions.data_ptr(), pm, counts.data_ptr(),
+                               _stream(held)), "iris_page_plan")
+    return PagePlan(offsets, slots, positions, table, counts, masks)
+
+
+def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: torch.Tensor,
+                v_pages: torch.Tensor) -> None:
+    """K and V rows [tokens][kv_dim] into the pools [pages][page_size][kv_dim]
+    at their slots; a slot outside the pools (-1) skips its row."""
+    tokens, kv_dim = k.shape
+    pk, pv, ps = _need(k, "k", dim=2), _need(v, "v", dim=2), _dense(slots, "slots", torch.int64)
+    ck, cv = _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
+    if v.shape != k.shape or k_pages.shape != v_pages.shape or k_pages.shape[2] != kv_dim:
+        raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
+                         f"{tuple(v_pages.shape)} do not match")
+    _same(slots.numel(), tokens, "slots")
+    check(lib().iris_page_append(pk, pv, k.stride(0), v.stride(0), tokens, kv_dim, ps, ck, cv,
+                                 k_pages.shape[0] * k_pages.shape[1], _stream(k)), "iris_page_append")
+
+
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, longest: int, *,
+                     heads: int, kv_heads: int, scale_q32: int = 0, window: int = 0,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of packed prompts: q [tokens][heads * head_dim], k and v
+    [tokens][kv_heads * head_dim] (rows may be parts of a fused q|k|v row);
+    request r's rows are offsets[r] .. offsets[r + 1] - 1, the longest request
+    at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense)."""
+    tokens = q.shape[0]
+    pq, pk, pv, po = _need(q, "q", dim=2), _need(k, "k", dim=2), _need(v, "v", dim=2), _dense(offsets, "offsets")
+    if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
+        raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
+    dim = q.shape[1] // heads
+    if k.shape != (tokens, kv_heads * dim) or v.shape != k.shape:
+        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are not {tokens} rows of {kv_heads} heads of {dim}")
+    if out is None:
+        out = torch.empty((tokens, heads * dim), dtype=torch.int32, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
+    a = _lib.PromptAttention(pq, pk, pv, po, _need(out, "out", dim=2), q.stride(0), k.stride(0), v.stride(0),
+                             out.stride(0), offsets.numel() - 1, tokens, longest, heads, kv_heads, dim, window,
+                             scale_q32)
+    L, ref = lib(), C.byref(a)
+    ws = _workspace(L.iris_prompt_attention_workspace(ref), q.device)
+    check(L.iris_prompt_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                                  _stream(q)), "iris_prompt_attention")
+    return out
+
+
+def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                   held: torch.Tensor, offsets: torch.Tensor, masks: torch.Tensor, nodes: int, longest: int, *,
+                   heads: int, kv_heads: int, scale_q32: int = 0, window: int = 0,
+                   positions: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of drafted nodes over the paged cache, their K/V appended
+    already: q [rows][heads * head_dim], request r's nodes the rows offsets[r]
+    .. offsets[r + 1] - 1 (at most `nodes` each), a node seeing the held[r]
+    cached tokens and the nodes of its mask. `longest`: the most cached tokens
+    and nodes a request has together. A node that sees nothing gives zeros."""
+    rows, requests = q.shape[0], held.numel()
+    pq, ck, cv = _need(q, "q", dim=2), _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
+    pt, ph, po = _dense(table, "table", dim=2), _dense(held, "held"), _dense(offsets, "offsets")
+    pm = _dense(masks, "masks", torch.int64)
+    pp = _dense(positions, "positions") if positions is not None else None
+    if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
+        raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
+    dim = q.shape[1] // heads
+    if k_pages.shape != v_pages.shape or k_pages.shape[2] != kv_heads * dim:
+        raise ValueError(f"pools {tuple(k_pages.shape)}, {tuple(v_pages.shape)} do not hold {kv_heads} heads of {dim}")
+    _same(table.shape[0], requests, "table")
+    _same(offsets.numel(), requests + 1, "offsets")
+    for x, name in ((masks, "masks"), (positions, "positions")):
+        if x is not None and x.numel() < rows:
+            raise ValueError(f"{name}: {x.numel()} entries, expected {rows}")
+    if out is None:
+        out = torch.empty((rows, heads * dim), dtype=torch.int32, device=q.device)
+    elif out.shape != q.shape:
+        raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
+    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _need(out, "out", dim=2), q.stride(0), out.stride(0),
+                           k_pages.shape[0], requests, rows, table.shape[1], k_pages.shape[1], nodes, longest, heads,
+                           kv_heads, dim, window, scale_q32)
+    L, ref = lib(), C.byref(a)
+    ws = _workspace(L.iris_tree_attention_workspace(ref), q.device)
+    check(L.iris_tree_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
+                                _stream(q)), "iris_tree_attention")
+    return out
+
+
+def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor, offsets: torch.Tensor,
+                held: torch.Tensor, table: torch.Tensor, path_width: int, *, k_pages: Optional[torch.Tensor] = None,
+                v_pages: Optional[torch.Tensor] = None) -> Accepted:
+    """The drafted nodes that greedy decoding accepts (from node 0, to the
+    child that holds the pick, until none does) and, with pools
+    [layers][pages][page_size][kv_dim], their K/V rows moved after the cached
+    ones, in place, in every layer."""
+    rows, requests = tokens.numel(), held.numel()
+    pt, pa, pk = _dense(tokens, "tokens"), _dense(parents, "parents"), _dense(picks, "picks")
+    po, ph, tb = _dense(offsets, "offsets"), _dense(held, "held"), _dense(table, "table", dim=2)
+    for x, n, name in ((parents, rows, "parents"), (picks, rows, "picks"), (offsets, requests + 1, "offsets"),
+                       (table[:, :1], requests if table.shape[1] else 0, "table")):
+        _same(x.numel(), n, name)
+    dev = held.device
+    path = torch.empty((requests, path_width), dtype=torch.int32, device=dev)
+    out = torch.empty((3, requests), dtype=torch.int32, device=dev)
+    layers, stride, pages, page, kv_dim, ck, cv = 0, 0, 0, 0, 0, None, None
+    if k_pages is not None or v_pages is not None:
+        if k_pages is None or v_pages is None or k_pages.shape != v_pages.shape:
+            raise ValueError("k_pages and v_pages are given together, of one shape")
+        ck, cv = _dense(k_pages, "k_pages", dim=4), _dense(v_pages, "v_pages", dim=4)
+        layers, pages, page, kv_dim = k_pages.shape
+        stride = pages * page * kv_dim
+    base = out.data_ptr()
+    check(lib().iris_tree_accept(pt, pa, pk, po, requests, rows, ph, path_width, path.data_ptr(), base,
+                                 base + 4 * requests, base + 8 * requests, tb, table.shape[1], page, ck, cv, layers,
+                                 stride, pages, kv_dim, _stream(held)), "iris_tree_accept")
+    return Accepted(path, out[0], out[1], out[2])
