@@ -433,6 +433,35 @@ IRIS_HD int32_t scaled_score_finish(int64_t sum, uint32_t scale_q32) {
 
 // ---- softmax (ops.rs:233-276, 508-556) -------------------------------------
 
+// softmax_exp_term (ops.rs:508-556) of the Q16.16 distance d below the maximum,
+// 1 <= d < 2^20 (from 2^20 = 16.0 on the term is 0; at 0 it is 2^32): the same
+// value as softmax_exp_term_act in 32-bit halves. k = floor(d 2^16 / ln2) from
+// one product (no d in the range comes nearer to a multiple of ln2 than the
+// product's error), r = d 2^16 - k ln2 below 2^32; each power is the high word
+// of a product, rounded half to even by one addition; each quotient by n is
+// floor((x + n/2) / n), one less where that is an odd tie.
+IRIS_HD uint32_t exp_term_power(uint32_t a, uint32_t r) {
+  const uint64_t p = (uint64_t)a * r;
+  return (uint32_t)((p + 0x7FFFFFFFu + ((uint32_t)(p >> 32) & 1)) >> 32);
+}
+template <uint32_t N>
+IRIS_HD uint32_t exp_term_over(uint32_t x) {
+  const uint32_t s = x + N / 2, q = s / N;
+  return q - (q * N == s ? q & 1 : 0);
+}
+IRIS_HD uint32_t exp_term_near(uint32_t d) {
+  // 2^52 / (ln2 in Q16.16 * 2^11), ln2 = 2977044472 / 2^32
+  const uint32_t k = (uint32_t)(((uint64_t)(d << 11) * 48408813u) >> 52);
+  const uint32_t r = (d << 16) - k * 2977044472u;
+  const uint32_t r2 = exp_term_power(r, r), r3 = exp_term_power(r2, r), r4 = exp_term_power(r3, r),
+                 r5 = exp_term_power(r4, r);
+  const uint32_t a = 0u - r + ((r2 + ((r2 >> 1) & 1)) >> 1) - exp_term_over<6>(r3) + exp_term_over<24>(r4) -
+                     exp_term_over<120>(r5);
+  // a / 2^k, ties to even: the bits shifted out, at the top of a word
+  const uint32_t f = a >> k, out = k ? a << (32 - k) : 0;
+  return f + (out + (f & 1) > 0x80000000u);
+}
+
 // softmax_exp_term(act_to_acc(sub_sat(logit, max))): e^delta in Q32.32.
 IRIS_HD int64_t softmax_exp_term_act(int32_t logit, int32_t max_logit) {
   const int64_t ln2 = 2977044472ll;
