@@ -7,6 +7,7 @@
 #include "../../include/iris_b200.h"
 #include "common.cuh"
 #include "layers.cuh"
+#include "prompt_mma.cuh"
 #include "serve.cuh"
 #include "serve_attn.cuh"
 #include "tree_mma.cuh"
@@ -203,8 +204,8 @@ using namespace iris;
 extern "C" {
 
 uint64_t iris_prompt_attention_workspace(const IrisPromptAttention* a) {
-  if (check_prompt(a) || !a->tokens) return 0;
-  return 0;
+  if (check_prompt(a) || !a->tokens || !prompt_mma_usable(*a)) return 0;
+  return prompt_mma_workspace(*a);
 }
 
 int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -212,6 +213,7 @@ int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_
   if (bad || !a->tokens) return bad;
   const uint64_t need = iris_prompt_attention_workspace(a);
   if (need && (!aligned16(workspace) || workspace_bytes < need)) return IRIS_ESCRATCH;
+  if (prompt_mma_usable(*a)) return (int)launch_prompt_mma(*a, (uint8_t*)workspace, (cudaStream_t)stream);
   prompt_rows_kernel<<<dim3(a->tokens, a->heads), kRowThreads, 0, (cudaStream_t)stream>>>(*a);
   return (int)cudaGetLastError();
 }

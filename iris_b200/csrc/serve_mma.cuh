@@ -215,7 +215,7 @@ __device__ __forceinline__ uint32_t sum_recip(uint64_t sum) { return sum ? (uint
 // quotient first moves v by at most 1/4: so the weight is (y + 2^14) >> 15
 // unless a multiple of 2^15 lies within 1/4 below or 2.75 above y + 2^14;
 // there (4 values of 32768) the exact division decides.
-__device__ __noinline__ int32_t exact_weight(uint32_t term, uint64_t sum) {
+static __device__ __noinline__ int32_t exact_weight(uint32_t term, uint64_t sum) {
   return softmax_weight((int64_t)kept_term(term), sum);
 }
 __device__ __forceinline__ int32_t weight_of(uint32_t term, uint32_t recip, uint64_t sum) {
