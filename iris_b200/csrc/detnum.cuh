@@ -462,6 +462,22 @@ IRIS_HD uint32_t exp_term_near(uint32_t d) {
   return f + (out + (f & 1) > 0x80000000u);
 }
 
+// The same term within one: the polynomial by Horner's rule in truncated 32-bit
+// products, shifted down. From kExpExactBelow on (k >= 3, where the shift
+// drops most of the truncation) exp_term_near is this or one more, so one bit a
+// distance makes it exact; the host test checks every distance.
+static constexpr uint32_t kExpExactBelow = 136278;  // ceil(3 ln2 in Q16.16)
+IRIS_HD uint32_t exp_term_estimate(uint32_t d) {
+  const uint32_t k = (uint32_t)(((uint64_t)(d << 11) * 48408813u) >> 52);
+  const uint32_t r = (d << 16) - k * 2977044472u;
+  uint32_t a = 178956971u - mulhi_u32(r, 35791394u);  // 2^32 / 24, 2^32 / 120
+  a = 715827883u - mulhi_u32(r, a);                   // 2^32 / 6
+  a = 2147483648u - mulhi_u32(r, a);
+  a = 0u - mulhi_u32(r, a);
+  a = 0u - mulhi_u32(r, a);
+  return a >> k;
+}
+
 // softmax_exp_term(act_to_acc(sub_sat(logit, max))): e^delta in Q32.32.
 IRIS_HD int64_t softmax_exp_term_act(int32_t logit, int32_t max_logit) {
   const int64_t ln2 = 2977044472ll;

@@ -16,6 +16,7 @@
 #include "common.cuh"
 #include "layers.cuh"
 #include "prompt_mma.cuh"
+#include "prompt_tc.cuh"
 #include "serve_attn.cuh"
 #include "serve_mma.cuh"
 #include "tc.cuh"
@@ -31,10 +32,12 @@ constexpr uint32_t kSortRequests = 1024;
 struct PromptScratch {
   uint32_t* order;   // [requests]: the requests, longest first
   uint32_t* tiles;   // [requests + 1]: tiles before each of them
-  uint32_t* next;    // the item counter
+  uint32_t* next;    // the item counters of this kernel and of prompt_tc_kernel
   int32_t* scores;   // [blocks][RT][pitch]
   int64_t* acc;      // [blocks][RT][d]: value sums, where several warps or segments add to one
   uint32_t pitch, blocks;
+  const uint32_t* wide;  // [flags]: with the tensor-core kernel before this one, whether it left the call to it
+  uint32_t flags;
 };
 
 // The tiles of each request, longest first (up to 1024 requests; more keep
@@ -48,8 +51,9 @@ __global__ void __launch_bounds__(1024) prompt_items_kernel(IrisPromptAttention 
     const uint32_t b = clamp_offset(a.offsets[r], a.tokens), e = clamp_offset(a.offsets[r + 1], a.tokens);
     return e > b ? min(e - b, a.longest) : 0u;
   };
+  pdl_trigger();
   if (tid == 0) {
-    *sc.next = 0;
+    sc.next[0] = sc.next[1] = 0;
     carry = 0;
   }
   const bool sorted = a.requests <= kSortRequests;
@@ -246,6 +250,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
   const QueryTile tile{frag, steps};
   pdl_wait();
   pdl_trigger();
+  if (sc.flags) {
+    uint32_t wide = 0;
+    for (uint32_t i = tid; i < sc.flags; i += kPromptThreads) wide |= sc.wide[i];
+    if (!__syncthreads_or(wide != 0)) return;
+  }
   const uint32_t items = sc.tiles[a.requests] * a.kv_heads;
   for (;;) {
     __syncthreads();  // the tile before is done with the shared memory
@@ -373,33 +382,52 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // cover 16 dimensions x 32 rows, sixteen warps).
 uint32_t row_tile(const IrisPromptAttention& a) { return a.head_dim <= 128 ? 64 : 32; }
 
-size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc) {
+// The tensor-core kernel's packing and its two further launches pay from
+// requests of a few hundred rows on.
+constexpr uint32_t kTcLongest = 256;
+bool on_tensor_cores(const IrisPromptAttention& a) { return a.longest >= kTcLongest && prompt_tc_usable(a); }
+
+size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, PromptTcScratch* tc) {
   const uint32_t rt = row_tile(a), group = a.heads / a.kv_heads;
   const uint64_t tiles = ((uint64_t)a.tokens * group + rt - 1) / rt + a.requests;
   sc->blocks = (uint32_t)std::min<uint64_t>(tiles * a.kv_heads, (uint64_t)device_sms());
   const uint32_t keys = a.window ? std::min<uint64_t>(a.longest, (uint64_t)a.window + rt + 16) : a.longest;
-  sc->pitch = (keys + 31) / 32 * 32 + 32;
+  sc->pitch = (keys + 15 + 127) / 128 * 128;  // a tile's first key is rounded down to 16, its last up to 128
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t* p = base + at;
     at += up256(bytes);
     return p;
   };
-  sc->next = (uint32_t*)take(4);
+  sc->next = (uint32_t*)take(8);
   sc->tiles = (uint32_t*)take(((size_t)a.requests + 1) * 4);
   sc->order = (uint32_t*)take((size_t)a.requests * 4);
   sc->scores = (int32_t*)take((size_t)sc->blocks * rt * sc->pitch * 4);
   sc->acc = (int64_t*)take((size_t)sc->blocks * rt * a.head_dim * 8);
+  sc->wide = nullptr;
+  sc->flags = 0;
+  if (on_tensor_cores(a)) {
+    at += prompt_tc_carve(a, base + at, tc);
+    tc->order = sc->order;
+    tc->tiles = sc->tiles;
+    tc->next = sc->next + 1;
+    tc->scores = sc->scores;
+    tc->pitch = sc->pitch;
+    sc->wide = tc->wide;
+    sc->flags = tc->flags;
+  }
   return at;
 }
 
 template <uint32_t RT>
-cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, cudaStream_t stream) {
+cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, const PromptTcScratch& tc,
+                   cudaStream_t stream) {
   const uint32_t smem = RT / 8 * (a.head_dim / 32) * 1024 + 2 * kPromptKeys / 32 * (RT / 8) * 512;
   cudaError_t e = cudaFuncSetAttribute(prompt_mma_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   prompt_items_kernel<<<1, 1024, 0, stream>>>(a, sc, RT);
   e = cudaGetLastError();
+  if (e == cudaSuccess && sc.flags) e = launch_prompt_tc(a, tc, sc.blocks, stream);
   if (e != cudaSuccess) return e;
   return launch_k(prompt_mma_kernel<RT>, dim3(sc.blocks), dim3(kPromptThreads), smem, stream, a, sc);
 }
@@ -412,13 +440,15 @@ bool prompt_mma_usable(const IrisPromptAttention& a) {
 
 uint64_t prompt_mma_workspace(const IrisPromptAttention& a) {
   PromptScratch sc;
-  return carve(a, nullptr, &sc);
+  PromptTcScratch tc;
+  return carve(a, nullptr, &sc, &tc);
 }
 
 cudaError_t launch_prompt_mma(const IrisPromptAttention& a, uint8_t* workspace, cudaStream_t stream) {
   PromptScratch sc;
-  carve(a, workspace, &sc);
-  return row_tile(a) == 64 ? launch<64>(a, sc, stream) : launch<32>(a, sc, stream);
+  PromptTcScratch tc;
+  carve(a, workspace, &sc, &tc);
+  return row_tile(a) == 64 ? launch<64>(a, sc, tc, stream) : launch<32>(a, sc, tc, stream);
 }
 
 }  // namespace iris

@@ -1,0 +1,540 @@
+// Packed prompt attention on the tcgen05 tensor cores (kind::i8), head_dim 128.
+//
+// The same three phases as prompt_mma.cu, with the contractions on the
+// fifth-generation tensor cores. Operands are packed once a call into K-major
+// byte planes (three: 24-bit values; where any operand is wider the kernel
+// leaves the call to prompt_mma_kernel, launched behind it, which then runs):
+// queries [K/V head][plane][token * group + head][128], keys [head][plane]
+// [token][128], values transposed [head][plane][128][token]. A tile of 64 query
+// rows that share a K/V head goes through
+//   1. scores: 128 keys x 64 rows x 32 dims a product, nine plane pairs into
+//      five int32 diagonals of 64 TMEM columns; the epilogue warps carry the
+//      diagonals together, release them to the next tile's products and write
+//      the scores to the block's scratch (L2) while those run;
+//   2. terms in place, a row a warp; an exponential is its polynomial in
+//      truncated 32-bit products plus one bit of a table in shared memory that
+//      makes it exact (exp_term_estimate);
+//   3. weights of 128 keys into shared memory as two swizzled byte planes, and
+//      128 dims x 64 rows x 32 positions a product, six plane pairs into four
+//      diagonals that stay in TMEM over all keys.
+// Sixteen epilogue warps, one warp that feeds the ring (16 KB, one plane of 128
+// keys a slot) by TMA and one that issues the products. Every wait is bounded;
+// a give-up ends the block and is recorded in the fault word.
+#include <algorithm>
+
+#include "../../include/iris_b200.h"
+#include "common.cuh"
+#include "layers.cuh"
+#include "prompt_tc.cuh"
+#include "q8.cuh"
+#include "serve_attn.cuh"
+#include "serve_mma.cuh"
+#include "tc.cuh"
+#include "tcgen05.cuh"
+
+namespace iris {
+
+namespace {
+
+constexpr uint32_t kPtD = 128, kPtRows = 64, kPtKeys = 128;
+constexpr uint32_t kPtEpiWarps = 16, kPtEpi = 32 * kPtEpiWarps, kPtThreads = kPtEpi + 64;
+constexpr uint32_t kPtSlots = 5, kPtSlot = kPtKeys * kPtD;  // one plane of a key or value tile
+constexpr uint32_t kPtQPlane = kPtRows * kPtD;              // one plane of the query rows; of a weight tile
+constexpr uint32_t kPtWBuf = 2 * kPtQPlane;                 // two weight planes
+constexpr uint32_t kPtTable = (kExpTerms - kExpExactBelow / 32 * 32) / 32;  // words
+constexpr uint32_t kPtRing = kPtSlots * kPtSlot;
+constexpr uint32_t kPtOperands = 2 * kPtWBuf;  // the query planes (3 x 8 KB), later two weight buffers
+constexpr uint32_t kPtSmem = 1024 + kPtRing + kPtOperands + kPtTable * 4;
+static_assert(3 * kPtQPlane <= kPtOperands, "query planes");
+static_assert(5 * kPtRows <= 512, "TMEM columns");
+
+// ---- packing -------------------------------------------------------------------
+
+// Rows of 128 values (row r, part g at src + (r / per) * stride + (g * per + r %
+// per) * 128) into planes dst[g][3][rows][128]; flags what is past 24 bits.
+__device__ __forceinline__ uint32_t pack_row4(const int32_t* src, uint8_t* dst, uint64_t plane) {
+  const int4 x = *(const int4*)src;
+  uint32_t p[4];
+  split_planes(x.x, x.y, x.z, x.w, p);
+#pragma unroll
+  for (uint32_t i = 0; i < 3; ++i) *(uint32_t*)(dst + i * plane) = p[i];
+  return past_24_bits(p);
+}
+
+constexpr uint32_t kPackThreads = 256;
+
+// blockIdx.y: 0 queries, 1 keys, 2 values (transposed through shared memory, 32
+// tokens x 32 dims a pass), 3 the exponential's correction bits.
+__global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAttention a, PromptTcScratch sc) {
+  __shared__ int32_t tile[32][33];
+  const uint32_t tid = threadIdx.x, group = a.heads / a.kv_heads;
+  pdl_trigger();
+  uint32_t wide = 0;
+  if (blockIdx.y <= 1) {
+    const bool keys = blockIdx.y == 1;
+    const uint32_t per = keys ? 1 : group;
+    const uint64_t rows = (uint64_t)a.tokens * per, n = rows * a.kv_heads * 32;
+    const int32_t* src = keys ? a.k : a.q;
+    const uint64_t stride = keys ? a.k_stride : a.q_stride;
+    uint8_t* dst = keys ? sc.kp : sc.qp;
+    for (uint64_t i = (uint64_t)blockIdx.x * kPackThreads + tid; i < n; i += (uint64_t)gridDim.x * kPackThreads) {
+      const uint32_t c = (uint32_t)(i & 31), h = (uint32_t)((i >> 5) % (per * a.kv_heads));
+      const uint64_t token = (i >> 5) / (per * a.kv_heads);
+      const uint64_t row = token * per + h % per;
+      wide |= pack_row4(src + token * stride + (uint64_t)h * kPtD + 4 * c,
+                        dst + ((uint64_t)(h / per) * 3 * rows + row) * kPtD + 4 * c, rows * kPtD);
+    }
+  } else if (blockIdx.y == 2) {
+    const uint32_t tx = tid & 31, ty = tid >> 5;
+    const uint32_t tts = (a.tokens + 31) / 32;
+    for (uint64_t u = blockIdx.x; u < (uint64_t)tts * 4 * a.kv_heads; u += gridDim.x) {
+      const uint32_t g = (uint32_t)(u % a.kv_heads), d0 = (uint32_t)(u / a.kv_heads % 4) * 32,
+                     t0 = (uint32_t)(u / a.kv_heads / 4) * 32;
+      __syncthreads();
+      for (uint32_t r = ty; r < 32; r += 8) {
+        const uint32_t t = t0 + r;
+        tile[r][tx] = t < a.tokens ? a.v[(uint64_t)t * a.v_stride + g * kPtD + d0 + tx] : 0;
+      }
+      __syncthreads();
+      // thread: dimension tid / 8, four tokens
+      const uint32_t d = tid >> 3, t = 4 * (tid & 7);
+      uint32_t p[4];
+      split_planes(tile[t][d], tile[t + 1][d], tile[t + 2][d], tile[t + 3][d], p);
+      wide |= past_24_bits(p);
+#pragma unroll
+      for (uint32_t i = 0; i < 3; ++i)
+        *(uint32_t*)(sc.vt + (((uint64_t)g * 3 + i) * kPtD + d0 + d) * sc.tpitch + t0 + t) = p[i];
+    }
+  } else {
+    const uint32_t lane = tid & 31;
+    for (uint32_t d = (kExpExactBelow / 32 * 32) + blockIdx.x * kPackThreads + tid; d < kExpTerms;
+         d += gridDim.x * kPackThreads) {
+      const uint32_t bits = __ballot_sync(0xffffffffu, exp_term_near(d) != exp_term_estimate(d));
+      if (lane == 0) sc.exp_bits[d / 32 - kExpExactBelow / 32] = bits;
+    }
+  }
+  wide = __syncthreads_or(wide != 0);
+  if (tid == 0) sc.wide[blockIdx.y * gridDim.x + blockIdx.x] = wide ? 1 : 0;
+  pdl_wait();  // the item list, which the kernel after this one reads, is complete too
+}
+
+// ---- the attention ----------------------------------------------------------------
+
+struct PtShared {
+  uint64_t full[kPtSlots], empty[kPtSlots], q_full, s_done, t_free, w_full[2], w_empty[2], v_done;
+  uint64_t sum[kPtRows];
+  int32_t top[kPtRows], query[kPtRows], wsum[kPtRows];
+  uint32_t recip[kPtRows], first[kPtRows];
+  uint32_t item, tmem, dead, wide;
+};
+
+// mbar_wait_bounded that gives up at once after any wait of the block has.
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, PtShared& s, unsigned int* fault) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_ns();
+  for (;;) {
+    if (mbar_try_wait_suspend(bar, parity)) return true;
+    if (*(volatile uint32_t*)&s.dead) return false;
+    if (global_ns() - t0 > 1000000000ull) {
+      *(volatile uint32_t*)&s.dead = 1;
+      atomicOr(fault, 1u);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
+
+// exp_term_near by the estimate and its correction bit.
+__device__ __forceinline__ uint32_t term_by_table(uint32_t d, const uint32_t* bits) {
+  const uint32_t word = bits[(d >> 5) - kExpExactBelow / 32];
+  return exp_term_estimate(d) + (__funnelshift_r(word, 0, d) & 1);
+}
+
+__global__ void __launch_bounds__(kPtThreads, 1)
+    prompt_tc_kernel(IrisPromptAttention a, PromptTcScratch sc, const __grid_constant__ CUtensorMap qmap,
+                     const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                     unsigned int* fault) {
+  extern __shared__ uint8_t pt_raw[];
+  __shared__ __align__(8) PtShared s;
+  uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t* ops = ring + kPtRing;  // query planes, then weight buffers
+  uint32_t* bits = (uint32_t*)(ops + kPtOperands);
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (uint32_t i = 0; i < kPtSlots; ++i) {
+      mbar_init(&s.full[i], 1);
+      mbar_init(&s.empty[i], 1);
+    }
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.s_done, 1);
+    mbar_init(&s.t_free, kPtEpiWarps);
+    for (uint32_t i = 0; i < 2; ++i) {
+      mbar_init(&s.w_full[i], kPtEpiWarps);
+      mbar_init(&s.w_empty[i], 1);
+    }
+    mbar_init(&s.v_done, 1);
+    s.dead = 0;
+    s.wide = 0;
+    mbar_fence_init();
+  }
+  if (warp == kPtEpiWarps) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&s.tmem)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  pdl_wait();
+  pdl_trigger();
+  {
+    uint32_t wide = 0;
+    for (uint32_t i = tid; i < sc.flags; i += kPtThreads) wide |= sc.wide[i];
+    if (wide) s.wide = 1;
+    for (uint32_t i = tid; i < kPtTable; i += kPtThreads) bits[i] = sc.exp_bits[i];
+  }
+  __syncthreads();
+  const bool run = s.wide == 0;
+  const uint32_t items = run ? sc.tiles[a.requests] * a.kv_heads : 0, group = a.heads / a.kv_heads;
+  int32_t* scores = sc.scores + (uint64_t)blockIdx.x * kPtRows * sc.pitch;
+
+  // each role's running counts of the barriers' phases
+  uint32_t ring_n = 0, n_item = 0, n_s = 0, n_w = 0;
+  uint32_t issued[kPtSlots] = {};
+  bool ok = true;
+  for (;; ++n_item) {
+    __syncthreads();  // the item before is done with the shared memory and the accumulators
+    if (tid == 0) s.item = s.dead ? UINT32_MAX : atomicAdd(sc.next, 1u);
+    __syncthreads();
+    const uint32_t item = s.item;
+    if (item >= items) break;
+    const uint32_t g = item % a.kv_heads, at = item / a.kv_heads;
+    const uint32_t rank = request_of(sc.tiles, a.requests, at), r = sc.order[rank];
+    const uint32_t begin = clamp_offset(a.offsets[r], a.tokens);
+    const uint32_t len = min(clamp_offset(a.offsets[r + 1], a.tokens) - begin, a.longest);
+    const uint32_t f0 = (sc.tiles[rank + 1] - 1 - at) * kPtRows, rows = min(kPtRows, len * group - f0);
+    const uint32_t q0 = f0 / group, q1 = (f0 + rows - 1) / group;
+    // keys by their packed row from k0 on, a multiple of 16 (the transposed
+    // values' TMA starts there); rows of other requests are hidden
+    const uint32_t k0 = (begin + window_start(q0, a.window)) / 16 * 16, count = begin + q1 + 1 - k0;
+    const uint32_t ktiles = (count + kPtKeys - 1) / kPtKeys;
+
+    if (warp == kPtEpiWarps) {
+      if (lane == 0) {  // TMA producer
+        mbar_arrive_expect_tx(&s.q_full, 3 * kPtQPlane);
+        for (uint32_t j = 0; j < 3; ++j)
+          tma_load_3d(ops + j * kPtQPlane, &qmap, 0, (int32_t)(begin * group + f0), (int32_t)(g * 3 + j), &s.q_full);
+        for (uint32_t u = 0; u < 6 * ktiles && ok; ++u, ++ring_n) {
+          const uint32_t slot = ring_n % kPtSlots, use = ring_n / kPtSlots;
+          if (use > 0 && !pt_wait(&s.empty[slot], (use - 1) & 1, s, fault)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&s.full[slot], kPtSlot);
+          const bool vals = u >= 3 * ktiles;
+          const uint32_t v = vals ? u - 3 * ktiles : u, t = k0 + v / 3 * kPtKeys, plane = g * 3 + v % 3;
+          if (vals) tma_load_3d(ring + slot * kPtSlot, &vmap, (int32_t)t, 0, (int32_t)plane, &s.full[slot]);
+          else tma_load_3d(ring + slot * kPtSlot, &kmap, 0, (int32_t)t, (int32_t)plane, &s.full[slot]);
+          ++issued[slot];
+        }
+      }
+    } else if (warp == kPtEpiWarps + 1) {
+      if (lane == 0) {  // product issuer
+        ok = ok && pt_wait(&s.q_full, n_item & 1, s, fault);
+        const uint32_t ops_a = smem_addr(ops);
+        tc_fence_after();
+        for (uint32_t kt = 0; kt < ktiles && ok; ++kt) {
+          if (kt && !pt_wait(&s.t_free, (n_s - 1) & 1, s, fault)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint32_t touched = 0;
+#pragma unroll
+          for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
+            const uint32_t slot = ring_n % kPtSlots;
+            if (!ok || !pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t base = smem_addr(ring + slot * kPtSlot);
+#pragma unroll
+            for (uint32_t kk = 0; kk < 4; ++kk)
+#pragma unroll
+              for (uint32_t j = 0; j < 3; ++j) {
+                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base + kk * 32), tc_desc(ops_a + j * kPtQPlane + kk * 32),
+                       tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
+                touched |= 1u << (i + j);
+              }
+            tc_commit(&s.empty[slot]);
+          }
+          if (ok) tc_commit(&s.s_done);
+          ++n_s;
+        }
+        // the diagonals of the last score tile are read before the value sums take their columns
+        ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+        tc_fence_after();
+        uint32_t touched = 0;
+        for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
+          const uint32_t buf = n_w & 1;
+          if (!pt_wait(&s.w_full[buf], (n_w >> 1) & 1, s, fault)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
+            const uint32_t slot = ring_n % kPtSlots;
+            if (!ok || !pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t base = smem_addr(ring + slot * kPtSlot);
+#pragma unroll
+            for (uint32_t kk = 0; kk < 4; ++kk)
+#pragma unroll
+              for (uint32_t j = 0; j < 2; ++j) {
+                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base + kk * 32),
+                       tc_desc(ops_a + buf * kPtWBuf + j * kPtQPlane + kk * 32), tc_idesc(i == 2, false),
+                       (touched >> (i + j)) & 1u);
+                touched |= 1u << (i + j);
+              }
+            tc_commit(&s.empty[slot]);
+          }
+          if (ok) tc_commit(&s.w_empty[buf]);
+        }
+        if (ok) tc_commit(&s.v_done);
+      }
+    } else {
+      // epilogue warps: TMEM lanes 32 quad .. (keys, then dims), rows 16 cg ..
+      const uint32_t quad = warp & 3, cg = warp >> 2;
+      if (tid < kPtRows) {
+        s.top[tid] = INT32_MIN;
+        s.query[tid] = tid < rows ? (int32_t)((f0 + tid) / group) : -1;
+        s.wsum[tid] = 0;
+      }
+      epi_sync();
+      // 1. scores
+      int32_t best[16];
+#pragma unroll
+      for (uint32_t c = 0; c < 16; ++c) best[c] = INT32_MIN;
+      for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
+        if (!pt_wait(&s.s_done, n_s & 1, s, fault)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        uint32_t lo[16];
+        int32_t hi[16];
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          uint32_t v[5][8];
+#pragma unroll
+          for (uint32_t d = 0; d < 5; ++d) tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16 + h * 8, v[d]);
+          tmem_ld_wait();
+#pragma unroll
+          for (uint32_t c = 0; c < 8; ++c) {
+            const int32_t x[5] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c],
+                                  (int32_t)v[4][c]};
+            carry_diagonals(x, &hi[h * 8 + c], &lo[h * 8 + c]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.t_free);
+        const uint32_t t = kt * kPtKeys + 32 * quad + lane, key = k0 + t;
+        // the warp's keys, seen by every row of the tile?
+        const uint32_t kw = k0 + kt * kPtKeys + 32 * quad;
+        const bool open = rows == kPtRows && kw + 31 <= begin + q0 && kw >= begin + window_start(q1, a.window);
+        int32_t* out = scores + (uint64_t)(cg * 16) * sc.pitch + t;
+#pragma unroll
+        for (uint32_t c = 0; c < 16; ++c) {
+          int32_t x = score_of(hi[c], lo[c], a.scale_q32);
+          if (!open) {
+            const int32_t q = s.query[cg * 16 + c];
+            if (q < 0 || key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window)) x = INT32_MIN;
+          }
+          best[c] = max(best[c], x);
+          __stcg(out + c * sc.pitch, x);
+        }
+      }
+#pragma unroll
+      for (uint32_t c = 0; c < 16; ++c) {
+        const int32_t x = __reduce_max_sync(0xffffffffu, best[c]);
+        if (lane == 0) atomicMax(&s.top[cg * 16 + c], x);
+      }
+      epi_sync();
+      // 2. terms in place, a row a warp (hidden keys: see prompt_mma.cu)
+      const uint32_t padded = ktiles * kPtKeys;
+      for (uint32_t i = warp; i < kPtRows; i += kPtEpiWarps) {
+        const int32_t top = s.top[i], q = s.query[i];
+        const bool ask = top < INT32_MIN + (1 << 20);
+        int32_t* row = scores + (uint64_t)i * sc.pitch;
+        uint64_t sum = 0;
+        uint32_t first = UINT32_MAX;
+        if (q >= 0) {
+          for (uint32_t t = 4 * lane; t < padded; t += 128) {
+            const int4 x = __ldcg((const int4*)(row + t));
+            const int32_t v[4] = {x.x, x.y, x.z, x.w};
+            uint32_t e[4];
+#pragma unroll
+            for (uint32_t u = 0; u < 4; ++u) {
+              const uint32_t d = (uint32_t)top - (uint32_t)v[u];
+              e[u] = 0;
+              if (d < kExpTerms) {
+                if (d >= kExpExactBelow) {
+                  e[u] = term_by_table(d, bits);
+                } else {
+                  const uint32_t key = k0 + t + u;
+                  e[u] = d ? exp_term_near(d) : kTermTop;
+                  if (ask && (key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window))) e[u] = 0;
+                  else if (!d) first = min(first, t + u);
+                  sum += e[u] == kTermTop;  // 2^32
+                }
+                sum += e[u];
+              }
+            }
+            __stcg((uint4*)(row + t), make_uint4(e[0], e[1], e[2], e[3]));
+          }
+        }
+        sum = (uint64_t)warp_sum_i64((int64_t)sum);
+        first = __reduce_min_sync(0xffffffffu, first);
+        __syncwarp();
+        if (lane == 0) {
+          s.sum[i] = sum;
+          s.recip[i] = sum_recip(sum);
+          s.first[i] = first;
+          if (q >= 0 && first < padded) row[first] = 0;  // its weight comes last
+        }
+      }
+      epi_sync();
+      // 3. weights: eight keys of a row a thread, two rows' worth a tile
+      int32_t all[2] = {};
+      for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
+        const uint32_t buf = n_w & 1, use = n_w >> 1;
+        if (use > 0 && !pt_wait(&s.w_empty[buf], (use - 1) & 1, s, fault)) {
+          ok = false;
+          break;
+        }
+        uint8_t* wb = ops + buf * kPtWBuf;
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          const uint32_t i = (tid >> 4) + 32 * h, c = tid & 15;
+          const int32_t* e = scores + (uint64_t)i * sc.pitch + kt * kPtKeys + 8 * c;
+          const uint4 x0 = __ldcg((const uint4*)e), x1 = __ldcg((const uint4*)(e + 4));
+          const uint32_t term[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
+          const uint32_t recip = s.recip[i];
+          const uint64_t sum = s.sum[i];
+          int32_t w[8];
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) {
+            w[j] = weight_of(term[j], recip, sum);
+            all[h] += w[j];
+          }
+          const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
+          const uint32_t u0 = __byte_perm(w[4], w[5], 0x5140), u1 = __byte_perm(w[6], w[7], 0x5140);
+          // 128-byte rows in the 128-byte swizzle: 16-byte pieces exchanged by the row's low bits
+          uint8_t* dst = wb + i * 128 + (((c >> 1) ^ (i & 7)) << 4) + (c & 1) * 8;
+          *(uint2*)dst = make_uint2(__byte_perm(t0, t1, 0x5410), __byte_perm(u0, u1, 0x5410));
+          *(uint2*)(dst + kPtQPlane) = make_uint2(__byte_perm(t0, t1, 0x7632), __byte_perm(u0, u1, 0x7632));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.w_full[buf]);
+      }
+#pragma unroll
+      for (uint32_t h = 0; h < 2; ++h) {
+        int32_t x = all[h];
+#pragma unroll
+        for (uint32_t o = 1; o <= 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if ((lane & 15) == 0) s.wsum[(tid >> 4) + 32 * h] = x;
+      }
+      epi_sync();
+      if (ok && pt_wait(&s.v_done, n_item & 1, s, fault)) {
+        tc_fence_after();
+        uint32_t v[4][16];
+#pragma unroll
+        for (uint32_t d = 0; d < 4; ++d) {
+          tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16, v[d]);
+          tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16 + 8, v[d] + 8);
+        }
+        tmem_ld_wait();
+        const uint32_t x = 32 * quad + lane;
+#pragma unroll
+        for (uint32_t c = 0; c < 16; ++c) {
+          const uint32_t i = cg * 16 + c;
+          if (i < rows) {
+            const int32_t y[4] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c]};
+            int64_t total = diagonal_sum(y);
+            mac_wide(total, sub_sat(kOneAct, s.wsum[i]), a.v[(uint64_t)(k0 + s.first[i]) * a.v_stride + g * kPtD + x]);
+            a.out[(uint64_t)(begin + s.query[i]) * a.out_stride + (g * group + (f0 + i) % group) * kPtD + x] =
+                requantize(total);
+          }
+        }
+      } else {
+        ok = false;
+      }
+      tc_fence_before();
+    }
+    __syncwarp();
+  }
+  // every issued copy has landed before the block exits
+  if (warp == kPtEpiWarps && lane == 0)
+    for (uint32_t i = 0; i < kPtSlots; ++i)
+      if (issued[i]) mbar_wait_bounded(&s.full[i], (issued[i] - 1) & 1, fault);
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kPtEpiWarps) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+}  // namespace
+
+bool prompt_tc_usable(const IrisPromptAttention& a) {
+  return a.head_dim == kPtD && a.longest <= kPvKeys && a.tokens >= kPtKeys && (uint64_t)a.tokens * (a.heads / a.kv_heads) < 0x7FFFFFFFull &&
+         (uint64_t)a.kv_heads * 3 < 0x7FFFFFFFull && tensor_map_encoder() != nullptr && device_fault_word() != nullptr;
+}
+
+size_t prompt_tc_carve(const IrisPromptAttention& a, uint8_t* base, PromptTcScratch* sc) {
+  const uint64_t group = a.heads / a.kv_heads;
+  sc->tpitch = (a.tokens + 127) / 128 * 128;
+  sc->pack_blocks = 148 * 4;
+  sc->flags = 4 * sc->pack_blocks;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    uint8_t* p = base + at;
+    at += (bytes + 255) / 256 * 256;
+    return p;
+  };
+  sc->qp = take((size_t)a.kv_heads * 3 * a.tokens * group * kPtD);
+  sc->kp = take((size_t)a.kv_heads * 3 * a.tokens * kPtD);
+  sc->vt = take((size_t)a.kv_heads * 3 * kPtD * sc->tpitch);
+  sc->exp_bits = (uint32_t*)take((size_t)kPtTable * 4);
+  sc->wide = (uint32_t*)take((size_t)sc->flags * 4);
+  return at;
+}
+
+cudaError_t launch_prompt_tc(const IrisPromptAttention& a, const PromptTcScratch& sc, uint32_t blocks,
+                             cudaStream_t stream) {
+  const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads);
+  CUtensorMap qmap, kmap, vmap;
+  if (!make_map(&qmap, sc.qp, kPtD, rows, (uint64_t)a.kv_heads * 3, kPtD, rows * kPtD, kPtRows, 1) ||
+      !make_map(&kmap, sc.kp, kPtD, a.tokens, (uint64_t)a.kv_heads * 3, kPtD, (uint64_t)a.tokens * kPtD, kPtKeys, 1) ||
+      !make_map(&vmap, sc.vt, sc.tpitch, kPtD, (uint64_t)a.kv_heads * 3, sc.tpitch, (uint64_t)kPtD * sc.tpitch, kPtD, 1))
+    return cudaErrorInvalidValue;
+  cudaError_t e = cudaFuncSetAttribute(prompt_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPtSmem);
+  if (e != cudaSuccess) return e;
+  e = launch_k(prompt_pack_kernel, dim3(sc.pack_blocks, 4), dim3(kPackThreads), 0, stream, a, sc);
+  if (e != cudaSuccess) return e;
+  return launch_k(prompt_tc_kernel, dim3(blocks), dim3(kPtThreads), kPtSmem, stream, a, sc, qmap, kmap, vmap,
+                  device_fault_word());
+}
+
+}  // namespace iris

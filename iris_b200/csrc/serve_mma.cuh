@@ -140,9 +140,15 @@ __device__ __forceinline__ int32_t score_of(int32_t hi, uint32_t lo, uint32_t sc
   return clamp_i32((s + 0x7FFF + ((s >> 16) & 1)) >> 16);
 }
 // Five diagonals: carried byte by byte, the low 32 bits from the bytes left behind.
+__device__ __forceinline__ void carry_diagonals(const int32_t (&v)[5], int32_t* hi, uint32_t* lo) {
+  const int32_t y = v[1] + (v[0] >> 8), z = v[2] + (y >> 8), u = v[3] + (z >> 8);
+  *hi = v[4] + (u >> 8);
+  *lo = __byte_perm(__byte_perm(v[0], y, 0x0040), __byte_perm(z, u, 0x0040), 0x5410);
+}
 __device__ __forceinline__ int32_t diagonal_score(const int32_t (&v)[5], uint32_t scale) {
-  const int32_t y = v[1] + (v[0] >> 8), z = v[2] + (y >> 8), u = v[3] + (z >> 8), hi = v[4] + (u >> 8);
-  const uint32_t lo = __byte_perm(__byte_perm(v[0], y, 0x0040), __byte_perm(z, u, 0x0040), 0x5410);
+  int32_t hi;
+  uint32_t lo;
+  carry_diagonals(v, &hi, &lo);
   return score_of(hi, lo, scale);
 }
 // Seven: the sum wraps at 64 bits, as the definition's does.

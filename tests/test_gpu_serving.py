@@ -66,6 +66,14 @@ PROMPTS = [
     ([300], 4, 1, 128, True, 0, "zero"),        # all scores equal
     ([1100], 1, 1, 64, True, 0, "equal"),
     ([0, 700, 30], 2, 1, 128, True, 1, "model"),  # a window of one: every row sees itself only
+    # heads of 128 values in requests of 256 rows or more
+    ([257, 3, 130], 4, 1, 128, True, 0, "model"),
+    ([300, 31], 2, 2, 128, False, 0, "model"),
+    ([290], 8, 1, 128, True, 100, "model"),
+    ([400, 17, 0, 64], 3, 1, 128, True, 33, "model"),
+    ([270], 2, 1, 128, True, 0, "wide"),
+    ([270, 5], 2, 1, 128, False, 0, "full"),
+    ([900], 1, 1, 128, True, 0, "equal"),
 ]
 
 
