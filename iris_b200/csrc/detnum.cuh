@@ -435,11 +435,22 @@ IRIS_HD int32_t scaled_score_finish(int64_t sum, uint32_t scale_q32) {
 
 // softmax_exp_term (ops.rs:508-556) of the Q16.16 distance d below the maximum,
 // 1 <= d < 2^20 (from 2^20 = 16.0 on the term is 0; at 0 it is 2^32): the same
-// value as softmax_exp_term_act in 32-bit halves. k = floor(d 2^16 / ln2) from
-// one product (no d in the range comes nearer to a multiple of ln2 than the
-// product's error), r = d 2^16 - k ln2 below 2^32; each power is the high word
-// of a product, rounded half to even by one addition; each quotient by n is
-// floor((x + n/2) / n), one less where that is an odd tie.
+// value as softmax_exp_term_act in 32-bit halves. k = floor(d 2^16 / ln2), r = d
+// 2^16 - k ln2 below 2^32; each power is the high word of a product, rounded
+// half to even by one addition; each quotient by n is floor((x + n/2) / n), one
+// less where that is an odd tie.
+//
+// k by one float multiply-add rounded down: the integer lands in the low bits
+// of 1.5 2^23. No d in the range comes nearer to a multiple of ln2 than the
+// factor's error (the host test checks every one).
+IRIS_HD uint32_t exp_term_turns(uint32_t d) {
+  const float turn = 2.2013779e-5f;  // 1 / ln2 in Q16.16
+#if defined(__CUDA_ARCH__)
+  return __float_as_uint(__fmaf_rd((float)d, turn, 12582912.0f)) - 0x4B400000u;
+#else
+  return (uint32_t)((double)d * (double)turn);  // exact: 20 by 24 bits
+#endif
+}
 IRIS_HD uint32_t exp_term_power(uint32_t a, uint32_t r) {
   const uint64_t p = (uint64_t)a * r;
   return (uint32_t)((p + 0x7FFFFFFFu + ((uint32_t)(p >> 32) & 1)) >> 32);
@@ -450,8 +461,7 @@ IRIS_HD uint32_t exp_term_over(uint32_t x) {
   return q - (q * N == s ? q & 1 : 0);
 }
 IRIS_HD uint32_t exp_term_near(uint32_t d) {
-  // 2^52 / (ln2 in Q16.16 * 2^11), ln2 = 2977044472 / 2^32
-  const uint32_t k = (uint32_t)(((uint64_t)(d << 11) * 48408813u) >> 52);
+  const uint32_t k = exp_term_turns(d);
   const uint32_t r = (d << 16) - k * 2977044472u;
   const uint32_t r2 = exp_term_power(r, r), r3 = exp_term_power(r2, r), r4 = exp_term_power(r3, r),
                  r5 = exp_term_power(r4, r);
@@ -468,7 +478,7 @@ IRIS_HD uint32_t exp_term_near(uint32_t d) {
 // distance makes it exact; the host test checks every distance.
 static constexpr uint32_t kExpExactBelow = 136278;  // ceil(3 ln2 in Q16.16)
 IRIS_HD uint32_t exp_term_estimate(uint32_t d) {
-  const uint32_t k = (uint32_t)(((uint64_t)(d << 11) * 48408813u) >> 52);
+  const uint32_t k = exp_term_turns(d);
   const uint32_t r = (d << 16) - k * 2977044472u;
   uint32_t a = 178956971u - mulhi_u32(r, 35791394u);  // 2^32 / 24, 2^32 / 120
   a = 715827883u - mulhi_u32(r, a);                   // 2^32 / 6

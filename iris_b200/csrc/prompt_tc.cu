@@ -8,9 +8,10 @@
 // [token][128], values transposed [head][plane][128][token]. A tile of 64 query
 // rows that share a K/V head goes through
 //   1. scores: 128 keys x 64 rows x 32 dims a product, nine plane pairs into
-//      five int32 diagonals of 64 TMEM columns; the epilogue warps carry the
-//      diagonals together, release them to the next tile's products and write
-//      the scores to the block's scratch (L2) while those run;
+//      five int32 diagonals of 64 TMEM columns (five of eight column groups,
+//      taken in turn); the epilogue warps carry the diagonals together, release
+//      them and write the scores to the block's scratch (L2) while the next
+//      tile's products run;
 //   2. terms in place, a row a warp; an exponential is its polynomial in
 //      truncated 32-bit products plus one bit of a table in shared memory that
 //      makes it exact (exp_term_estimate);
@@ -46,7 +47,7 @@ constexpr uint32_t kPtRing = kPtSlots * kPtSlot;
 constexpr uint32_t kPtOperands = 2 * kPtWBuf;  // the query planes (3 x 8 KB), later two weight buffers
 constexpr uint32_t kPtSmem = 1024 + kPtRing + kPtOperands + kPtTable * 4;
 static_assert(3 * kPtQPlane <= kPtOperands, "query planes");
-static_assert(5 * kPtRows <= 512, "TMEM columns");
+static_assert(8 * kPtRows == 512, "TMEM column groups");
 
 // ---- packing -------------------------------------------------------------------
 
@@ -145,10 +146,21 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, PtShared
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
 
-// exp_term_near by the estimate and its correction bit.
-__device__ __forceinline__ uint32_t term_by_table(uint32_t d, const uint32_t* bits) {
-  const uint32_t word = bits[(d >> 5) - kExpExactBelow / 32];
-  return exp_term_estimate(d) + (__funnelshift_r(word, 0, d) & 1);
+// The terms of four scores; true where one lies nearer to the maximum than the
+// table covers (kExpExactBelow), its entry then to be replaced.
+__device__ __forceinline__ bool terms_by_table(const int4& x, int32_t top, const uint32_t* bits, uint32_t (&e)[4]) {
+  const int32_t v[4] = {x.x, x.y, x.z, x.w};
+  uint32_t near = UINT32_MAX;
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    const uint32_t d = (uint32_t)top - (uint32_t)v[u];
+    near = min(near, d);
+    const uint32_t c = min(max(d, kExpExactBelow), kExpTerms - 1);
+    const uint32_t word = bits[(c >> 5) - kExpExactBelow / 32];
+    const uint32_t t = exp_term_estimate(c) + (__funnelshift_r(word, 0, c) & 1);
+    e[u] = d < kExpTerms ? t : 0;
+  }
+  return near < kExpExactBelow;
 }
 
 __global__ void __launch_bounds__(kPtThreads, 1)
@@ -246,34 +258,42 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         ok = ok && pt_wait(&s.q_full, n_item & 1, s, fault);
         const uint32_t ops_a = smem_addr(ops);
         tc_fence_after();
-        for (uint32_t kt = 0; kt < ktiles && ok; ++kt) {
-          if (kt && !pt_wait(&s.t_free, (n_s - 1) & 1, s, fault)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t touched = 0;
+        for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
+          // diagonal d of the n-th score tile lies in column group (5 n + d) % 8:
+          // the first three diagonals take groups that the tile before does
+          // not use, so six of the nine plane pairs run while it is read
+          uint32_t base[3], touched = 0;
+          auto pairs = [&](uint32_t i, uint32_t j) {
 #pragma unroll
-          for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
-            const uint32_t slot = ring_n % kPtSlots;
-            if (!ok || !pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault)) {
+            for (uint32_t kk = 0; kk < 4; ++kk) {
+              tc_mma(tmem + ((5 * n_s + i + j) & 7) * kPtRows, tc_desc(base[i] + kk * 32),
+                     tc_desc(ops_a + j * kPtQPlane + kk * 32), tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
+              touched |= 1u << (i + j);
+            }
+          };
+#pragma unroll
+          for (uint32_t i = 0; i < 3; ++i) {
+            const uint32_t n = ring_n + i, slot = n % kPtSlots;
+            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t base = smem_addr(ring + slot * kPtSlot);
+            base[i] = smem_addr(ring + slot * kPtSlot);
 #pragma unroll
-            for (uint32_t kk = 0; kk < 4; ++kk)
-#pragma unroll
-              for (uint32_t j = 0; j < 3; ++j) {
-                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base + kk * 32), tc_desc(ops_a + j * kPtQPlane + kk * 32),
-                       tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
-                touched |= 1u << (i + j);
-              }
-            tc_commit(&s.empty[slot]);
+            for (uint32_t j = 0; i + j < 3; ++j) pairs(i, j);
+            if (i == 0) tc_commit(&s.empty[slot]);
           }
-          if (ok) tc_commit(&s.s_done);
-          ++n_s;
+          if (ok && kt) ok = pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+          if (!ok) break;
+          tc_fence_after();
+          pairs(1, 2);
+          tc_commit(&s.empty[(ring_n + 1) % kPtSlots]);
+          pairs(2, 1);
+          pairs(2, 2);
+          tc_commit(&s.empty[(ring_n + 2) % kPtSlots]);
+          tc_commit(&s.s_done);
+          ring_n += 3;
         }
         // the diagonals of the last score tile are read before the value sums take their columns
         ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
@@ -335,7 +355,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (uint32_t h = 0; h < 2; ++h) {
           uint32_t v[5][8];
 #pragma unroll
-          for (uint32_t d = 0; d < 5; ++d) tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16 + h * 8, v[d]);
+          for (uint32_t d = 0; d < 5; ++d)
+            tmem_ld8(tmem + ((32 * quad) << 16) + ((5 * n_s + d) & 7) * kPtRows + cg * 16 + h * 8, v[d]);
           tmem_ld_wait();
 #pragma unroll
           for (uint32_t c = 0; c < 8; ++c) {
@@ -378,28 +399,38 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         uint64_t sum = 0;
         uint32_t first = UINT32_MAX;
         if (q >= 0) {
-          for (uint32_t t = 4 * lane; t < padded; t += 128) {
-            const int4 x = __ldcg((const int4*)(row + t));
-            const int32_t v[4] = {x.x, x.y, x.z, x.w};
-            uint32_t e[4];
+          // eight scores a lane and turn, the next eight loaded ahead
+          const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+          int4 x[2], y[2] = {hidden, hidden};
+          auto load = [&](int4 (&z)[2], uint32_t t) {
 #pragma unroll
-            for (uint32_t u = 0; u < 4; ++u) {
-              const uint32_t d = (uint32_t)top - (uint32_t)v[u];
-              e[u] = 0;
-              if (d < kExpTerms) {
-                if (d >= kExpExactBelow) {
-                  e[u] = term_by_table(d, bits);
-                } else {
-                  const uint32_t key = k0 + t + u;
-                  e[u] = d ? exp_term_near(d) : kTermTop;
-                  if (ask && (key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window))) e[u] = 0;
-                  else if (!d) first = min(first, t + u);
-                  sum += e[u] == kTermTop;  // 2^32
+            for (uint32_t m = 0; m < 2; ++m) z[m] = t + 128 * m < padded ? __ldcg((const int4*)(row + t + 128 * m)) : hidden;
+          };
+          load(x, 4 * lane);
+          for (uint32_t t = 4 * lane; t < padded; t += 256) {
+            if (t + 256 < padded) load(y, t + 256);
+#pragma unroll
+            for (uint32_t m = 0; m < 2; ++m) {
+              uint32_t e[4];
+              if (terms_by_table(x[m], top, bits, e) || ask) {
+                const int32_t v[4] = {x[m].x, x[m].y, x[m].z, x[m].w};
+#pragma unroll 1
+                for (uint32_t u = 0; u < 4; ++u) {
+                  const uint32_t d = (uint32_t)top - (uint32_t)v[u], at = t + 128 * m + u, key = k0 + at;
+                  const bool gone = ask && (key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window));
+                  if (d >= kExpExactBelow && !gone) continue;
+                  const uint32_t z = gone ? 0 : d ? exp_term_near(d) : kTermTop;
+                  if (z == kTermTop) first = min(first, at);
+                  sum += z == kTermTop;  // 2^32
+#pragma unroll
+                  for (uint32_t o = 0; o < 4; ++o)
+                    if (o == u) e[o] = z;
                 }
-                sum += e[u];
               }
+              sum += (uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3]);
+              if (t + 128 * m < padded) __stcg((uint4*)(row + t + 128 * m), make_uint4(e[0], e[1], e[2], e[3]));
+              x[m] = y[m];
             }
-            __stcg((uint4*)(row + t), make_uint4(e[0], e[1], e[2], e[3]));
           }
         }
         sum = (uint64_t)warp_sum_i64((int64_t)sum);
@@ -415,6 +446,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       epi_sync();
       // 3. weights: eight keys of a row a thread, two rows' worth a tile
       int32_t all[2] = {};
+      uint4 next[2][2];
+      auto load_terms = [&](uint32_t kt) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+          const int32_t* e = scores + (uint64_t)((tid >> 4) + 32 * h) * sc.pitch + kt * kPtKeys + 8 * (tid & 15);
+          next[h][0] = __ldcg((const uint4*)e);
+          next[h][1] = __ldcg((const uint4*)(e + 4));
+        }
+      };
+      load_terms(0);
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
         const uint32_t buf = n_w & 1, use = n_w >> 1;
         if (use > 0 && !pt_wait(&s.w_empty[buf], (use - 1) & 1, s, fault)) {
@@ -422,11 +463,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           break;
         }
         uint8_t* wb = ops + buf * kPtWBuf;
+        uint4 now[2][2];
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) now[h][0] = next[h][0], now[h][1] = next[h][1];
+        if (kt + 1 < ktiles) load_terms(kt + 1);
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
           const uint32_t i = (tid >> 4) + 32 * h, c = tid & 15;
-          const int32_t* e = scores + (uint64_t)i * sc.pitch + kt * kPtKeys + 8 * c;
-          const uint4 x0 = __ldcg((const uint4*)e), x1 = __ldcg((const uint4*)(e + 4));
+          const uint4 x0 = now[h][0], x1 = now[h][1];
           const uint32_t term[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
           const uint32_t recip = s.recip[i];
           const uint64_t sum = s.sum[i];
@@ -454,6 +498,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (uint32_t o = 1; o <= 8; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
         if ((lane & 15) == 0) s.wsum[(tid >> 4) + 32 * h] = x;
       }
+      // the first maxima's values, ahead of the last products
+      int32_t vf[16];
+#pragma unroll
+      for (uint32_t c = 0; c < 16; ++c)
+        vf[c] = cg * 16 + c < rows
+                    ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * kPtD + 32 * quad + lane]
+                    : 0;
       epi_sync();
       if (ok && pt_wait(&s.v_done, n_item & 1, s, fault)) {
         tc_fence_after();
@@ -471,7 +522,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           if (i < rows) {
             const int32_t y[4] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c]};
             int64_t total = diagonal_sum(y);
-            mac_wide(total, sub_sat(kOneAct, s.wsum[i]), a.v[(uint64_t)(k0 + s.first[i]) * a.v_stride + g * kPtD + x]);
+            mac_wide(total, sub_sat(kOneAct, s.wsum[i]), vf[c]);
             a.out[(uint64_t)(begin + s.query[i]) * a.out_stride + (g * group + (f0 + i) % group) * kPtD + x] =
                 requantize(total);
           }

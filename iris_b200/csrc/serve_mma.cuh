@@ -133,11 +133,16 @@ __device__ __forceinline__ uint32_t key_products(const int32_t* k0, const int32_
   return wide;
 }
 
-// The score of a sum hi 2^32 + lo (serve_score), scale below 2^31.
+// The score of a sum hi 2^32 + lo (serve_score), scale below 2^31: the sum
+// times the scale down 32 bits, then down 16 to nearest even (one addition, as
+// in mul_sat), saturated where the high word is past 16 bits.
 __device__ __forceinline__ int32_t score_of(int32_t hi, uint32_t lo, uint32_t scale) {
-  int64_t s = (int64_t)(((uint64_t)(uint32_t)hi << 32) | lo);
-  if (scale) s = (int64_t)hi * (int32_t)scale + (int64_t)(((uint64_t)lo * scale) >> 32);
-  return clamp_i32((s + 0x7FFF + ((s >> 16) & 1)) >> 16);
+  uint64_t s = ((uint64_t)(uint32_t)hi << 32) | lo;
+  if (scale) s = (uint64_t)((int64_t)hi * (int32_t)scale) + __umulhi(lo, scale);
+  s += 0x7FFF + (((uint32_t)s >> 16) & 1);
+  const int32_t top = (int32_t)(s >> 32);
+  const int32_t low = (int32_t)__funnelshift_r((uint32_t)s, (uint32_t)top, 16);
+  return (uint32_t)(top + 0x8000) < 0x10000u ? low : (top >> 31) ^ INT32_MAX;
 }
 // Five diagonals: carried byte by byte, the low 32 bits from the bytes left behind.
 __device__ __forceinline__ void carry_diagonals(const int32_t (&v)[5], int32_t* hi, uint32_t* lo) {

@@ -1,0 +1,15 @@
+// The serving kernels' exponential (iris_b200/csrc/detnum.cuh) as host code.
+#include "../../iris_b200/csrc/detnum.cuh"
+
+extern "C" {
+// term[d] = exp_term_near(d), estimate[d] = exp_term_estimate(d) and want[d] =
+// softmax_exp_term_act of a score d below the maximum, for 1 <= d < 2^20.
+void serving_exp_terms(uint32_t* term, uint32_t* estimate, int64_t* want) {
+  for (uint32_t d = 1; d < 1u << 20; ++d) {
+    term[d] = iris::exp_term_near(d);
+    estimate[d] = d >= iris::kExpExactBelow ? iris::exp_term_estimate(d) : 0;
+    want[d] = iris::softmax_exp_term_act(-(int32_t)d, 0);
+  }
+}
+uint32_t serving_exact_below() { return iris::kExpExactBelow; }
+}

@@ -91,6 +91,31 @@ def test_prompt_attention_equals_the_definition(S, lengths, heads, kv_heads, d, 
     assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, scale, window))
 
 
+@pytest.mark.parametrize("heads,kv_heads,d,step", [(4, 1, 128, 61), (2, 2, 64, 61), (2, 1, 36, 61), (4, 2, 128, 1)])
+def test_scores_at_the_lowest_value(S, heads, kv_heads, d, step):
+    """Every score within 16.0 of the lowest one, or saturated at it: what a row
+    does not see must not be told by a low score."""
+    rng = np.random.default_rng(d + step)
+    lengths = [300, 40]
+    n = sum(lengths)
+    unit = -(1 << 31) // (d << 22 >> 16)  # a key value whose score is about -2^31 against queries of 2^22
+    q = np.full((n, heads * d), 1 << 22, np.int32)
+    k = np.full((n, kv_heads * d), unit + step, np.int32)
+    k[rng.random(n) < 0.3] += 9 if step > 1 else -3  # with a step of 1 some fall below the lowest score
+    v = values(rng, (n, kv_heads * d), "model")
+    offsets = np.array([0, 300, 340], np.int32)
+    for window in (0, 50):
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 300, heads=heads, kv_heads=kv_heads,
+                                 window=window).cpu().numpy()
+        assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, 0, window))
+    x = tree_inputs(rng, [150, 0], [9, 5], heads, kv_heads, d, 16, "model", holes=[(0, 3, -1)])
+    x["q"][:] = 1 << 22
+    x["k_pages"][:] = unit + step
+    x["k_pages"][::3] += 9 if step > 1 else -3
+    x["masks"][12] = 0
+    check_tree(S, x, heads, kv_heads, 0, 0, [9, 5])
+
+
 def test_prompt_attention_over_parts_of_fused_rows_and_a_strided_output(S):
     import torch
     rng = np.random.default_rng(3)
