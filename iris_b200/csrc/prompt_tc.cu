@@ -45,6 +45,11 @@ constexpr uint32_t kPtWBuf = 2 * kPtQPlane;                 // two weight planes
 constexpr uint32_t kPtTable = (kExpTerms - kExpExactBelow / 32 * 32) / 32;  // words
 constexpr uint32_t kPtRing = kPtSlots * kPtSlot;
 constexpr uint32_t kPtOperands = 2 * kPtWBuf;  // the query planes (3 x 8 KB), later two weight buffers
+constexpr uint32_t kPtList = kPtOperands / 4 / kPtEpiWarps;  // words of a warp's list of near scores
+constexpr uint32_t kPtNearBits = 18;                         // kExpExactBelow below 2^18, places below 2^14
+constexpr uint32_t kPtLongest = (1u << (32 - kPtNearBits)) - kPtKeys;
+static_assert(kExpExactBelow < 1u << kPtNearBits && kPtList >= 512, "list entries");
+static_assert(kPtLongest + 15 + kPtKeys <= kPvKeys + kPtKeys, "int32 diagonals of the value sums");
 constexpr uint32_t kPtSmem = 1024 + kPtRing + kPtOperands + kPtTable * 4;
 static_assert(3 * kPtQPlane <= kPtOperands, "query planes");
 static_assert(8 * kPtRows == 512, "TMEM column groups");
@@ -146,21 +151,19 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, PtShared
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
 
-// The terms of four scores; true where one lies nearer to the maximum than the
-// table covers (kExpExactBelow), its entry then to be replaced.
-__device__ __forceinline__ bool terms_by_table(const int4& x, int32_t top, const uint32_t* bits, uint32_t (&e)[4]) {
+// The terms of four scores and their distances below the maximum, good from
+// kExpExactBelow on.
+__device__ __forceinline__ void terms_by_table(const int4& x, int32_t top, const uint32_t* bits, uint32_t (&e)[4],
+                                               uint32_t (&d)[4]) {
   const int32_t v[4] = {x.x, x.y, x.z, x.w};
-  uint32_t near = UINT32_MAX;
 #pragma unroll
   for (uint32_t u = 0; u < 4; ++u) {
-    const uint32_t d = (uint32_t)top - (uint32_t)v[u];
-    near = min(near, d);
-    const uint32_t c = min(max(d, kExpExactBelow), kExpTerms - 1);
+    d[u] = (uint32_t)top - (uint32_t)v[u];
+    const uint32_t c = min(max(d[u], kExpExactBelow), kExpTerms - 1);
     const uint32_t word = bits[(c >> 5) - kExpExactBelow / 32];
     const uint32_t t = exp_term_estimate(c) + (__funnelshift_r(word, 0, c) & 1);
-    e[u] = d < kExpTerms ? t : 0;
+    e[u] = d[u] < kExpTerms ? t : 0;
   }
-  return near < kExpExactBelow;
 }
 
 __global__ void __launch_bounds__(kPtThreads, 1)
@@ -262,35 +265,48 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           // diagonal d of the n-th score tile lies in column group (5 n + d) % 8:
           // the first three diagonals take groups that the tile before does
           // not use, so six of the nine plane pairs run while it is read
+          // (a step's products go to different diagonals in turn, so that
+          // none waits for the one before it)
           uint32_t base[3], touched = 0;
-          auto pairs = [&](uint32_t i, uint32_t j) {
-#pragma unroll
-            for (uint32_t kk = 0; kk < 4; ++kk) {
-              tc_mma(tmem + ((5 * n_s + i + j) & 7) * kPtRows, tc_desc(base[i] + kk * 32),
-                     tc_desc(ops_a + j * kPtQPlane + kk * 32), tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
-              touched |= 1u << (i + j);
-            }
+          auto product = [&](uint32_t i, uint32_t j, uint32_t kk) {
+            tc_mma(tmem + ((5 * n_s + i + j) & 7) * kPtRows, tc_desc(base[i] + kk * 32),
+                   tc_desc(ops_a + j * kPtQPlane + kk * 32), tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
+            touched |= 1u << (i + j);
           };
-#pragma unroll
-          for (uint32_t i = 0; i < 3; ++i) {
+          auto plane = [&](uint32_t i) {
             const uint32_t n = ring_n + i, slot = n % kPtSlots;
-            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) {
-              ok = false;
-              break;
-            }
+            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) ok = false;
             tc_fence_after();
             base[i] = smem_addr(ring + slot * kPtSlot);
+          };
+          plane(0);
+          if (!ok) break;
 #pragma unroll
-            for (uint32_t j = 0; i + j < 3; ++j) pairs(i, j);
-            if (i == 0) tc_commit(&s.empty[slot]);
+          for (uint32_t kk = 0; kk < 4; ++kk) {
+            product(0, 2, kk);
+            product(0, 1, kk);
+            product(0, 0, kk);
           }
-          if (ok && kt) ok = pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+          tc_commit(&s.empty[ring_n % kPtSlots]);
+          plane(1);
+          plane(2);
+          if (!ok) break;
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; ++kk) {
+            product(1, 1, kk);
+            product(1, 0, kk);
+            product(2, 0, kk);
+          }
+          if (kt) ok = pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
           if (!ok) break;
           tc_fence_after();
-          pairs(1, 2);
+#pragma unroll
+          for (uint32_t kk = 0; kk < 4; ++kk) {
+            product(1, 2, kk);
+            product(2, 2, kk);
+            product(2, 1, kk);
+          }
           tc_commit(&s.empty[(ring_n + 1) % kPtSlots]);
-          pairs(2, 1);
-          pairs(2, 2);
           tc_commit(&s.empty[(ring_n + 2) % kPtSlots]);
           tc_commit(&s.s_done);
           ring_n += 3;
@@ -306,26 +322,29 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             break;
           }
           tc_fence_after();
+          uint32_t base[3];
 #pragma unroll
-          for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
-            const uint32_t slot = ring_n % kPtSlots;
-            if (!ok || !pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t base = smem_addr(ring + slot * kPtSlot);
+          for (uint32_t i = 0; i < 3; ++i) {
+            const uint32_t n = ring_n + i, slot = n % kPtSlots;
+            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) ok = false;
+            base[i] = smem_addr(ring + slot * kPtSlot);
+          }
+          if (!ok) break;
+          tc_fence_after();
 #pragma unroll
-            for (uint32_t kk = 0; kk < 4; ++kk)
+          for (uint32_t kk = 0; kk < 4; ++kk)
 #pragma unroll
-              for (uint32_t j = 0; j < 2; ++j) {
-                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base + kk * 32),
+            for (uint32_t j = 0; j < 2; ++j)
+#pragma unroll
+              for (uint32_t i = 0; i < 3; ++i) {
+                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base[i] + kk * 32),
                        tc_desc(ops_a + buf * kPtWBuf + j * kPtQPlane + kk * 32), tc_idesc(i == 2, false),
                        (touched >> (i + j)) & 1u);
                 touched |= 1u << (i + j);
               }
-            tc_commit(&s.empty[slot]);
-          }
+#pragma unroll
+          for (uint32_t i = 0; i < 3; ++i) tc_commit(&s.empty[(ring_n + i) % kPtSlots]);
+          ring_n += 3;
           if (ok) tc_commit(&s.w_empty[buf]);
         }
         if (ok) tc_commit(&s.v_done);
@@ -392,45 +411,70 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       epi_sync();
       // 2. terms in place, a row a warp (hidden keys: see prompt_mma.cu)
       const uint32_t padded = ktiles * kPtKeys;
+      uint32_t* list = (uint32_t*)ops + warp * kPtList;  // (the query planes are done with)
       for (uint32_t i = warp; i < kPtRows; i += kPtEpiWarps) {
         const int32_t top = s.top[i], q = s.query[i];
         const bool ask = top < INT32_MIN + (1 << 20);
         int32_t* row = scores + (uint64_t)i * sc.pitch;
         uint64_t sum = 0;
         uint32_t first = UINT32_MAX;
-        if (q >= 0) {
-          // eight scores a lane and turn, the next eight loaded ahead
+        if (q >= 0 && !ask) {
+          // eight scores a lane and turn, the next eight loaded ahead; those
+          // nearer to the maximum than the table goes are put on a list (place
+          // and distance in one word) and done 32 at a time, exactly
           const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
           int4 x[2], y[2] = {hidden, hidden};
+          uint32_t listed = 0;
           auto load = [&](int4 (&z)[2], uint32_t t) {
 #pragma unroll
             for (uint32_t m = 0; m < 2; ++m) z[m] = t + 128 * m < padded ? __ldcg((const int4*)(row + t + 128 * m)) : hidden;
           };
+          auto drain = [&] {
+            __syncwarp();
+            for (uint32_t n = lane; n < listed; n += 32) {
+              const uint32_t at = list[n] >> kPtNearBits, d = list[n] & ((1u << kPtNearBits) - 1);
+              const uint32_t z = d ? exp_term_near(d) : kTermTop;
+              if (!d) first = min(first, at);
+              sum += kept_term(z);
+              __stcg((uint32_t*)(row + at), z);
+            }
+            listed = 0;
+            __syncwarp();
+          };
           load(x, 4 * lane);
-          for (uint32_t t = 4 * lane; t < padded; t += 256) {
+          for (uint32_t t = 4 * lane; t < padded + 4 * lane; t += 256) {
             if (t + 256 < padded) load(y, t + 256);
 #pragma unroll
             for (uint32_t m = 0; m < 2; ++m) {
-              uint32_t e[4];
-              if (terms_by_table(x[m], top, bits, e) || ask) {
-                const int32_t v[4] = {x[m].x, x[m].y, x[m].z, x[m].w};
-#pragma unroll 1
-                for (uint32_t u = 0; u < 4; ++u) {
-                  const uint32_t d = (uint32_t)top - (uint32_t)v[u], at = t + 128 * m + u, key = k0 + at;
-                  const bool gone = ask && (key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window));
-                  if (d >= kExpExactBelow && !gone) continue;
-                  const uint32_t z = gone ? 0 : d ? exp_term_near(d) : kTermTop;
-                  if (z == kTermTop) first = min(first, at);
-                  sum += z == kTermTop;  // 2^32
+              uint32_t e[4], d[4];
+              terms_by_table(x[m], top, bits, e, d);
+              if (__any_sync(0xffffffffu, min(min(d[0], d[1]), min(d[2], d[3])) < kExpExactBelow)) {
 #pragma unroll
-                  for (uint32_t o = 0; o < 4; ++o)
-                    if (o == u) e[o] = z;
+                for (uint32_t u = 0; u < 4; ++u) {
+                  const bool near = d[u] < kExpExactBelow;
+                  const uint32_t all = __ballot_sync(0xffffffffu, near);
+                  if (near) {
+                    list[listed + __popc(all & ((1u << lane) - 1))] = (t + 128 * m + u) << kPtNearBits | d[u];
+                    e[u] = 0;
+                  }
+                  listed += __popc(all);
                 }
               }
               sum += (uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3]);
               if (t + 128 * m < padded) __stcg((uint4*)(row + t + 128 * m), make_uint4(e[0], e[1], e[2], e[3]));
               x[m] = y[m];
             }
+            if (listed + 256 > kPtList) drain();
+          }
+          drain();
+        } else if (q >= 0) {
+          // every score within 16.0 of the lowest: hidden keys by their place
+          const uint32_t k1 = begin + (uint32_t)q, ks = begin + window_start((uint32_t)q, a.window);
+          for (uint32_t t = lane; t < padded; t += 32) {
+            const uint32_t z = k0 + t < ks || k0 + t > k1 ? 0 : term_of(row[t], top);
+            if (z == kTermTop) first = min(first, t);
+            sum += kept_term(z);
+            __stcg((uint32_t*)(row + t), z);
           }
         }
         sum = (uint64_t)warp_sum_i64((int64_t)sum);
@@ -549,7 +593,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 }  // namespace
 
 bool prompt_tc_usable(const IrisPromptAttention& a) {
-  return a.head_dim == kPtD && a.longest <= kPvKeys && a.tokens >= kPtKeys && (uint64_t)a.tokens * (a.heads / a.kv_heads) < 0x7FFFFFFFull &&
+  return a.head_dim == kPtD && a.longest <= kPtLongest && a.tokens >= kPtKeys && (uint64_t)a.tokens * (a.heads / a.kv_heads) < 0x7FFFFFFFull &&
          (uint64_t)a.kv_heads * 3 < 0x7FFFFFFFull && tensor_map_encoder() != nullptr && device_fault_word() != nullptr;
 }
 
