@@ -2,22 +2,24 @@
 //
 // The same three phases as prompt_mma.cu, with the contractions on the
 // fifth-generation tensor cores. Operands are packed once a call into K-major
-// byte planes (three: 24-bit values; where any operand is wider the kernel
+// byte planes (three signed digits: 24-bit values, nearly; where any operand is wider the kernel
 // leaves the call to prompt_mma_kernel, launched behind it, which then runs):
 // queries [K/V head][plane][token * group + head][128], keys [head][plane]
 // [token][128], values transposed [head][plane][128][token]. A tile of 64 query
 // rows that share a K/V head goes through
-//   1. scores: 128 keys x 64 rows x 32 dims a product, nine plane pairs into
-//      five int32 diagonals of 64 TMEM columns (five of eight column groups,
-//      taken in turn); the epilogue warps carry the diagonals together, release
-//      them and write the scores to the block's scratch (L2) while the next
-//      tile's products run;
+//   1. scores: 128 keys x 192 rows x 32 dims a product (one key plane against
+//      the three query planes side by side), nine plane pairs into five int32
+//      diagonals of 64 TMEM columns; the epilogue warps carry the diagonals
+//      together, release them and write the scores to the block's scratch (L2)
+//      while the next tile's products run;
 //   2. terms in place, a row a warp; an exponential is its polynomial in
 //      truncated 32-bit products plus one bit of a table in shared memory that
 //      makes it exact (exp_term_estimate);
 //   3. weights of 128 keys into shared memory as two swizzled byte planes, and
-//      128 dims x 64 rows x 32 positions a product, six plane pairs into four
-//      diagonals that stay in TMEM over all keys.
+//      128 dims x 128 rows (both weight planes) x 32 positions a product, six
+//      plane pairs into four diagonals that stay in TMEM over all keys.
+// Products of 64 rows each took 148 cycles, whatever their order: the wide ones
+// do three times the work in one.
 // Sixteen epilogue warps, one warp that feeds the ring (16 KB, one plane of 128
 // keys a slot) by TMA and one that issues the products. Every wait is bounded;
 // a give-up ends the block and is recorded in the fault word.
@@ -56,15 +58,25 @@ static_assert(8 * kPtRows == 512, "TMEM column groups");
 
 // ---- packing -------------------------------------------------------------------
 
+// Four values as signed base-256 digits, x = c0 + 2^8 c1 + 2^16 c2 with every
+// digit in [-128, 127]: the bytes of x + 0x808080, each less 128. p[3] is not 0
+// where a value is outside [-0x808080, 0x7F7F7F]. With all digits signed, one
+// product takes a plane against several others side by side.
+__device__ __forceinline__ void split_digits(int32_t x, int32_t y, int32_t z, int32_t w, uint32_t (&p)[4]) {
+  split_planes(x + 0x808080, y + 0x808080, z + 0x808080, w + 0x808080, p);
+#pragma unroll
+  for (uint32_t i = 0; i < 3; ++i) p[i] ^= 0x80808080u;
+}
+
 // Rows of 128 values (row r, part g at src + (r / per) * stride + (g * per + r %
 // per) * 128) into planes dst[g][3][rows][128]; flags what is past 24 bits.
 __device__ __forceinline__ uint32_t pack_row4(const int32_t* src, uint8_t* dst, uint64_t plane) {
   const int4 x = *(const int4*)src;
   uint32_t p[4];
-  split_planes(x.x, x.y, x.z, x.w, p);
+  split_digits(x.x, x.y, x.z, x.w, p);
 #pragma unroll
   for (uint32_t i = 0; i < 3; ++i) *(uint32_t*)(dst + i * plane) = p[i];
-  return past_24_bits(p);
+  return p[3];
 }
 
 constexpr uint32_t kPackThreads = 256;
@@ -105,8 +117,8 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
       // thread: dimension tid / 8, four tokens
       const uint32_t d = tid >> 3, t = 4 * (tid & 7);
       uint32_t p[4];
-      split_planes(tile[t][d], tile[t + 1][d], tile[t + 2][d], tile[t + 3][d], p);
-      wide |= past_24_bits(p);
+      split_digits(tile[t][d], tile[t + 1][d], tile[t + 2][d], tile[t + 3][d], p);
+      wide |= p[3];
 #pragma unroll
       for (uint32_t i = 0; i < 3; ++i)
         *(uint32_t*)(sc.vt + (((uint64_t)g * 3 + i) * kPtD + d0 + d) * sc.tpitch + t0 + t) = p[i];
@@ -149,6 +161,22 @@ __device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, PtShared
   }
 }
 
+// tc_mma and tc_commit issued by the lane with `leader`, without a branch.
+__device__ __forceinline__ void pt_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(ad), "l"(bd), "r"(idesc), "r"((uint32_t)acc), "r"((uint32_t)leader)
+      : "memory");
+}
+__device__ __forceinline__ void pt_commit(uint64_t* bar, bool leader) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
+      "r"((uint32_t)leader)
+      : "memory");
+}
+
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
 
 // The terms of four scores and their distances below the maximum, good from
@@ -175,7 +203,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* ops = ring + kPtRing;  // query planes, then weight buffers
   uint32_t* bits = (uint32_t*)(ops + kPtOperands);
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const bool leader = lane == 0;
   if (tid == 0) {
     for (uint32_t i = 0; i < kPtSlots; ++i) {
       mbar_init(&s.full[i], 1);
@@ -215,6 +244,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const bool run = s.wide == 0;
   const uint32_t items = run ? sc.tiles[a.requests] * a.kv_heads : 0, group = a.heads / a.kv_heads;
   int32_t* scores = sc.scores + (uint64_t)blockIdx.x * kPtRows * sc.pitch;
+  const uint32_t ring_a = smem_addr(ring);
+  const uint64_t ops_d = tc_desc(smem_addr(ops));
 
   // each role's running counts of the barriers' phases
   uint32_t ring_n = 0, n_item = 0, n_s = 0, n_w = 0;
@@ -250,105 +281,92 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           mbar_arrive_expect_tx(&s.full[slot], kPtSlot);
           const bool vals = u >= 3 * ktiles;
-          const uint32_t v = vals ? u - 3 * ktiles : u, t = k0 + v / 3 * kPtKeys, plane = g * 3 + v % 3;
+          const uint32_t v = vals ? u - 3 * ktiles : u, kt = v / 3, t = k0 + kt * kPtKeys;
+          // (every other score tile takes its planes from the last on)
+          const uint32_t plane = g * 3 + (vals || ((n_s + kt) & 1) == 0 ? v % 3 : 2 - v % 3);
           if (vals) tma_load_3d(ring + slot * kPtSlot, &vmap, (int32_t)t, 0, (int32_t)plane, &s.full[slot]);
           else tma_load_3d(ring + slot * kPtSlot, &kmap, 0, (int32_t)t, (int32_t)plane, &s.full[slot]);
           ++issued[slot];
         }
+        n_s += ktiles;
       }
     } else if (warp == kPtEpiWarps + 1) {
-      if (lane == 0) {  // product issuer
-        ok = ok && pt_wait(&s.q_full, n_item & 1, s, fault);
-        const uint32_t ops_a = smem_addr(ops);
-        tc_fence_after();
-        for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
-          // diagonal d of the n-th score tile lies in column group (5 n + d) % 8:
-          // the first three diagonals take groups that the tile before does
-          // not use, so six of the nine plane pairs run while it is read
-          // (a step's products go to different diagonals in turn, so that
-          // none waits for the one before it)
-          uint32_t base[3], touched = 0;
-          auto product = [&](uint32_t i, uint32_t j, uint32_t kk) {
-            tc_mma(tmem + ((5 * n_s + i + j) & 7) * kPtRows, tc_desc(base[i] + kk * 32),
-                   tc_desc(ops_a + j * kPtQPlane + kk * 32), tc_idesc(i == 2, j == 2), (touched >> (i + j)) & 1u);
-            touched |= 1u << (i + j);
-          };
-          auto plane = [&](uint32_t i) {
-            const uint32_t n = ring_n + i, slot = n % kPtSlots;
-            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) ok = false;
-            tc_fence_after();
-            base[i] = smem_addr(ring + slot * kPtSlot);
-          };
-          plane(0);
-          if (!ok) break;
-#pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk) {
-            product(0, 2, kk);
-            product(0, 1, kk);
-            product(0, 0, kk);
-          }
-          tc_commit(&s.empty[ring_n % kPtSlots]);
-          plane(1);
-          plane(2);
-          if (!ok) break;
-#pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk) {
-            product(1, 1, kk);
-            product(1, 0, kk);
-            product(2, 0, kk);
-          }
-          if (kt) ok = pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+      // product issuer: the whole warp walks the tiles (so that addresses and
+      // descriptors stay uniform), its first lane issues
+      ok = ok && pt_wait(&s.q_full, n_item & 1, s, fault);
+      tc_fence_after();
+      for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
+        // Key plane i against the three query planes side by side (192 rows) is
+        // diagonals i, i + 1, i + 2 in neighbouring column groups. The score
+        // tiles take groups 0-4 and 3-7 in turn, from the end that the tile
+        // before does not use, so a third of the products run while it is read.
+        const bool up = (n_s & 1) == 0;
+        const uint32_t cols = tmem + (up ? 0 : 3 * kPtRows);
+#pragma unroll 1
+        for (uint32_t st = 0; st < 3; ++st, ++ring_n) {
+          const uint32_t i = up ? st : 2 - st, slot = ring_n % kPtSlots;
+          ok = ok && pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault);
+          if (st == 1 && kt) ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
           if (!ok) break;
           tc_fence_after();
-#pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk) {
-            product(1, 2, kk);
-            product(2, 2, kk);
-            product(2, 1, kk);
+          const uint64_t key = tc_desc(ring_a + slot * kPtSlot);
+          const uint32_t col = cols + i * kPtRows;
+          // the first product into a diagonal overwrites it: all three of the
+          // first plane; then the outermost one of each further plane
+          if (st == 0) {
+            pt_mma(col, key, ops_d, tc_idesc_n(true, true, 3 * kPtRows), false, leader);
+          } else {
+            const uint32_t in = up ? 0 : 1, out = up ? 2 : 0;  // query planes of the other two, and of the outermost
+            pt_mma(col + in * kPtRows, key, ops_d + in * (kPtQPlane / 16), tc_idesc_n(true, true, 2 * kPtRows), true,
+                   leader);
+            pt_mma(col + out * kPtRows, key, ops_d + out * (kPtQPlane / 16), tc_idesc_n(true, true, kPtRows), false,
+                   leader);
           }
-          tc_commit(&s.empty[(ring_n + 1) % kPtSlots]);
-          tc_commit(&s.empty[(ring_n + 2) % kPtSlots]);
-          tc_commit(&s.s_done);
-          ring_n += 3;
+#pragma unroll
+          for (uint32_t kk = 1; kk < 4; ++kk)
+            pt_mma(col, key + 2 * kk, ops_d + 2 * kk, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
+          pt_commit(&s.empty[slot], leader);
         }
-        // the diagonals of the last score tile are read before the value sums take their columns
-        ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+        if (!ok) break;
+        pt_commit(&s.s_done, leader);
+      }
+      // the diagonals of the last score tile are read before the value sums take their columns
+      ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+      tc_fence_after();
+      for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
+        const uint32_t buf = n_w & 1;
+        ok = pt_wait(&s.w_full[buf], (n_w >> 1) & 1, s, fault);
+        uint32_t slot[3];
+        uint64_t val[3];
+#pragma unroll
+        for (uint32_t i = 0; i < 3; ++i) {
+          const uint32_t n = ring_n + i;
+          slot[i] = n % kPtSlots;
+          ok = ok && pt_wait(&s.full[slot[i]], (n / kPtSlots) & 1, s, fault);
+          val[i] = tc_desc(ring_a + slot[i] * kPtSlot);
+        }
+        if (!ok) break;
         tc_fence_after();
-        uint32_t touched = 0;
-        for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
-          const uint32_t buf = n_w & 1;
-          if (!pt_wait(&s.w_full[buf], (n_w >> 1) & 1, s, fault)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          uint32_t base[3];
+        // value plane i against both weight planes (128 rows): diagonals i, i + 1
+        const uint64_t w = ops_d + buf * (kPtWBuf / 16);
+#pragma unroll
+        for (uint32_t kk = 0; kk < 4; ++kk)
 #pragma unroll
           for (uint32_t i = 0; i < 3; ++i) {
-            const uint32_t n = ring_n + i, slot = n % kPtSlots;
-            if (!ok || !pt_wait(&s.full[slot], (n / kPtSlots) & 1, s, fault)) ok = false;
-            base[i] = smem_addr(ring + slot * kPtSlot);
+            const uint32_t col = tmem + i * kPtRows;
+            if (kk == 0 && kt == 0 && i) {
+              pt_mma(col, val[i], w, tc_idesc_n(true, false, kPtRows), true, leader);
+              pt_mma(col + kPtRows, val[i], w + kPtQPlane / 16, tc_idesc_n(true, false, kPtRows), false, leader);
+            } else {
+              pt_mma(col, val[i] + 2 * kk, w + 2 * kk, tc_idesc_n(true, false, 2 * kPtRows), kk || kt, leader);
+            }
           }
-          if (!ok) break;
-          tc_fence_after();
 #pragma unroll
-          for (uint32_t kk = 0; kk < 4; ++kk)
-#pragma unroll
-            for (uint32_t j = 0; j < 2; ++j)
-#pragma unroll
-              for (uint32_t i = 0; i < 3; ++i) {
-                tc_mma(tmem + (i + j) * kPtRows, tc_desc(base[i] + kk * 32),
-                       tc_desc(ops_a + buf * kPtWBuf + j * kPtQPlane + kk * 32), tc_idesc(i == 2, false),
-                       (touched >> (i + j)) & 1u);
-                touched |= 1u << (i + j);
-              }
-#pragma unroll
-          for (uint32_t i = 0; i < 3; ++i) tc_commit(&s.empty[(ring_n + i) % kPtSlots]);
-          ring_n += 3;
-          if (ok) tc_commit(&s.w_empty[buf]);
-        }
-        if (ok) tc_commit(&s.v_done);
+        for (uint32_t i = 0; i < 3; ++i) pt_commit(&s.empty[slot[i]], leader);
+        pt_commit(&s.w_empty[buf], leader);
+        ring_n += 3;
       }
+      if (ok) pt_commit(&s.v_done, leader);
     } else {
       // epilogue warps: TMEM lanes 32 quad .. (keys, then dims), rows 16 cg ..
       const uint32_t quad = warp & 3, cg = warp >> 2;
@@ -375,7 +393,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           uint32_t v[5][8];
 #pragma unroll
           for (uint32_t d = 0; d < 5; ++d)
-            tmem_ld8(tmem + ((32 * quad) << 16) + ((5 * n_s + d) & 7) * kPtRows + cg * 16 + h * 8, v[d]);
+            tmem_ld8(tmem + ((32 * quad) << 16) + ((n_s & 1) * 3 + d) * kPtRows + cg * 16 + h * 8, v[d]);
           tmem_ld_wait();
 #pragma unroll
           for (uint32_t c = 0; c < 8; ++c) {
