@@ -472,20 +472,32 @@ IRIS_HD uint32_t exp_term_near(uint32_t d) {
   return f + (out + (f & 1) > 0x80000000u);
 }
 
-// The same term within one: the polynomial by Horner's rule in truncated 32-bit
-// products, shifted down. From kExpExactBelow on (k >= 3, where the shift
-// drops most of the truncation) exp_term_near is this or one more, so one bit a
-// distance makes it exact; the host test checks every distance.
-static constexpr uint32_t kExpExactBelow = 136278;  // ceil(3 ln2 in Q16.16)
+// The same term within one: the polynomial by Horner's rule in double precision,
+// two units low, its integer part taken by adding 2^52, shifted down. From
+// kExpExactBelow on (k >= 3, where the shift drops the powers' own roundings)
+// exp_term_near is this or one more, so one bit a distance makes it exact; the
+// host test checks every distance.
+static constexpr uint32_t kExpExactBelow = 136288;  // 3 ln2 in Q16.16, up to a multiple of 32
 IRIS_HD uint32_t exp_term_estimate(uint32_t d) {
   const uint32_t k = exp_term_turns(d);
   const uint32_t r = (d << 16) - k * 2977044472u;
-  uint32_t a = 178956971u - mulhi_u32(r, 35791394u);  // 2^32 / 24, 2^32 / 120
-  a = 715827883u - mulhi_u32(r, a);                   // 2^32 / 6
-  a = 2147483648u - mulhi_u32(r, a);
-  a = 0u - mulhi_u32(r, a);
-  a = 0u - mulhi_u32(r, a);
-  return a >> k;
+  constexpr double u = 1.0 / 4294967296.0;  // r counts 2^-32
+#if defined(__CUDA_ARCH__)
+  const double x = __hiloint2double(0x43300000, (int)r) - 4503599627370496.0;
+#else
+  const double x = (double)r;
+#endif
+  double a = fma(x, -u * u * u * u / 120.0, u * u * u / 24.0);
+  a = fma(x, a, -u * u / 6.0);
+  a = fma(x, a, u / 2.0);
+  a = fma(x, a, -1.0);
+  a = fma(x, a, 4294967296.0 - 2.0 + 4503599627370496.0);
+#if defined(__CUDA_ARCH__)
+  const uint32_t y = (uint32_t)__double2loint(a);
+#else
+  const uint32_t y = (uint32_t)(uint64_t)(a - 4503599627370496.0);
+#endif
+  return y >> k;
 }
 
 // softmax_exp_term(act_to_acc(sub_sat(logit, max))): e^delta in Q32.32.

@@ -44,7 +44,9 @@ constexpr uint32_t kPtEpiWarps = 16, kPtEpi = 32 * kPtEpiWarps, kPtThreads = kPt
 constexpr uint32_t kPtSlots = 5, kPtSlot = kPtKeys * kPtD;  // one plane of a key or value tile
 constexpr uint32_t kPtQPlane = kPtRows * kPtD;              // one plane of the query rows; of a weight tile
 constexpr uint32_t kPtWBuf = 2 * kPtQPlane;                 // two weight planes
-constexpr uint32_t kPtTable = (kExpTerms - kExpExactBelow / 32 * 32) / 32;  // words
+constexpr uint32_t kPtFar = kExpTerms - kExpExactBelow;  // distances with a correction bit
+constexpr uint32_t kPtTable = kPtFar / 32;               // words
+constexpr uint32_t kPtBlock = kPtRows * kPtKeys;           // scores of a key tile: [row][key]
 constexpr uint32_t kPtRing = kPtSlots * kPtSlot;
 constexpr uint32_t kPtOperands = 2 * kPtWBuf;  // the query planes (3 x 8 KB), later two weight buffers
 constexpr uint32_t kPtList = kPtOperands / 4 / kPtEpiWarps;  // words of a warp's list of near scores
@@ -125,10 +127,10 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
     }
   } else {
     const uint32_t lane = tid & 31;
-    for (uint32_t d = (kExpExactBelow / 32 * 32) + blockIdx.x * kPackThreads + tid; d < kExpTerms;
-         d += gridDim.x * kPackThreads) {
+    for (uint32_t c = blockIdx.x * kPackThreads + tid; c < kPtFar; c += gridDim.x * kPackThreads) {
+      const uint32_t d = kExpExactBelow + c;
       const uint32_t bits = __ballot_sync(0xffffffffu, exp_term_near(d) != exp_term_estimate(d));
-      if (lane == 0) sc.exp_bits[d / 32 - kExpExactBelow / 32] = bits;
+      if (lane == 0) sc.exp_bits[c / 32] = bits;
     }
   }
   wide = __syncthreads_or(wide != 0);
@@ -179,18 +181,16 @@ __device__ __forceinline__ void pt_commit(uint64_t* bar, bool leader) {
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
 
-// The terms of four scores and their distances below the maximum, good from
-// kExpExactBelow on.
-__device__ __forceinline__ void terms_by_table(const int4& x, int32_t top, const uint32_t* bits, uint32_t (&e)[4],
-                                               uint32_t (&d)[4]) {
-  const int32_t v[4] = {x.x, x.y, x.z, x.w};
+// The terms of eight scores, 0 below kExpExactBelow, and their distances.
+__device__ __forceinline__ void terms_by_table(const int4 (&x)[2], int32_t top, const uint32_t* bits, uint32_t (&e)[8],
+                                               uint32_t (&d)[8]) {
+  const int32_t v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
-  for (uint32_t u = 0; u < 4; ++u) {
+  for (uint32_t u = 0; u < 8; ++u) {
     d[u] = (uint32_t)top - (uint32_t)v[u];
-    const uint32_t c = min(max(d[u], kExpExactBelow), kExpTerms - 1);
-    const uint32_t word = bits[(c >> 5) - kExpExactBelow / 32];
-    const uint32_t t = exp_term_estimate(c) + (__funnelshift_r(word, 0, c) & 1);
-    e[u] = d[u] < kExpTerms ? t : 0;
+    const uint32_t c = d[u] - kExpExactBelow, i = min(c, kPtFar - 1);
+    const uint32_t t = exp_term_estimate(d[u]) + (__funnelshift_r(bits[i >> 5], 0, i) & 1);
+    e[u] = c < kPtFar ? t : 0;
   }
 }
 
@@ -336,35 +336,28 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
         const uint32_t buf = n_w & 1;
         ok = pt_wait(&s.w_full[buf], (n_w >> 1) & 1, s, fault);
-        uint32_t slot[3];
-        uint64_t val[3];
-#pragma unroll
-        for (uint32_t i = 0; i < 3; ++i) {
-          const uint32_t n = ring_n + i;
-          slot[i] = n % kPtSlots;
-          ok = ok && pt_wait(&s.full[slot[i]], (n / kPtSlots) & 1, s, fault);
-          val[i] = tc_desc(ring_a + slot[i] * kPtSlot);
-        }
-        if (!ok) break;
-        tc_fence_after();
         // value plane i against both weight planes (128 rows): diagonals i, i + 1
         const uint64_t w = ops_d + buf * (kPtWBuf / 16);
-#pragma unroll
-        for (uint32_t kk = 0; kk < 4; ++kk)
-#pragma unroll
-          for (uint32_t i = 0; i < 3; ++i) {
-            const uint32_t col = tmem + i * kPtRows;
-            if (kk == 0 && kt == 0 && i) {
-              pt_mma(col, val[i], w, tc_idesc_n(true, false, kPtRows), true, leader);
-              pt_mma(col + kPtRows, val[i], w + kPtQPlane / 16, tc_idesc_n(true, false, kPtRows), false, leader);
-            } else {
-              pt_mma(col, val[i] + 2 * kk, w + 2 * kk, tc_idesc_n(true, false, 2 * kPtRows), kk || kt, leader);
-            }
+#pragma unroll 1
+        for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
+          const uint32_t slot = ring_n % kPtSlots, col = tmem + i * kPtRows;
+          ok = ok && pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault);
+          if (!ok) break;
+          tc_fence_after();
+          const uint64_t val = tc_desc(ring_a + slot * kPtSlot);
+          if (kt == 0 && i) {
+            pt_mma(col, val, w, tc_idesc_n(true, false, kPtRows), true, leader);
+            pt_mma(col + kPtRows, val, w + kPtQPlane / 16, tc_idesc_n(true, false, kPtRows), false, leader);
+          } else {
+            pt_mma(col, val, w, tc_idesc_n(true, false, 2 * kPtRows), kt != 0, leader);
           }
 #pragma unroll
-        for (uint32_t i = 0; i < 3; ++i) pt_commit(&s.empty[slot[i]], leader);
+          for (uint32_t kk = 1; kk < 4; ++kk)
+            pt_mma(col, val + 2 * kk, w + 2 * kk, tc_idesc_n(true, false, 2 * kPtRows), true, leader);
+          pt_commit(&s.empty[slot], leader);
+        }
+        if (!ok) break;
         pt_commit(&s.w_empty[buf], leader);
-        ring_n += 3;
       }
       if (ok) pt_commit(&s.v_done, leader);
     } else {
@@ -405,11 +398,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.t_free);
-        const uint32_t t = kt * kPtKeys + 32 * quad + lane, key = k0 + t;
+        const uint32_t key = k0 + kt * kPtKeys + 32 * quad + lane;
         // the warp's keys, seen by every row of the tile?
         const uint32_t kw = k0 + kt * kPtKeys + 32 * quad;
         const bool open = rows == kPtRows && kw + 31 <= begin + q0 && kw >= begin + window_start(q1, a.window);
-        int32_t* out = scores + (uint64_t)(cg * 16) * sc.pitch + t;
+        int32_t* out = scores + (uint64_t)kt * kPtBlock + cg * 16 * kPtKeys + 32 * quad + lane;
 #pragma unroll
         for (uint32_t c = 0; c < 16; ++c) {
           int32_t x = score_of(hi[c], lo[c], a.scale_q32);
@@ -418,7 +411,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             if (q < 0 || key > begin + (uint32_t)q || key < begin + window_start((uint32_t)q, a.window)) x = INT32_MIN;
           }
           best[c] = max(best[c], x);
-          __stcg(out + c * sc.pitch, x);
+          __stcg(out + c * kPtKeys, x);
         }
       }
 #pragma unroll
@@ -433,19 +426,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       for (uint32_t i = warp; i < kPtRows; i += kPtEpiWarps) {
         const int32_t top = s.top[i], q = s.query[i];
         const bool ask = top < INT32_MIN + (1 << 20);
-        int32_t* row = scores + (uint64_t)i * sc.pitch;
+        int32_t* row = scores + i * kPtKeys;  // key t at (t / 128) blocks + t % 128
         uint64_t sum = 0;
         uint32_t first = UINT32_MAX;
         if (q >= 0 && !ask) {
-          // eight scores a lane and turn, the next eight loaded ahead; those
-          // nearer to the maximum than the table goes are put on a list (place
-          // and distance in one word) and done 32 at a time, exactly
+          // eight scores a lane and turn (two key tiles), the next eight loaded
+          // ahead; those nearer to the maximum than the table goes are put on a
+          // list (place and distance in one word) and done 32 at a time, exactly
           const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
           int4 x[2], y[2] = {hidden, hidden};
           uint32_t listed = 0;
-          auto load = [&](int4 (&z)[2], uint32_t t) {
-#pragma unroll
-            for (uint32_t m = 0; m < 2; ++m) z[m] = t + 128 * m < padded ? __ldcg((const int4*)(row + t + 128 * m)) : hidden;
+          auto load = [&](int4 (&z)[2], uint32_t kt) {
+            const int32_t* at = row + (uint64_t)kt * kPtBlock + 4 * lane;
+            z[0] = __ldcg((const int4*)at);
+            z[1] = kt + 1 < ktiles ? __ldcg((const int4*)(at + kPtBlock)) : hidden;
           };
           auto drain = [&] {
             __syncwarp();
@@ -454,45 +448,50 @@ __global__ void __launch_bounds__(kPtThreads, 1)
               const uint32_t z = d ? exp_term_near(d) : kTermTop;
               if (!d) first = min(first, at);
               sum += kept_term(z);
-              __stcg((uint32_t*)(row + at), z);
+              __stcg((uint32_t*)row + (at / kPtKeys) * kPtBlock + at % kPtKeys, z);
             }
             listed = 0;
             __syncwarp();
           };
-          load(x, 4 * lane);
-          for (uint32_t t = 4 * lane; t < padded + 4 * lane; t += 256) {
-            if (t + 256 < padded) load(y, t + 256);
+          load(x, 0);
+          for (uint32_t kt = 0; kt < ktiles; kt += 2) {
+            if (kt + 2 < ktiles) load(y, kt + 2);
+            uint32_t e[8], d[8];
+            terms_by_table(x, top, bits, e, d);
+            sum += ((uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3])) + ((uint64_t)e[4] + e[5] + ((uint64_t)e[6] + e[7]));
+            uint32_t* at = (uint32_t*)row + (uint64_t)kt * kPtBlock + 4 * lane;
+            __stcg((uint4*)at, make_uint4(e[0], e[1], e[2], e[3]));
+            if (kt + 1 < ktiles) __stcg((uint4*)(at + kPtBlock), make_uint4(e[4], e[5], e[6], e[7]));
+            const uint32_t least = min(min(min(d[0], d[1]), min(d[2], d[3])), min(min(d[4], d[5]), min(d[6], d[7])));
+            if (__any_sync(0xffffffffu, least < kExpExactBelow)) {
+              uint32_t near = 0;
 #pragma unroll
-            for (uint32_t m = 0; m < 2; ++m) {
-              uint32_t e[4], d[4];
-              terms_by_table(x[m], top, bits, e, d);
-              if (__any_sync(0xffffffffu, min(min(d[0], d[1]), min(d[2], d[3])) < kExpExactBelow)) {
+              for (uint32_t u = 0; u < 8; ++u) near |= (d[u] < kExpExactBelow ? 1u : 0u) << u;
+              for (uint32_t who; (who = __ballot_sync(0xffffffffu, near != 0)) != 0; near &= near - 1) {
+                if (near) {
+                  const uint32_t u = __ffs(near) - 1;
+                  uint32_t dist = d[0];
 #pragma unroll
-                for (uint32_t u = 0; u < 4; ++u) {
-                  const bool near = d[u] < kExpExactBelow;
-                  const uint32_t all = __ballot_sync(0xffffffffu, near);
-                  if (near) {
-                    list[listed + __popc(all & ((1u << lane) - 1))] = (t + 128 * m + u) << kPtNearBits | d[u];
-                    e[u] = 0;
-                  }
-                  listed += __popc(all);
+                  for (uint32_t o = 1; o < 8; ++o) dist = u == o ? d[o] : dist;
+                  list[listed + __popc(who & ((1u << lane) - 1))] =
+                      ((kt + u / 4) * kPtKeys + 4 * lane + u % 4) << kPtNearBits | dist;
                 }
+                listed += __popc(who);
               }
-              sum += (uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3]);
-              if (t + 128 * m < padded) __stcg((uint4*)(row + t + 128 * m), make_uint4(e[0], e[1], e[2], e[3]));
-              x[m] = y[m];
+              if (listed + 256 > kPtList) drain();
             }
-            if (listed + 256 > kPtList) drain();
+            x[0] = y[0], x[1] = y[1];
           }
           drain();
         } else if (q >= 0) {
           // every score within 16.0 of the lowest: hidden keys by their place
           const uint32_t k1 = begin + (uint32_t)q, ks = begin + window_start((uint32_t)q, a.window);
           for (uint32_t t = lane; t < padded; t += 32) {
-            const uint32_t z = k0 + t < ks || k0 + t > k1 ? 0 : term_of(row[t], top);
+            int32_t* at = row + (t / kPtKeys) * kPtBlock + t % kPtKeys;
+            const uint32_t z = k0 + t < ks || k0 + t > k1 ? 0 : term_of(__ldcg(at), top);
             if (z == kTermTop) first = min(first, t);
             sum += kept_term(z);
-            __stcg((uint32_t*)(row + t), z);
+            __stcg((uint32_t*)at, z);
           }
         }
         sum = (uint64_t)warp_sum_i64((int64_t)sum);
@@ -502,7 +501,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           s.sum[i] = sum;
           s.recip[i] = sum_recip(sum);
           s.first[i] = first;
-          if (q >= 0 && first < padded) row[first] = 0;  // its weight comes last
+          if (q >= 0 && first < padded) __stcg(row + (first / kPtKeys) * kPtBlock + first % kPtKeys, 0);  // its weight comes last
         }
       }
       epi_sync();
@@ -512,7 +511,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       auto load_terms = [&](uint32_t kt) {
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
-          const int32_t* e = scores + (uint64_t)((tid >> 4) + 32 * h) * sc.pitch + kt * kPtKeys + 8 * (tid & 15);
+          const int32_t* e = scores + (uint64_t)kt * kPtBlock + ((tid >> 4) + 32 * h) * kPtKeys + 8 * (tid & 15);
           next[h][0] = __ldcg((const uint4*)e);
           next[h][1] = __ldcg((const uint4*)(e + 4));
         }
@@ -537,11 +536,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           const uint32_t recip = s.recip[i];
           const uint64_t sum = s.sum[i];
           int32_t w[8];
+          weights_of(term, recip, sum, w);
 #pragma unroll
-          for (uint32_t j = 0; j < 8; ++j) {
-            w[j] = weight_of(term[j], recip, sum);
-            all[h] += w[j];
-          }
+          for (uint32_t j = 0; j < 8; ++j) all[h] += w[j];
           const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
           const uint32_t u0 = __byte_perm(w[4], w[5], 0x5140), u1 = __byte_perm(w[6], w[7], 0x5140);
           // 128-byte rows in the 128-byte swizzle: 16-byte pieces exchanged by the row's low bits

@@ -229,6 +229,30 @@ __device__ __forceinline__ uint32_t sum_recip(uint64_t sum) { return sum ? (uint
 static __device__ __noinline__ int32_t exact_weight(uint32_t term, uint64_t sum) {
   return softmax_weight((int64_t)kept_term(term), sum);
 }
+// Eight weights of one row: the doubtful ones found together.
+__device__ __forceinline__ void weights_of(const uint32_t (&term)[8], uint32_t recip, uint64_t sum, int32_t (&w)[8]) {
+  uint32_t y[8], least = 0x7FFF;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) {
+    y[j] = __umulhi(term[j], recip) + (1u << 14);
+    least = min(least, (y[j] + 3) & 0x7FFF);
+    w[j] = (int32_t)(y[j] >> 15);
+  }
+  if (least <= 3 && recip) {
+#pragma unroll 1
+    for (uint32_t j = 0; j < 8; ++j) {
+      uint32_t t = 0, z = 0;
+#pragma unroll
+      for (uint32_t o = 0; o < 8; ++o)
+        if (o == j) t = term[o], z = y[o];
+      if (((z + 3) & 0x7FFF) > 3) continue;
+      const int32_t exact = exact_weight(t, sum);
+#pragma unroll
+      for (uint32_t o = 0; o < 8; ++o)
+        if (o == j) w[o] = exact;
+    }
+  }
+}
 __device__ __forceinline__ int32_t weight_of(uint32_t term, uint32_t recip, uint64_t sum) {
   const uint32_t y = (uint32_t)(((uint64_t)term * recip) >> 32) + (1u << 14);
   if (((y + 3) & 0x7FFF) <= 3) return recip ? exact_weight(term, sum) : 0;
