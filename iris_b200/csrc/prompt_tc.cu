@@ -423,6 +423,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       // 2. terms in place, a row a warp (hidden keys: see prompt_mma.cu)
       const uint32_t padded = ktiles * kPtKeys;
       uint32_t* list = (uint32_t*)ops + warp * kPtList;  // (the query planes are done with)
+      // eight scores a lane and turn (two key tiles) of a row
+      const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+      auto load = [&](int4 (&z)[2], const int32_t* row, uint32_t kt) {
+        const int32_t* at = row + (uint64_t)kt * kPtBlock + 4 * lane;
+        z[0] = __ldcg((const int4*)at);
+        z[1] = kt + 1 < ktiles ? __ldcg((const int4*)(at + kPtBlock)) : hidden;
+      };
+      int4 x[2];
+      load(x, scores + warp * kPtKeys, 0);
       for (uint32_t i = warp; i < kPtRows; i += kPtEpiWarps) {
         const int32_t top = s.top[i], q = s.query[i];
         const bool ask = top < INT32_MIN + (1 << 20);
@@ -430,17 +439,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         uint64_t sum = 0;
         uint32_t first = UINT32_MAX;
         if (q >= 0 && !ask) {
-          // eight scores a lane and turn (two key tiles), the next eight loaded
-          // ahead; those nearer to the maximum than the table goes are put on a
-          // list (place and distance in one word) and done 32 at a time, exactly
-          const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-          int4 x[2], y[2] = {hidden, hidden};
+          // the next eight (or the next row's first) are loaded ahead; scores
+          // nearer to the maximum than the table goes are put on a list (place
+          // and distance in one word) and done 32 at a time, exactly
+          int4 y[2] = {hidden, hidden};
           uint32_t listed = 0;
-          auto load = [&](int4 (&z)[2], uint32_t kt) {
-            const int32_t* at = row + (uint64_t)kt * kPtBlock + 4 * lane;
-            z[0] = __ldcg((const int4*)at);
-            z[1] = kt + 1 < ktiles ? __ldcg((const int4*)(at + kPtBlock)) : hidden;
-          };
           auto drain = [&] {
             __syncwarp();
             for (uint32_t n = lane; n < listed; n += 32) {
@@ -453,9 +456,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             listed = 0;
             __syncwarp();
           };
-          load(x, 0);
           for (uint32_t kt = 0; kt < ktiles; kt += 2) {
-            if (kt + 2 < ktiles) load(y, kt + 2);
+            if (kt + 2 < ktiles) load(y, row, kt + 2);
+            else if (i + kPtEpiWarps < kPtRows) load(y, row + kPtEpiWarps * kPtKeys, 0);
             uint32_t e[8], d[8];
             terms_by_table(x, top, bits, e, d);
             sum += ((uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3])) + ((uint64_t)e[4] + e[5] + ((uint64_t)e[6] + e[7]));
@@ -483,7 +486,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             x[0] = y[0], x[1] = y[1];
           }
           drain();
-        } else if (q >= 0) {
+        } else {
+          if (i + kPtEpiWarps < kPtRows) load(x, row + kPtEpiWarps * kPtKeys, 0);
+        }
+        if (q >= 0 && ask) {
           // every score within 16.0 of the lowest: hidden keys by their place
           const uint32_t k1 = begin + (uint32_t)q, ks = begin + window_start((uint32_t)q, a.window);
           for (uint32_t t = lane; t < padded; t += 32) {
@@ -499,16 +505,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         __syncwarp();
         if (lane == 0) {
           s.sum[i] = sum;
-          s.recip[i] = sum_recip(sum);
           s.first[i] = first;
           if (q >= 0 && first < padded) __stcg(row + (first / kPtKeys) * kPtBlock + first % kPtKeys, 0);  // its weight comes last
         }
       }
+      __syncwarp();
+      if (lane < kPtRows / kPtEpiWarps) {
+        const uint32_t i = warp + lane * kPtEpiWarps;
+        s.recip[i] = sum_recip(s.sum[i]);
+      }
       epi_sync();
       // 3. weights: eight keys of a row a thread, two rows' worth a tile
       int32_t all[2] = {};
-      uint4 next[2][2];
-      auto load_terms = [&](uint32_t kt) {
+      uint4 next[2][2], after[2][2];
+      auto load_terms = [&](uint4 (&next)[2][2], uint32_t kt) {
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
           const int32_t* e = scores + (uint64_t)kt * kPtBlock + ((tid >> 4) + 32 * h) * kPtKeys + 8 * (tid & 15);
@@ -516,7 +526,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           next[h][1] = __ldcg((const uint4*)(e + 4));
         }
       };
-      load_terms(0);
+      load_terms(next, 0);
+      if (ktiles > 1) load_terms(after, 1);
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
         const uint32_t buf = n_w & 1, use = n_w >> 1;
         if (use > 0 && !pt_wait(&s.w_empty[buf], (use - 1) & 1, s, fault)) {
@@ -526,8 +537,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         uint8_t* wb = ops + buf * kPtWBuf;
         uint4 now[2][2];
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) now[h][0] = next[h][0], now[h][1] = next[h][1];
-        if (kt + 1 < ktiles) load_terms(kt + 1);
+        for (uint32_t h = 0; h < 2; ++h)
+#pragma unroll
+          for (uint32_t m = 0; m < 2; ++m) now[h][m] = next[h][m], next[h][m] = after[h][m];
+        if (kt + 2 < ktiles) load_terms(after, kt + 2);
 #pragma unroll
         for (uint32_t h = 0; h < 2; ++h) {
           const uint32_t i = (tid >> 4) + 32 * h, c = tid & 15;
