@@ -472,15 +472,14 @@ IRIS_HD uint32_t exp_term_near(uint32_t d) {
   return f + (out + (f & 1) > 0x80000000u);
 }
 
-// The same term within one: the polynomial by Horner's rule in double precision,
-// two units low, its integer part taken by adding 2^52, shifted down. From
-// kExpExactBelow on (k >= 3, where the shift drops the powers' own roundings)
-// exp_term_near is this or one more, so one bit a distance makes it exact; the
-// host test checks every distance.
-static constexpr uint32_t kExpExactBelow = 136288;  // 3 ln2 in Q16.16, up to a multiple of 32
-IRIS_HD uint32_t exp_term_estimate(uint32_t d) {
+// The polynomial of that term by Horner's rule in double precision, two units
+// low, its integer part y taken by adding 2^52: the exact one, with its powers'
+// and quotients' own roundings, lies in [y, y + 4] (the host test checks what
+// the two forms below make of it on every distance).
+IRIS_HD uint32_t exp_term_polynomial(uint32_t d, uint32_t* turns) {
   const uint32_t k = exp_term_turns(d);
   const uint32_t r = (d << 16) - k * 2977044472u;
+  *turns = k;
   constexpr double u = 1.0 / 4294967296.0;  // r counts 2^-32
 #if defined(__CUDA_ARCH__)
   const double x = __hiloint2double(0x43300000, (int)r) - 4503599627370496.0;
@@ -493,11 +492,27 @@ IRIS_HD uint32_t exp_term_estimate(uint32_t d) {
   a = fma(x, a, -1.0);
   a = fma(x, a, 4294967296.0 - 2.0 + 4503599627370496.0);
 #if defined(__CUDA_ARCH__)
-  const uint32_t y = (uint32_t)__double2loint(a);
+  return (uint32_t)__double2loint(a);
 #else
-  const uint32_t y = (uint32_t)(uint64_t)(a - 4503599627370496.0);
+  return (uint32_t)(uint64_t)(a - 4503599627370496.0);
 #endif
-  return y >> k;
+}
+// The term within one: exp_term_near is this or one more from kExpExactBelow on
+// (k >= 3, where the shift drops the roundings), so one bit a distance, kept in a
+// table, makes it exact.
+static constexpr uint32_t kExpExactBelow = 136288;  // 3 ln2 in Q16.16, up to a multiple of 32
+IRIS_HD uint32_t exp_term_floor(uint32_t d) {
+  uint32_t k;
+  const uint32_t y = exp_term_polynomial(d, &k);
+  return y >> (k & 31);
+}
+// The term without a table, and whether it may be wrong: y / 2^k to nearest,
+// unless a half lies in [y, y + 4] / 2^k (always for k < 3).
+IRIS_HD uint32_t exp_term_estimate(uint32_t d, bool* doubt) {
+  uint32_t k;
+  const uint32_t y = exp_term_polynomial(d, &k), one = 1u << (k & 31);
+  *doubt = (((one >> 1) - y) & (one - 1)) <= 4;
+  return ((y >> ((k - 1) & 31)) + 1) >> 1;
 }
 
 // softmax_exp_term(act_to_acc(sub_sat(logit, max))): e^delta in Q32.32.

@@ -184,11 +184,9 @@ __device__ __noinline__ bool prompt_values(const IrisPromptAttention& a, const P
       const uint32_t recip = s.recip[i];
       const uint64_t sum = s.sum[i];
       int32_t x[8], all = 0;
+      weights_of(term, recip, sum, x);
 #pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) {
-        x[j] = weight_of(term[j], recip, sum);
-        all += x[j];
-      }
+      for (uint32_t j = 0; j < 8; ++j) all += x[j];
       put_weight_fragment(wb + (st * NT + n) * 64, lane, x);
       all += __shfl_xor_sync(0xffffffffu, all, 1);
       all += __shfl_xor_sync(0xffffffffu, all, 2);
@@ -244,6 +242,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
   const uint32_t steps = a.head_dim / 32;
   uint2* frag = (uint2*)prompt_sm;                  // [NT][steps][4][32]
   uint2* w = frag + NT * steps * 128;               // [2][kPromptKeys / 32][NT][2][32]
+  uint32_t* lists = (uint32_t*)(w + 2 * kPromptKeys / 32 * NT * 64);  // [warps][kTermList]
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int32_t* scores = sc.scores + (uint64_t)blockIdx.x * RT * sc.pitch;
   int64_t* acc_buf = sc.acc + (uint64_t)blockIdx.x * RT * a.head_dim;
@@ -338,24 +337,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
     const uint32_t written = (p.count + 15) / 16 * 16, padded = (p.count + 31) / 32 * 32;
     for (uint32_t i = warp; i < RT; i += kPromptWarps) {
       const int32_t top = s.top[i], q = s.query[i];
-      const bool ask = top < INT32_MIN + (1 << 20);
       int32_t* row = scores + (uint64_t)i * sc.pitch;
       uint64_t sum = 0;
       uint32_t first = UINT32_MAX;
-      if (q >= 0) {
-        for (uint32_t t = 4 * lane; t < padded; t += 128) {
-          const int4 x = t < written ? __ldcg((const int4*)(row + t)) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-          const int32_t v[4] = {x.x, x.y, x.z, x.w};
-          uint32_t e[4];
-#pragma unroll
-          for (uint32_t u = 0; u < 4; ++u) {
-            e[u] = term_of(v[u], top);
-            const uint32_t key = p.base + t + u;
-            if (ask && (t + u >= p.count || key > (uint32_t)q || key < window_start((uint32_t)q, a.window))) e[u] = 0;
-            sum += kept_term(e[u]);
-            if (e[u] == kTermTop) first = min(first, t + u);
-          }
-          __stcg((uint4*)(row + t), make_uint4(e[0], e[1], e[2], e[3]));
+      if (q >= 0 && top >= INT32_MIN + (1 << 20)) {
+        int4 x[2];
+        row_load(x, row, 128, 0, written, lane);
+        const RowTerms r = row_terms(row, 128, written, padded, top, lists + warp * kTermList, lane, x, nullptr);
+        sum = r.sum;
+        first = r.first;
+      } else if (q >= 0) {
+        for (uint32_t t = lane; t < padded; t += 32) {
+          const uint32_t key = p.base + t;
+          const bool gone = t >= p.count || key > (uint32_t)q || key < window_start((uint32_t)q, a.window);
+          const uint32_t e = gone ? 0 : term_of(__ldcg(row + t), top);
+          if (e == kTermTop) first = min(first, t);
+          sum += kept_term(e);
+          __stcg((uint32_t*)row + t, e);
         }
       }
       sum = (uint64_t)warp_sum_i64((int64_t)sum);
@@ -365,7 +363,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
         s.sum[i] = sum;
         s.recip[i] = sum_recip(sum);
         s.first[i] = first;
-        if (q >= 0) row[first] = 0;  // its weight comes last
+        if (q >= 0) __stcg(row + first, 0);  // its weight comes last
       }
     }
     __syncthreads();
@@ -422,7 +420,8 @@ size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, Pro
 template <uint32_t RT>
 cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, const PromptTcScratch& tc,
                    cudaStream_t stream) {
-  const uint32_t smem = RT / 8 * (a.head_dim / 32) * 1024 + 2 * kPromptKeys / 32 * (RT / 8) * 512;
+  const uint32_t smem = RT / 8 * (a.head_dim / 32) * 1024 + 2 * kPromptKeys / 32 * (RT / 8) * 512 +
+                        kPromptWarps * kTermList * 4;
   cudaError_t e = cudaFuncSetAttribute(prompt_mma_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   prompt_items_kernel<<<1, 1024, 0, stream>>>(a, sc, RT);

@@ -13,8 +13,8 @@
 //      together, release them and write the scores to the block's scratch (L2)
 //      while the next tile's products run;
 //   2. terms in place, a row a warp; an exponential is its polynomial in
-//      truncated 32-bit products plus one bit of a table in shared memory that
-//      makes it exact (exp_term_estimate);
+//      double precision plus one bit of a table in shared memory that
+//      makes it exact (exp_term_floor);
 //   3. weights of 128 keys into shared memory as two swizzled byte planes, and
 //      128 dims x 128 rows (both weight planes) x 32 positions a product, six
 //      plane pairs into four diagonals that stay in TMEM over all keys.
@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
     const uint32_t lane = tid & 31;
     for (uint32_t c = blockIdx.x * kPackThreads + tid; c < kPtFar; c += gridDim.x * kPackThreads) {
       const uint32_t d = kExpExactBelow + c;
-      const uint32_t bits = __ballot_sync(0xffffffffu, exp_term_near(d) != exp_term_estimate(d));
+      const uint32_t bits = __ballot_sync(0xffffffffu, exp_term_near(d) != exp_term_floor(d));
       if (lane == 0) sc.exp_bits[c / 32] = bits;
     }
   }
@@ -189,7 +189,7 @@ __device__ __forceinline__ void terms_by_table(const int4 (&x)[2], int32_t top, 
   for (uint32_t u = 0; u < 8; ++u) {
     d[u] = (uint32_t)top - (uint32_t)v[u];
     const uint32_t c = d[u] - kExpExactBelow, i = min(c, kPtFar - 1);
-    const uint32_t t = exp_term_estimate(d[u]) + (__funnelshift_r(bits[i >> 5], 0, i) & 1);
+    const uint32_t t = exp_term_floor(d[u]) + (__funnelshift_r(bits[i >> 5], 0, i) & 1);
     e[u] = c < kPtFar ? t : 0;
   }
 }

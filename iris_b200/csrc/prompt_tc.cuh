@@ -9,7 +9,7 @@ namespace iris {
 
 struct PromptTcScratch {
   uint8_t *qp, *kp, *vt;  // byte planes
-  uint32_t* exp_bits;     // corrections of exp_term_estimate
+  uint32_t* exp_bits;     // corrections of exp_term_floor
   uint32_t* wide;         // [flags], non-zero where a packing block met a value past 24 bits
   uint64_t tpitch;        // tokens a row of vt
   uint32_t pack_blocks, flags;

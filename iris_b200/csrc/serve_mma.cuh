@@ -16,6 +16,7 @@
 // memory to the matrix unit through registers only, whatever page they lie in.
 #pragma once
 #include "common.cuh"
+#include "layers.cuh"
 #include "serve_attn.cuh"
 
 namespace iris {
@@ -211,6 +212,86 @@ __device__ __forceinline__ uint32_t term_of(int32_t score, int32_t top) {
   return d ? exp_term_near(d) : kTermTop;
 }
 
+// A warp turns the scores of a row into their terms, in place: key t lies at row +
+// (t / 128) * block + t % 128, keys from `count` on are hidden, terms are written
+// up to `stored` (both multiples of 4). Eight scores a lane and turn, with the
+// next eight loaded ahead (x holds the first on entry; then those of `next`,
+// where that is not NULL). Terms whose estimate is in doubt - the few keys near
+// the maximum, and hardly any far from it - go on a list (place and distance in
+// one word) and are done 32 at a time, exactly. Returns this lane's part of the
+// sum and the first place of the maximum.
+constexpr uint32_t kTermList = 512;    // words of shared memory a warp
+constexpr uint32_t kTermTiles = 32;    // key tiles that a list's places reach over
+struct RowTerms {
+  uint64_t sum;
+  uint32_t first;
+};
+__device__ __forceinline__ void row_load(int4 (&z)[2], const int32_t* row, uint32_t block, uint32_t kt, uint32_t count,
+                                         uint32_t lane) {
+  const int32_t* at = row + (uint64_t)kt * block + 4 * lane;
+  const uint32_t t = kt * 128 + 4 * lane;
+  const int4 hidden = make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
+  z[0] = t < count ? __ldcg((const int4*)at) : hidden;
+  z[1] = t + 128 < count ? __ldcg((const int4*)(at + block)) : hidden;
+}
+__device__ __forceinline__ RowTerms row_terms(int32_t* row, uint32_t block, uint32_t count, uint32_t stored, int32_t top,
+                                              uint32_t* list, uint32_t lane, int4 (&x)[2], const int32_t* next) {
+  RowTerms out{0, UINT32_MAX};
+  uint32_t listed = 0, base = 0;
+  auto drain = [&] {
+    __syncwarp();
+    for (uint32_t n = lane; n < listed; n += 32) {
+      const uint32_t at = base * 128 + (list[n] >> 20), d = list[n] & ((1u << 20) - 1);
+      const uint32_t z = d ? exp_term_near(d) : kTermTop;
+      if (!d) out.first = min(out.first, at);
+      out.sum += kept_term(z);
+      __stcg((uint32_t*)row + (uint64_t)(at / 128) * block + at % 128, z);
+    }
+    listed = 0;
+    __syncwarp();
+  };
+  const uint32_t tiles = (max(count, stored) + 127) / 128;
+  for (uint32_t kt = 0; kt < tiles; kt += 2) {
+    if (kt - base + 2 > kTermTiles) {
+      drain();
+      base = kt;
+    }
+    int4 y[2];
+    if (kt + 2 < tiles) row_load(y, row, block, kt + 2, count, lane);
+    else if (next) row_load(y, next, block, 0, count, lane);
+    const int32_t v[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+    uint32_t e[8], d[8], doubts = 0;
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) {
+      d[u] = (uint32_t)top - (uint32_t)v[u];
+      bool doubt;
+      const uint32_t z = exp_term_estimate(d[u], &doubt);
+      const bool some = d[u] < kExpTerms;
+      e[u] = some && !doubt ? z : 0;
+      doubts |= (some && doubt ? 1u : 0u) << u;
+    }
+    out.sum += ((uint64_t)e[0] + e[1] + ((uint64_t)e[2] + e[3])) + ((uint64_t)e[4] + e[5] + ((uint64_t)e[6] + e[7]));
+    const uint32_t t = kt * 128 + 4 * lane;
+    uint32_t* at = (uint32_t*)row + (uint64_t)kt * block + 4 * lane;
+    if (t < stored) __stcg((uint4*)at, make_uint4(e[0], e[1], e[2], e[3]));
+    if (t + 128 < stored) __stcg((uint4*)(at + block), make_uint4(e[4], e[5], e[6], e[7]));
+    for (uint32_t who; (who = __ballot_sync(0xffffffffu, doubts != 0)) != 0; doubts &= doubts - 1) {
+      if (doubts) {
+        const uint32_t u = __ffs(doubts) - 1;
+        uint32_t dist = d[0];
+#pragma unroll
+        for (uint32_t o = 1; o < 8; ++o) dist = u == o ? d[o] : dist;
+        list[listed + __popc(who & ((1u << lane) - 1))] = ((kt - base + u / 4) * 128 + 4 * lane + u % 4) << 20 | dist;
+      }
+      listed += __popc(who);
+    }
+    if (listed + 256 > kTermList) drain(), base = kt + 2;
+    x[0] = y[0], x[1] = y[1];
+  }
+  drain();
+  return out;
+}
+
 // A row's divisor: its exact sum and floor(2^63 / sum) (at most 2^31: the
 // maximum's own term makes the sum at least 2^32); 0 where nothing is seen.
 struct RowSum {
@@ -253,12 +334,6 @@ __device__ __forceinline__ void weights_of(const uint32_t (&term)[8], uint32_t r
     }
   }
 }
-__device__ __forceinline__ int32_t weight_of(uint32_t term, uint32_t recip, uint64_t sum) {
-  const uint32_t y = (uint32_t)(((uint64_t)term * recip) >> 32) + (1u << 14);
-  if (((y + 3) & 0x7FFF) <= 3) return recip ? exact_weight(term, sum) : 0;
-  return (int32_t)(y >> 15);
-}
-
 // ---- value sums ---------------------------------------------------------------------
 //
 // sum_t w_t v_t with the first maximum's weight left out (it takes the residual

@@ -158,6 +158,7 @@ __global__ void __launch_bounds__(kTreeThreads) tree_terms_kernel(IrisTreeAttent
   const uint32_t r = blockIdx.z, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t row = blockIdx.x * kTreeWarps + warp;  // node * heads + head
   const uint32_t seg = blockIdx.y;
+  __shared__ uint32_t lists[kTreeWarps][kTermList];
   pdl_wait();
   pdl_trigger();
   const TreeRequest q(a, r);
@@ -170,25 +171,27 @@ __global__ void __launch_bounds__(kTreeThreads) tree_terms_kernel(IrisTreeAttent
   top = __reduce_max_sync(0xffffffffu, top);
   const bool ask = top < INT32_MIN + (1 << 20);
   const uint32_t last = (q.count + 15) / 16 * 16;  // scores are written up to here
-  const uint32_t t1 = min(seg * kTreeSegment + kTreeSegment, (q.count + 31) / 32 * 32);
-  int32_t* s = sc.scores + id * sc.pitch;
+  const uint32_t s0 = seg * kTreeSegment, count = min(kTreeSegment, last - s0);
+  const uint32_t stored = min(kTreeSegment, (q.count + 31) / 32 * 32 - s0);
+  int32_t* s = sc.scores + id * sc.pitch + s0;
   uint64_t sum = 0;
   uint32_t first = UINT32_MAX;
-  for (uint32_t t = seg * kTreeSegment + 4 * lane; t < t1; t += 128) {
-    int4 x = t < last ? *(const int4*)(s + t) : make_int4(INT32_MIN, INT32_MIN, INT32_MIN, INT32_MIN);
-    const int32_t v[4] = {x.x, x.y, x.z, x.w};
-    uint32_t e[4];
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u) {
-      e[u] = term_of(v[u], top);
-      if (ask && !(t + u < q.count &&
-                   page_row(a.table + (size_t)r * a.width, a.width, a.page_size, a.pages, q.base + t + u) >= 0 &&
-                   is_visible(a, q, node, q.base + t + u)))
-        e[u] = 0;
-      sum += kept_term(e[u]);
-      if (e[u] == kTermTop) first = min(first, t + u);
+  if (!ask) {
+    int4 x[2];
+    row_load(x, s, 128, 0, count, lane);
+    const RowTerms t = row_terms(s, 128, count, stored, top, lists[warp], lane, x, nullptr);
+    sum = t.sum;
+    if (t.first != UINT32_MAX) first = s0 + t.first;
+  } else {
+    for (uint32_t t = lane; t < stored; t += 32) {
+      const uint32_t key = q.base + s0 + t;
+      const bool seen = key < q.keys && page_row(a.table + (size_t)r * a.width, a.width, a.page_size, a.pages, key) >= 0 &&
+                        is_visible(a, q, node, key);
+      const uint32_t e = seen ? term_of(__ldcg(s + t), top) : 0;
+      if (e == kTermTop) first = min(first, s0 + t);
+      sum += kept_term(e);
+      __stcg((uint32_t*)s + t, e);
     }
-    *(uint4*)(s + t) = make_uint4(e[0], e[1], e[2], e[3]);
   }
   sum = (uint64_t)warp_sum_i64((int64_t)sum);
   first = __reduce_min_sync(0xffffffffu, first);
@@ -286,9 +289,9 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_values_kernel(IrisTreeAt
         const uint4 lo = *(const uint4*)s, hi = *(const uint4*)(s + 16);
         const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
         const uint32_t at = s0 + st * 32 + 4 * (lane & 3);
+        weights_of(e, recip_s[i], sum_s[i], x);
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) {
-          x[j] = weight_of(e[j], recip_s[i], sum_s[i]);
           if (at + (j >> 2) * 16 + (j & 3) == first_s[i]) x[j] = 0;  // its weight comes last
           total += x[j];
         }

@@ -2,12 +2,17 @@
 #include "../../iris_b200/csrc/detnum.cuh"
 
 extern "C" {
-// term[d] = exp_term_near(d), estimate[d] = exp_term_estimate(d) and want[d] =
-// softmax_exp_term_act of a score d below the maximum, for 1 <= d < 2^20.
-void serving_exp_terms(uint32_t* term, uint32_t* estimate, int64_t* want) {
+// term[d] = exp_term_near(d), estimate[d] = exp_term_estimate(d), doubt[d] what
+// it says of itself, floor[d] = exp_term_floor(d) and want[d] = softmax_exp_term_act of a score d below the
+// maximum, for 1 <= d < 2^20.
+void serving_exp_terms(uint32_t* term, uint32_t* estimate, uint8_t* doubt, uint32_t* floor,
+                       int64_t* want) {
   for (uint32_t d = 1; d < 1u << 20; ++d) {
+    bool may_be_wrong;
     term[d] = iris::exp_term_near(d);
-    estimate[d] = d >= iris::kExpExactBelow ? iris::exp_term_estimate(d) : 0;
+    estimate[d] = iris::exp_term_estimate(d, &may_be_wrong);
+    doubt[d] = may_be_wrong;
+    floor[d] = iris::exp_term_floor(d);
     want[d] = iris::softmax_exp_term_act(-(int32_t)d, 0);
   }
 }

@@ -1,6 +1,7 @@
 """The serving kernels' exponential on every distance it takes, as host code:
-the 32-bit form equals softmax_exp_term, and the estimate that one bit corrects
-is it or one less from its first distance on."""
+the 32-bit form equals softmax_exp_term, and so does the estimate wherever it
+has no doubt, which is nearly everywhere far from the maximum; the floor that
+one bit corrects is it or one less from its first distance on."""
 import ctypes as C
 import os
 import subprocess
@@ -18,10 +19,14 @@ def test_every_exponential(tmp_path):
                     os.path.join(HERE, "native", "serving_shim.cc")], check=True)
     L = C.CDLL(str(so))
     n = 1 << 20
-    term, estimate, want = np.zeros(n, np.uint32), np.zeros(n, np.uint32), np.zeros(n, np.int64)
-    L.serving_exp_terms(*(a.ctypes.data_as(C.c_void_p) for a in (term, estimate, want)))
+    term, estimate, doubt, floor, want = (np.zeros(n, t) for t in (np.uint32, np.uint32, np.uint8, np.uint32, np.int64))
+    L.serving_exp_terms(*(a.ctypes.data_as(C.c_void_p) for a in (term, estimate, doubt, floor, want)))
     assert np.array_equal(term[1:].astype(np.int64), want[1:])
+    sure = doubt == 0
+    sure[0] = False
+    assert np.array_equal(estimate[sure].astype(np.int64), want[sure])
+    assert doubt[1:].mean() < 0.25 and doubt[500000:].mean() < 0.01
     below = L.serving_exact_below()
-    off = want[below:] - estimate[below:].astype(np.int64)
-    assert off.min() >= 0 and off.max() <= 1
+    off = want[below:] - floor[below:].astype(np.int64)
+    assert below % 32 == 0 and off.min() >= 0 and off.max() <= 1
     assert np.array_equal(ref.exp_term(np.arange(1, n)), want[1:])  # the tests' own restatement
