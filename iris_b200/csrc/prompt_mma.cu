@@ -302,30 +302,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
       const bool open = p.base + t0 + 15 <= q0 && (!a.window || p.base + t0 >= window_start(q1, a.window));
 #pragma unroll 1
       for (uint32_t nt0 = 0; nt0 < NT; nt0 += 4) {
-        int32_t best[4][2];
-#pragma unroll
-        for (uint32_t n = 0; n < 4; ++n) best[n][0] = best[n][1] = INT32_MIN;
+        int32_t x[4][4];
+        key_scores<4>(pa, pb, tile, q_wide, nt0, lane, a.scale_q32, x);
         int32_t* out = scores + (uint64_t)(8 * nt0 + 2 * (lane & 3)) * sc.pitch + t0 + (lane >> 2);
-        key_scores<4>(pa, pb, tile, q_wide, nt0, lane, a.scale_q32, [&](uint32_t n, uint32_t e, int32_t x) {
-          if (!open) {
-            const int32_t q = s.query[8 * (nt0 + n) + 2 * (lane & 3) + (e & 1)];
-            const uint32_t key = e >> 1 ? kb : ka;
-            if (q < 0 || key > (uint32_t)q || key < window_start((uint32_t)q, a.window)) x = INT32_MIN;
-          }
-          __stcg(out + (8 * n + (e & 1)) * sc.pitch + 8 * (e >> 1), x);
 #pragma unroll
-          for (uint32_t m = 0; m < 4; ++m)
-            if (m == n) best[m][e & 1] = max(best[m][e & 1], x);
-        });
+        for (uint32_t n = 0; n < 4; ++n)
+#pragma unroll
+          for (uint32_t e = 0; e < 4; ++e) {
+            if (!open) {
+              const int32_t q = s.query[8 * (nt0 + n) + 2 * (lane & 3) + (e & 1)];
+              const uint32_t key = e >> 1 ? kb : ka;
+              if (q < 0 || key > (uint32_t)q || key < window_start((uint32_t)q, a.window)) x[n][e] = INT32_MIN;
+            }
+            __stcg(out + (8 * n + (e & 1)) * sc.pitch + 8 * (e >> 1), x[n][e]);
+          }
 #pragma unroll
         for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
           for (uint32_t e = 0; e < 2; ++e) {
-            int32_t x = best[n][e];
-            x = max(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = max(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = max(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            if (lane < 4) atomicMax(&s.top[8 * (nt0 + n) + 2 * lane + e], x);
+            int32_t m = max(x[n][e], x[n][e + 2]);
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            if (lane < 4) atomicMax(&s.top[8 * (nt0 + n) + 2 * lane + e], m);
           }
       }
     }

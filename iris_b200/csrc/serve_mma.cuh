@@ -165,26 +165,9 @@ __device__ __forceinline__ int32_t diagonal_score(const int32_t (&v)[7], uint32_
   return score_of((int32_t)(s >> 32), (uint32_t)s, scale);
 }
 
-// Scores of 16 keys against rows [8 nt0, 8 nt0 + 8 NT) of a tile: emit(n, e,
-// score) for the lane's four elements of each n: row 8 (nt0 + n) + 2 (lane % 4)
-// + (e & 1), key lane / 4 + 8 (e >> 1).
-template <uint32_t NT, class Emit>
-__device__ __forceinline__ void key_scores(const int32_t* k0, const int32_t* k1, const QueryTile& q, bool q_wide,
-                                           uint32_t nt0, uint32_t lane, uint32_t scale, const Emit& emit) {
-  if (!q_wide) {
-    int32_t acc[NT][5][4];
-    const uint32_t wide = key_products<3, NT>(k0, k1, q, nt0, lane, acc);
-    if (!__any_sync(0xffffffffu, wide != 0)) {
-#pragma unroll
-      for (uint32_t n = 0; n < NT; ++n)
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e) {
-          const int32_t v[5] = {acc[n][0][e], acc[n][1][e], acc[n][2][e], acc[n][3][e], acc[n][4][e]};
-          emit(n, e, diagonal_score(v, scale));
-        }
-      return;
-    }
-  }
+template <uint32_t NT>
+static __device__ __noinline__ void wide_key_scores(const int32_t* k0, const int32_t* k1, const QueryTile& q,
+                                                    uint32_t nt0, uint32_t lane, uint32_t scale, int32_t (&s)[NT][4]) {
 #pragma unroll 1
   for (uint32_t n = 0; n < NT; ++n) {
     int32_t acc[1][7][4];
@@ -193,9 +176,30 @@ __device__ __forceinline__ void key_scores(const int32_t* k0, const int32_t* k1,
     for (uint32_t e = 0; e < 4; ++e) {
       const int32_t v[7] = {acc[0][0][e], acc[0][1][e], acc[0][2][e], acc[0][3][e],
                             acc[0][4][e], acc[0][5][e], acc[0][6][e]};
-      emit(n, e, diagonal_score(v, scale));
+      s[n][e] = diagonal_score(v, scale);
     }
   }
+}
+
+// Scores of 16 keys against rows [8 nt0, 8 nt0 + 8 NT) of a tile: the lane's four
+// elements of each n are row 8 (nt0 + n) + 2 (lane % 4) + (e & 1), key lane / 4 +
+// 8 (e >> 1).
+template <uint32_t NT>
+__device__ __forceinline__ void key_scores(const int32_t* k0, const int32_t* k1, const QueryTile& q, bool q_wide,
+                                           uint32_t nt0, uint32_t lane, uint32_t scale, int32_t (&s)[NT][4]) {
+  if (!q_wide) {
+    int32_t acc[NT][5][4];
+    const uint32_t wide = key_products<3, NT>(k0, k1, q, nt0, lane, acc);
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        const int32_t v[5] = {acc[n][0][e], acc[n][1][e], acc[n][2][e], acc[n][3][e], acc[n][4][e]};
+        s[n][e] = diagonal_score(v, scale);
+      }
+    if (!__any_sync(0xffffffffu, wide != 0)) return;
+  }
+  wide_key_scores<NT>(k0, k1, q, nt0, lane, scale, s);
 }
 
 // ---- weights ----------------------------------------------------------------------
@@ -373,6 +377,42 @@ __device__ __forceinline__ uint32_t value_products(const int2 (&x)[8], const uin
     }
   }
   return wide;
+}
+
+// A value fragment (16 dimensions x 32 positions) made once for all the warps
+// that take it: planes [plane][lane] of four words. Returns past_24_bits.
+template <uint32_t P>
+__device__ __forceinline__ uint32_t put_value_fragment(uint4* frag, const int2 (&x)[8], uint32_t lane) {
+  uint32_t p[4], q[4], r[4], t[4];
+  split_planes(x[0].x, x[1].x, x[2].x, x[3].x, p);
+  split_planes(x[0].y, x[1].y, x[2].y, x[3].y, q);
+  split_planes(x[4].x, x[5].x, x[6].x, x[7].x, r);
+  split_planes(x[4].y, x[5].y, x[6].y, x[7].y, t);
+#pragma unroll
+  for (uint32_t i = 0; i < P; ++i) frag[i * 32 + lane] = make_uint4(p[i], q[i], r[i], t[i]);
+  return P == 3 ? past_24_bits(p) | past_24_bits(q) | past_24_bits(r) | past_24_bits(t) : 0;
+}
+// acc += that fragment against the weights of 8 NT rows.
+template <uint32_t P, uint32_t NT>
+__device__ __forceinline__ void fragment_products(const uint4* frag, const uint2* w, uint32_t lane,
+                                                  int32_t (&acc)[NT][P + 1][4]) {
+  uint32_t a[P][4];
+#pragma unroll
+  for (uint32_t i = 0; i < P; ++i) {
+    const uint4 v = frag[i * 32 + lane];
+    a[i][0] = v.x, a[i][1] = v.y, a[i][2] = v.z, a[i][3] = v.w;
+  }
+#pragma unroll
+  for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint2 b = w[(n * 2 + j) * 32 + lane];
+#pragma unroll
+      for (uint32_t i = 0; i < P; ++i) {
+        if (i + 1 < P) mma_i8<false, false>(acc[n][i + j], a[i], b);
+        else mma_i8<true, false>(acc[n][i + j], a[i], b);
+      }
+    }
 }
 
 // The lane's fragment words of eight weights (positions 4 c .. 4 c + 3 and 16 +

@@ -39,8 +39,9 @@ struct TreeScratch {
   uint32_t* seg_first; // [rows * heads][segs]
   int64_t* acc;        // [rows * heads][d]
   int32_t* wsum;       // [rows * heads]
-  uint32_t* done;      // [requests * kv_heads]
+  uint32_t* done;      // [requests][kv_heads][groups]: finished blocks of the third launch
   uint32_t pitch, chunk, chunks, segs;
+  uint32_t vchunk, vchunks, groups;  // keys and row groups of the third launch's blocks
 };
 
 // One request's part of the call: its keys from `base` on (a multiple of 64; a
@@ -73,8 +74,11 @@ __device__ __forceinline__ bool is_visible(const IrisTreeAttention& a, const Tre
 }
 
 __global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAttention a, TreeScratch sc) {
+  constexpr uint32_t NT = kTreeTile / 8;
   extern __shared__ __align__(16) uint8_t tree_sm[];
   uint2* frag = (uint2*)tree_sm;  // [tile / 8][steps][4][32]
+  __shared__ __align__(16) uint64_t row_at[kTreeTile];  // the rows' scores
+  __shared__ uint32_t row_node[kTreeTile];
   __shared__ int32_t row_max[kTreeTile];
   __shared__ uint32_t q_wide;
   const uint32_t chunk = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
@@ -88,7 +92,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAt
       sc.acc[id * a.head_dim + x] = 0;
       if (x == 0) sc.wsum[id] = 0;
     }
-    if (tid == 0) sc.done[r * a.kv_heads + g] = 0;
+    for (uint32_t i = tid; i < sc.groups; i += kTreeThreads) sc.done[((size_t)r * a.kv_heads + g) * sc.groups + i] = 0;
   }
   if (key0 >= q.keys) return;
   const uint32_t key1 = min(key0 + sc.chunk, q.base + (q.count + 15) / 16 * 16);
@@ -97,18 +101,25 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAt
   const QueryTile tile{frag, steps};
   for (uint32_t f0 = 0; f0 < rows; f0 += kTreeTile) {
     if (f0) __syncthreads();
-    if (tid < kTreeTile) row_max[tid] = INT32_MIN;
+    if (tid < kTreeTile) {
+      // (rows past the last one repeat it)
+      const uint32_t f = min(f0 + tid, rows - 1), node = f / q.group, head = g * q.group + f % q.group;
+      row_node[tid] = node;
+      row_at[tid] = ((size_t)(q.begin + node) * a.heads + head) * sc.pitch;
+      row_max[tid] = INT32_MIN;
+    }
     if (tid == 0) q_wide = 0;
     __syncthreads();
-    for (uint32_t u = warp; u < kTreeTile / 8 * steps; u += kTreeWarps) {
-      const uint32_t nt = u / steps, f = f0 + 8 * nt + (lane >> 2);
-      const int32_t* src = nullptr;
-      if (f < rows)
-        src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+    for (uint32_t u = warp; u < NT * steps; u += kTreeWarps) {
+      const uint32_t nt = u / steps, i = 8 * nt + (lane >> 2), f = min(f0 + i, rows - 1);
+      const int32_t* src = a.q + (size_t)(q.begin + row_node[i]) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
       if (put_query_fragment(frag, steps, nt, u % steps, lane, src)) q_wide = 1;
     }
     __syncthreads();
     const bool wide = q_wide != 0;
+    int32_t best[NT][2];
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n) best[n][0] = best[n][1] = INT32_MIN;
     for (uint32_t t0 = key0 + 16 * warp; t0 < key1; t0 += 16 * kTreeWarps) {
       const uint32_t ka = t0 + (lane >> 2), kb = ka + 8;
       const int64_t ra = ka < q.keys ? page_row(table, a.width, a.page_size, a.pages, ka) : -1;
@@ -117,37 +128,45 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAt
       const int32_t* pb = rb >= 0 ? a.k_pages + (size_t)rb * kvd + g * a.head_dim : nullptr;
       // keys that every row sees need no look at the masks
       const bool open = t0 + 16 <= q.held && !a.window && __all_sync(0xffffffffu, ra >= 0 && rb >= 0);
-      int32_t best[2] = {INT32_MIN, INT32_MIN};
-      uint32_t done = 0;
-      key_scores<kTreeTile / 8>(pa, pb, tile, wide, 0, lane, a.scale_q32, [&](uint32_t n, uint32_t e, int32_t s) {
-        const uint32_t f = f0 + 8 * n + 2 * (lane & 3) + (e & 1), key = e >> 1 ? kb : ka;
-        if (f < rows) {
-          if (!open && !((e >> 1 ? rb : ra) >= 0 && is_visible(a, q, f / q.group, key))) s = INT32_MIN;
-          const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-          sc.scores[id * sc.pitch + (key - q.base)] = s;
-          best[e & 1] = max(best[e & 1], s);
-        }
-        if (++done % 4 == 0) {  // the four elements of these eight rows
-          int32_t x = best[0], y = best[1];
+      int32_t x[NT][4];
+      key_scores<NT>(pa, pb, tile, wide, 0, lane, a.scale_q32, x);
+      if (!open) {
+#pragma unroll 1
+        for (uint32_t u = 0; u < 2 * NT; ++u) {
+          const uint32_t node = row_node[8 * (u / 2) + 2 * (lane & 3) + (u & 1)];
+          const bool sa = ra >= 0 && is_visible(a, q, node, ka), sb = rb >= 0 && is_visible(a, q, node, kb);
 #pragma unroll
-          for (uint32_t o = 4; o <= 16; o <<= 1) {
-            x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
-            y = max(y, __shfl_xor_sync(0xffffffffu, y, o));
-          }
-          if (lane < 4) {
-            atomicMax(&row_max[8 * n + 2 * lane], x);
-            atomicMax(&row_max[8 * n + 2 * lane + 1], y);
-          }
-          best[0] = best[1] = INT32_MIN;
+          for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+            for (uint32_t e = 0; e < 2; ++e)
+              if (2 * n + e == u) {
+                if (!sa) x[n][e] = INT32_MIN;
+                if (!sb) x[n][e + 2] = INT32_MIN;
+              }
         }
-      });
+      }
+      int32_t* out = sc.scores + (ka - q.base);
+#pragma unroll
+      for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+        for (uint32_t e = 0; e < 2; ++e) {
+          int32_t* o = out + row_at[8 * n + 2 * (lane & 3) + e];
+          o[0] = x[n][e];
+          o[8] = x[n][e + 2];
+          best[n][e] = max(best[n][e], max(x[n][e], x[n][e + 2]));
+        }
     }
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+      for (uint32_t e = 0; e < 2; ++e) {
+        int32_t x = best[n][e];
+#pragma unroll
+        for (uint32_t o = 4; o <= 16; o <<= 1) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+        if (lane < 4) atomicMax(&row_max[8 * n + 2 * lane + e], x);
+      }
     __syncthreads();
-    if (tid < kTreeTile && f0 + tid < rows) {
-      const uint32_t f = f0 + tid;
-      const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-      sc.chunk_max[id * sc.chunks + chunk] = row_max[tid];
-    }
+    if (tid < kTreeTile && f0 + tid < rows) sc.chunk_max[row_at[tid] / sc.pitch * sc.chunks + chunk] = row_max[tid];
   }
 }
 
@@ -201,137 +220,187 @@ __global__ void __launch_bounds__(kTreeThreads) tree_terms_kernel(IrisTreeAttent
   }
 }
 
-template <uint32_t P>
-__device__ __forceinline__ uint32_t tree_value_tile(const IrisTreeAttention& a, const TreeScratch& sc,
-                                                    const TreeRequest& q, const uint2* w, const int64_t* row_s,
-                                                    uint32_t steps, uint32_t g, uint32_t f0, uint32_t dt,
-                                                    uint32_t step0, uint32_t step_by, uint32_t lane) {
-  constexpr uint32_t NT = kTreeTile / 8;
-  int32_t acc[NT][P + 1][4] = {};
-  const int32_t* v = a.v_pages + g * a.head_dim + 16 * dt + 2 * (lane >> 2);
+// Values: a block takes up to 16 NT rows (8 NT for heads past 128 values) of one
+// request and K/V head, and a chunk of its keys in stages of 64: the stage's
+// values as byte-plane fragments and its weights go to shared memory, made once
+// for all sixteen warps, which then take 16 dimensions x 8 NT rows each (where
+// those are fewer than the warps, every other 32 keys too). The next stage's
+// rows are in registers while this one's products run.
+constexpr uint32_t kValueThreads = 512, kValueWarps = kValueThreads / 32, kValueKeys = 64;
+
+struct ValueShared {
+  uint64_t sum[64];
+  uint32_t recip[64], first[64];
+  uint32_t id[64];  // the rows' places in the scratch, UINT32_MAX past the last
+  uint32_t wide, last;
+};
+
+template <uint32_t P, uint32_t NT>
+__device__ __noinline__ bool tree_chunk_values(const IrisTreeAttention& a, const TreeScratch& sc, ValueShared& s,
+                                               uint4* frag, uint2* wts, const uint32_t* row_s, uint32_t s0,
+                                               uint32_t count, uint32_t g) {
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t dts = a.head_dim / 16, halves = dts <= 8 ? 2 : 1, units = dts * halves;
+  const uint32_t split = units * 2 <= kValueWarps ? 2 : 1, unit = warp % units, part = warp / units;
+  const uint32_t dt = unit % dts, half = unit / dts;
+  const bool works = part < split;
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
-  uint32_t wide = 0;
-  for (uint32_t st = step0; st < steps; st += step_by) {
-    int2 x[8];
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const int64_t row = row_s[st * 32 + (i >> 2) * 16 + 4 * (lane & 3) + (i & 3)];
-      x[i] = row >= 0 ? *(const int2*)(v + (size_t)row * kvd) : make_int2(0, 0);
-    }
-    wide |= value_products<P, NT>(x, w + st * (NT * 64), lane, acc);
-  }
-  if (P == 3 && __any_sync(0xffffffffu, wide != 0)) return 1;
-  const uint32_t rows = q.nodes * q.group;
+  const uint32_t vfrags = dts * 2, wfrags = NT * halves * 2;  // fragments a stage
+  const uint32_t stages = (count + kValueKeys - 1) / kValueKeys;
+  int32_t acc[NT][P + 1][4];
 #pragma unroll
   for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-      const uint32_t f = f0 + 8 * n + 2 * (lane & 3) + (e & 1);
-      if (f < rows) {
-        int32_t d[P + 1];
+    for (uint32_t d = 0; d < P + 1; ++d)
 #pragma unroll
-        for (uint32_t j = 0; j < P + 1; ++j) d[j] = acc[n][j][e];
-        const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-        atomicAdd((unsigned long long*)(sc.acc + id * a.head_dim + 16 * dt + 2 * (lane >> 2) + (e >> 1)),
-                  (unsigned long long)diagonal_sum(d));
-      }
+      for (uint32_t e = 0; e < 4; ++e) acc[n][d][e] = 0;
+  // this warp's fragments of a stage: values 16 wide u / 2, keys of half u & 1 (one
+  // or, for wide heads, two), weights of rows 8 (u / 2) ..
+  int2 x[8];
+  uint4 t[2];
+  const uint32_t wn = warp / 2, wst = warp & 1, wrow = 8 * wn + (lane >> 2);
+  const bool weighs = warp < wfrags && s.id[wrow & 63] != UINT32_MAX;
+  auto load_values = [&](uint32_t st, uint32_t u) {
+    const int32_t* v = a.v_pages + g * a.head_dim + 16 * (u / 2) + 2 * (lane >> 2);
+    const uint32_t* row = row_s + st * kValueKeys + (u & 1) * 32 + 4 * (lane & 3);
+    const uint4 lo = *(const uint4*)row, hi = *(const uint4*)(row + 16);
+    const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) x[i] = *(const int2*)(v + (size_t)r[i] * kvd);
+  };
+  auto load_terms = [&](uint32_t st) {
+    t[0] = t[1] = make_uint4(0, 0, 0, 0);
+    const uint32_t at = st * kValueKeys + wst * 32;
+    if (weighs && at < count) {
+      const int32_t* e = sc.scores + (size_t)s.id[wrow] * sc.pitch + s0 + at + 4 * (lane & 3);
+      t[0] = __ldcg((const uint4*)e);
+      t[1] = __ldcg((const uint4*)(e + 16));
     }
-  return 0;
+  };
+  uint32_t wide = 0;
+  int32_t total = 0;
+  if (warp < vfrags) load_values(0, warp);
+  load_terms(0);
+  for (uint32_t st = 0; st < stages; ++st) {
+    uint4* fb = frag + (size_t)(st & 1) * vfrags * (P * 32);
+    uint2* wb = wts + (size_t)(st & 1) * wfrags * 64;
+    // fragments: [half of the keys][dimension tile], weights [half of the keys][row / 8]
+    for (uint32_t u = warp; u < vfrags; u += kValueWarps) {
+      if (u != warp) load_values(st, u);
+      wide |= put_value_fragment<P>(fb + ((u & 1) * dts + u / 2) * (P * 32), x, lane);
+    }
+    if (warp < wfrags) {
+      const uint32_t e[8] = {t[0].x, t[0].y, t[0].z, t[0].w, t[1].x, t[1].y, t[1].z, t[1].w};
+      int32_t w[8];
+      weights_of(e, weighs ? s.recip[wrow] : 0, s.sum[wrow & 63], w);
+      const uint32_t at = s0 + st * kValueKeys + wst * 32 + 4 * (lane & 3), first = s.first[wrow & 63];
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        if (at + (j >> 2) * 16 + (j & 3) == first) w[j] = 0;  // its weight comes last
+        total += w[j];
+      }
+      put_weight_fragment(wb + (wst * (wfrags / 2) + wn) * 64, lane, w);
+    }
+    if (st + 1 < stages) {
+      if (warp < vfrags) load_values(st + 1, warp);
+      load_terms(st + 1);
+    }
+    __syncthreads();
+    if (works)
+      for (uint32_t h = part; h < 2; h += split)
+        fragment_products<P, NT>(fb + (h * dts + dt) * (P * 32), wb + (h * (wfrags / 2) + half * NT) * 64, lane, acc);
+  }
+  if (P == 3) {
+    if (wide) s.wide = 1;
+    __syncthreads();
+    if (s.wide) return true;
+  }
+  if (warp < wfrags) {
+    total += __shfl_xor_sync(0xffffffffu, total, 1);
+    total += __shfl_xor_sync(0xffffffffu, total, 2);
+    if ((lane & 3) == 0 && weighs && total) atomicAdd(sc.wsum + s.id[wrow], total);
+  }
+  if (works) {
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+      for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t i = (half * NT + n) * 8 + 2 * (lane & 3) + (e & 1);
+        if (s.id[i] != UINT32_MAX) {
+          int32_t d[P + 1];
+#pragma unroll
+          for (uint32_t j = 0; j < P + 1; ++j) d[j] = acc[n][j][e];
+          atomicAdd((unsigned long long*)(sc.acc + (size_t)s.id[i] * a.head_dim + 16 * dt + 2 * (lane >> 2) + (e >> 1)),
+                    (unsigned long long)diagonal_sum(d));
+        }
+      }
+  }
+  return false;
 }
 
-__global__ void __launch_bounds__(kTreeThreads, 2) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
-  constexpr uint32_t NT = kTreeTile / 8;
+template <uint32_t NT>
+__global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
   extern __shared__ __align__(16) uint8_t tree_sm[];
-  uint2* w = (uint2*)tree_sm;                                   // [chunk / 32][NT][2][32]
-  int64_t* row_s = (int64_t*)(w + (size_t)sc.chunk / 32 * NT * 64);  // [chunk]
-  __shared__ uint64_t sum_s[kTreeTile];
-  __shared__ uint32_t recip_s[kTreeTile], first_s[kTreeTile], last_s;
-  const uint32_t chunk = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+  __shared__ ValueShared s;
+  const uint32_t dts = a.head_dim / 16, tile = 8 * NT * (dts <= 8 ? 2 : 1);  // rows
+  const uint32_t groups = (a.nodes * (a.heads / a.kv_heads) + tile - 1) / tile;
+  const uint32_t chunk = blockIdx.x, g = blockIdx.y / groups, f0 = blockIdx.y % groups * tile, r = blockIdx.z;
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t* row_s = (uint32_t*)tree_sm;                    // [vchunk]: pool rows of the chunk's keys
+  uint4* frag = (uint4*)(row_s + sc.vchunk);               // [2][2][dts][4][32]
+  uint2* wts = (uint2*)(frag + (size_t)4 * dts * 4 * 32);  // [2][2][tile / 8][2][32]
   const TreeRequest q(a, r);
-  const uint32_t rows = q.nodes * q.group, key0 = q.base + chunk * sc.chunk, s0 = chunk * sc.chunk;
-  const uint32_t chunks = (q.count + sc.chunk - 1) / sc.chunk, segs = (q.count + kTreeSegment - 1) / kTreeSegment;
-  if (!rows || key0 >= q.keys) return;
-  const uint32_t count = min(sc.chunk, (q.keys - key0 + 31) / 32 * 32), steps = count / 32;
-  for (uint32_t i = tid; i < count; i += kTreeThreads)
-    row_s[i] = key0 + i < q.keys ? page_row(a.table + (size_t)r * a.width, a.width, a.page_size, a.pages, key0 + i) : -1;
+  const uint32_t rows = q.nodes * q.group, s0 = chunk * sc.vchunk, key0 = q.base + s0;
+  const uint32_t chunks = (q.count + sc.vchunk - 1) / sc.vchunk, segs = (q.count + kTreeSegment - 1) / kTreeSegment;
+  if (f0 >= rows || key0 >= q.keys) return;
+  const uint32_t count = min(sc.vchunk, (q.keys - key0 + 31) / 32 * 32);
+  const int32_t* table = a.table + (size_t)r * a.width;
+  for (uint32_t i = tid; i < (count + kValueKeys - 1) / kValueKeys * kValueKeys; i += kValueThreads) {
+    const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
+    row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
+  }
+  if (tid == 0) s.wide = 0;
   pdl_wait();
-  for (uint32_t f0 = 0; f0 < rows; f0 += kTreeTile) {
-    __syncthreads();
-    for (uint32_t i = warp; i < kTreeTile; i += kTreeWarps) {
-      const uint32_t f = f0 + i;
-      uint64_t sum = 0;
-      uint32_t first = UINT32_MAX;
-      if (f < rows) {
-        const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-        for (uint32_t s = lane; s < segs; s += 32) {
-          sum += sc.seg_sum[id * sc.segs + s];
-          first = min(first, sc.seg_first[id * sc.segs + s]);
-        }
-        sum = (uint64_t)warp_sum_i64((int64_t)sum);
-        first = __reduce_min_sync(0xffffffffu, first);
+  for (uint32_t i = warp; i < tile; i += kValueWarps) {
+    const uint32_t f = f0 + i;
+    uint64_t sum = 0;
+    uint32_t first = UINT32_MAX, id = UINT32_MAX;
+    if (f < rows) {
+      id = (q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
+      for (uint32_t x = lane; x < segs; x += 32) {
+        sum += sc.seg_sum[(size_t)id * sc.segs + x];
+        first = min(first, sc.seg_first[(size_t)id * sc.segs + x]);
       }
-      if (lane == 0) {
-        sum_s[i] = sum;
-        recip_s[i] = sum_recip(sum);
-        first_s[i] = first;
-      }
+      sum = (uint64_t)warp_sum_i64((int64_t)sum);
+      first = __reduce_min_sync(0xffffffffu, first);
     }
-    __syncthreads();
-    // weights of the chunk: a warp takes eight rows and 32 keys at a time
-    for (uint32_t u = warp; u < NT * steps; u += kTreeWarps) {
-      const uint32_t n = u % NT, st = u / NT, i = 8 * n + (lane >> 2), f = f0 + i;
-      int32_t x[8];
-      int32_t total = 0;
-      if (f < rows) {
-        const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-        const int32_t* s = sc.scores + id * sc.pitch + s0 + st * 32 + 4 * (lane & 3);
-        const uint4 lo = *(const uint4*)s, hi = *(const uint4*)(s + 16);
-        const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-        const uint32_t at = s0 + st * 32 + 4 * (lane & 3);
-        weights_of(e, recip_s[i], sum_s[i], x);
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-          if (at + (j >> 2) * 16 + (j & 3) == first_s[i]) x[j] = 0;  // its weight comes last
-          total += x[j];
-        }
-        total += __shfl_xor_sync(0xfu << (lane & 28), total, 1);
-        total += __shfl_xor_sync(0xfu << (lane & 28), total, 2);
-        if ((lane & 3) == 0 && total) atomicAdd(sc.wsum + id, total);
-      } else {
-#pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) x[j] = 0;
-      }
-      put_weight_fragment(w + (size_t)(st * NT + n) * 64, lane, x);
-    }
-    __syncthreads();
-    // value sums: the warps take the head's 16-dimension tiles, and where
-    // those are fewer than the warps, alternate steps of the keys
-    const uint32_t tiles = a.head_dim / 16, split = max(1u, kTreeWarps / tiles);
-    for (uint32_t u = warp; u < tiles * split; u += kTreeWarps) {
-      const uint32_t dt = u % tiles, part = u / tiles;
-      if (tree_value_tile<3>(a, sc, q, w, row_s, steps, g, f0, dt, part, split, lane))
-        tree_value_tile<4>(a, sc, q, w, row_s, steps, g, f0, dt, part, split, lane);
+    if (lane == 0) {
+      s.sum[i] = sum;
+      s.recip[i] = sum_recip(sum);
+      s.first[i] = first;
+      s.id[i] = id;
     }
   }
-  // the last block of this request and head writes the outputs
+  __syncthreads();
+  if (tree_chunk_values<3, NT>(a, sc, s, frag, wts, row_s, s0, count, g)) {
+    __syncthreads();
+    tree_chunk_values<4, NT>(a, sc, s, frag, wts, row_s, s0, count, g);
+  }
+  // the last block of these rows writes the outputs
   __syncthreads();
   if (tid == 0) {
     __threadfence();
-    last_s = atom_add_acq_rel(sc.done + r * a.kv_heads + g, 1u) + 1 == chunks;
+    s.last = atom_add_acq_rel(sc.done + (size_t)r * gridDim.y + blockIdx.y, 1u) + 1 == chunks;
     __threadfence();
   }
   __syncthreads();
-  if (!last_s) return;
+  if (!s.last) return;
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
-  for (uint32_t f = warp; f < rows; f += kTreeWarps) {
-    const uint32_t node = f / q.group, head = g * q.group + f % q.group;
-    const size_t id = (size_t)(q.begin + node) * a.heads + head;
-    uint32_t first = UINT32_MAX;
-    for (uint32_t s = lane; s < segs; s += 32) first = min(first, sc.seg_first[id * sc.segs + s]);
-    first = __reduce_min_sync(0xffffffffu, first);
-    const int64_t row =
-        first < q.count ? page_row(a.table + (size_t)r * a.width, a.width, a.page_size, a.pages, q.base + first) : -1;
+  for (uint32_t i = warp; i < min(tile, rows - f0); i += kValueWarps) {
+    const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group;
+    const size_t id = s.id[i];
+    const uint32_t first = s.first[i];
+    const int64_t row = first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
     const int32_t top = sub_sat(kOneAct, __ldcg(sc.wsum + id));
     int32_t* out = a.out + (size_t)(q.begin + node) * a.out_stride + head * a.head_dim;
     for (uint32_t x = lane; x < a.head_dim; x += 32) {
@@ -345,19 +414,29 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_values_kernel(IrisTreeAt
 uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
-// Keys a block takes: as many as leave the blocks enough for two a
-// multiprocessor (fewer blocks reload fewer query fragments), at least 64.
-uint32_t chunk_keys(const IrisTreeAttention& a) {
-  const uint32_t groups = a.requests * a.kv_heads, want = 2 * 148;
-  uint32_t chunk = 512;
-  while (chunk > 64 && (uint64_t)groups * ceil_div(a.longest, chunk) < want) chunk /= 2;
+// Keys a block takes: as many as leave two blocks a multiprocessor (fewer
+// blocks remake fewer query fragments), from 64 on.
+uint32_t keys_a_block(uint64_t groups, uint32_t longest, uint32_t most, uint32_t want) {
+  uint32_t chunk = most;
+  while (chunk > 64 && groups * ceil_div(longest, chunk) < want) chunk /= 2;
   return chunk;
 }
 
+// Row tiles a warp of the third launch takes (8 rows each): as few as hold the
+// call's largest tree, so that a few rows do not pay for 64.
+uint32_t value_tiles(const IrisTreeAttention& a) {
+  const uint32_t rows = a.nodes * (a.heads / a.kv_heads), halves = a.head_dim <= 128 ? 2 : 1;
+  return rows <= 8 * halves ? 1 : rows <= 16 * halves ? 2 : 4;
+}
+uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a.head_dim <= 128 ? 2 : 1); }
+
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   const size_t rows = (size_t)a.rows * a.heads;
-  sc->chunk = chunk_keys(a);
+  sc->chunk = keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 2 * 148);
   sc->chunks = ceil_div(a.longest, sc->chunk);
+  sc->groups = ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
+  sc->vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->groups, a.longest, 4096, 2 * 148);
+  sc->vchunks = ceil_div(a.longest, sc->vchunk);
   sc->segs = ceil_div(a.longest, kTreeSegment);
   sc->pitch = ceil_div(a.longest, 64) * 64;
   size_t at = 0;
@@ -372,18 +451,30 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   sc->seg_first = (uint32_t*)take(rows * sc->segs * 4);
   sc->acc = (int64_t*)take(rows * a.head_dim * 8);
   sc->wsum = (int32_t*)take(rows * 4);
-  sc->done = (uint32_t*)take((size_t)a.requests * a.kv_heads * 4);
+  sc->done = (uint32_t*)take((size_t)a.requests * a.kv_heads * sc->groups * 4);
   return at;
 }
 
 constexpr uint32_t score_smem(uint32_t d) { return kTreeTile / 8 * (d / 32) * 4 * 256; }
-constexpr uint32_t value_smem(uint32_t chunk) { return chunk / 32 * (kTreeTile / 8) * 512 + chunk * 8; }
+constexpr uint32_t value_smem(uint32_t d, uint32_t vchunk, uint32_t rows) {
+  return vchunk * 4 + 4 * (d / 16) * 4 * 512 + 4 * (rows / 8) * 512;
+}
+
+template <uint32_t NT>
+cudaError_t launch_values(const IrisTreeAttention& a, const TreeScratch& sc, dim3 grid, uint32_t smem,
+                          cudaStream_t stream) {
+  const cudaError_t e =
+      cudaFuncSetAttribute(tree_values_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  return launch_k(tree_values_kernel<NT>, grid, dim3(kValueThreads), smem, stream, a, sc);
+}
 
 }  // namespace
 
 bool tree_mma_usable(const IrisTreeAttention& a) {
   return a.head_dim % 32 == 0 && a.scale_q32 < 0x80000000u && a.requests <= 65535 && a.kv_heads <= 65535 &&
-         a.longest > 0;
+         a.longest > 0 && a.pages > 0 && a.pages * a.page_size < 0xFFFFFFFFull &&
+         (uint64_t)a.rows * a.heads < 0xFFFFFFFFull && (uint64_t)a.heads * kTreeNodes <= 65535;
 }
 
 uint64_t tree_mma_workspace(const IrisTreeAttention& a) {
@@ -400,8 +491,13 @@ cudaError_t launch_tree_mma(const IrisTreeAttention& a, uint8_t* workspace, cuda
   e = launch_k(tree_terms_kernel, dim3(ceil_div(a.nodes * a.heads, kTreeWarps), sc.segs, a.requests),
                dim3(kTreeThreads), 0, stream, a, sc);
   if (e != cudaSuccess) return e;
-  return launch_k(tree_values_kernel, dim3(sc.chunks, a.kv_heads, a.requests), dim3(kTreeThreads),
-                  value_smem(sc.chunk), stream, a, sc);
+  const uint32_t smem = value_smem(a.head_dim, sc.vchunk, value_rows(a));
+  const dim3 grid(sc.vchunks, a.kv_heads * sc.groups, a.requests);
+  switch (value_tiles(a)) {
+    case 1: return launch_values<1>(a, sc, grid, smem, stream);
+    case 2: return launch_values<2>(a, sc, grid, smem, stream);
+    default: return launch_values<4>(a, sc, grid, smem, stream);
+  }
 }
 
 }  // namespace iris
