@@ -3,6 +3,8 @@
 // drafted tokens. Pages hold page_size token rows each; request r's token at
 // position p lies in row (table[r][p / page_size] * page_size + p % page_size)
 // of the pools.
+#include <algorithm>
+
 #include "../../include/iris_b200.h"
 #include "common.cuh"
 #include "serve.cuh"
@@ -16,48 +18,55 @@ namespace {
 // offsets[r] = sum of fresh[0..r), and the new pages of request r are the
 // entries [base[r], base[r + 1]) of the free list, base the prefix sums of
 // ceil((held + fresh) / page) - ceil(held / page). Every block computes both
-// prefix sums over all requests itself (the lengths are a few KB in L2), so
-// one launch needs no exchange between blocks; then it writes its share of
-// the requests' offsets and table entries and of the tokens' slots.
-constexpr uint32_t kPlanThreads = 256;
-constexpr uint32_t kPlanTokens = 1024;        // tokens a block
+// prefix sums over all requests itself (the lengths are a few KB in L2; one
+// coalesced round of loads and a scan in shared memory), so one launch needs no
+// exchange between blocks; then it writes its share of the requests' offsets
+// and table entries and of the tokens' slots. A warp finds its 32 tokens'
+// request by one search, which a lane repeats only where its token is past it.
+// Bound by latency: 4,001 requests and a million tokens move 12 MB.
+constexpr uint32_t kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanMaxRequests = 16384;  // two prefix sums of 4 bytes a request in shared memory
 
 struct PlanArgs {
   const int32_t *held, *fresh, *free_pages, *parents;
   uint32_t requests, page, width, n_free, tokens;
+  int32_t shift;  // log2 of the page size, -1 where it is no power of two
+  uint32_t share; // tokens a block (a multiple of its threads)
   int32_t *table, *offsets, *positions, *counts;
   int64_t *slots, *masks;
 };
 
-__device__ __forceinline__ uint32_t pages_of(uint32_t n, uint32_t page) { return (n + page - 1) / page; }
+__device__ __forceinline__ uint32_t page_of(uint32_t at, const PlanArgs& a) {
+  return a.shift >= 0 ? at >> a.shift : at / a.page;
+}
+__device__ __forceinline__ uint32_t pages_of(uint32_t n, const PlanArgs& a) { return page_of(n + a.page - 1, a); }
 
 __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
   extern __shared__ uint32_t plan_sm[];
   uint32_t* off = plan_sm;                    // [requests + 1]
   uint32_t* base = plan_sm + a.requests + 1;  // [requests + 1]
-  __shared__ unsigned long long part[kPlanThreads / 32];
-  __shared__ uint32_t faults;
+  __shared__ unsigned long long part[kPlanWarps];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) faults = 0;
-  __syncthreads();
-  // a thread's run of consecutive requests; tokens and pages summed together (each below 2^31)
-  const uint32_t per = (a.requests + kPlanThreads - 1) / kPlanThreads;
-  const uint32_t r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
-  uint64_t tok = 0, pg = 0;
   uint32_t bad = 0;
-  for (uint32_t r = r0; r < r1; ++r) {
+  // a request's tokens and new pages
+#pragma unroll 4
+  for (uint32_t r = tid; r < a.requests; r += kPlanThreads) {
     const int32_t h = a.held[r], f = a.fresh[r];
     const uint32_t hu = (uint32_t)max(h, 0), fu = (uint32_t)max(f, 0);
     if (h < 0 || f < 0 || hu + fu > (uint32_t)INT32_MAX) bad |= IRIS_PLAN_LENGTH;
-    const uint32_t after = pages_of(hu + fu, a.page), taken = after - pages_of(hu, a.page);
+    const uint32_t after = pages_of(hu + fu, a);
     if (after > a.width) bad |= IRIS_PLAN_WIDTH;
-    tok += fu;
-    pg += taken;
+    off[r] = fu;
+    base[r] = after - pages_of(hu, a);
   }
-  if (tok > (uint64_t)INT32_MAX) bad |= IRIS_PLAN_LENGTH;
-  unsigned long long sum = ((unsigned long long)(uint32_t)tok << 32) | (uint32_t)pg;
-  // exclusive prefix of the threads' sums; a sum of tokens past 2^31 is flagged and wraps harmlessly
+  __syncthreads();
+  // prefix sums: a thread's run of consecutive requests, both sums in one word
+  const uint32_t per = (a.requests + kPlanThreads - 1) / kPlanThreads;
+  const uint32_t r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
+  uint64_t tok = 0, pg = 0;
+  for (uint32_t r = r0; r < r1; ++r) tok += off[r], pg += base[r];
+  if (tok > (uint64_t)INT32_MAX) bad |= IRIS_PLAN_LENGTH;  // (then the offsets wrap; they stay below the tokens)
+  const unsigned long long sum = ((unsigned long long)(uint32_t)tok << 32) | (uint32_t)pg;
   unsigned long long incl = sum;
 #pragma unroll
   for (uint32_t d = 1; d < 32; d <<= 1) {
@@ -65,19 +74,19 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     if (lane >= d) incl += o;
   }
   if (lane == 31) part[warp] = incl;
-  if (bad) atomicOr(&faults, bad);
-  __syncthreads();
+  const uint32_t faults = (__syncthreads_or(bad & IRIS_PLAN_LENGTH) ? IRIS_PLAN_LENGTH : 0) |
+                          (__syncthreads_or(bad & IRIS_PLAN_WIDTH) ? IRIS_PLAN_WIDTH : 0);
   unsigned long long before = incl - sum;
   for (uint32_t w = 0; w < warp; ++w) before += part[w];
   uint32_t t0 = (uint32_t)(before >> 32), p0 = (uint32_t)before;
   for (uint32_t r = r0; r < r1; ++r) {
-    const uint32_t hu = (uint32_t)max(a.held[r], 0), fu = (uint32_t)max(a.fresh[r], 0);
+    const uint32_t f = off[r], n = base[r];
     off[r] = t0;
     base[r] = p0;
-    t0 += fu;
-    p0 += pages_of(hu + fu, a.page) - pages_of(hu, a.page);
+    t0 += f;
+    p0 += n;
   }
-  if (r1 == a.requests && r0 < r1) {
+  if (r1 == a.requests && (r0 < r1 || (a.requests == 0 && tid == 0))) {
     off[a.requests] = t0;
     base[a.requests] = p0;
   }
@@ -90,53 +99,57 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     a.counts[2] = (int32_t)(total > a.tokens ? total - a.tokens : 0);
     a.counts[3] = (int32_t)(faults | (pages > a.n_free ? IRIS_PLAN_POOL : 0) | (total > a.tokens ? IRIS_PLAN_TOKENS : 0));
   }
-  // the requests' offsets and new table entries, a warp a request
-  const uint32_t nwarps = gridDim.x * (kPlanThreads / 32);
-  for (uint32_t r = blockIdx.x * (kPlanThreads / 32) + warp; r <= a.requests; r += nwarps) {
-    if (lane == 0) a.offsets[r] = (int32_t)off[r];
-    if (r == a.requests) break;
-    const uint32_t first = pages_of((uint32_t)max(a.held[r], 0), a.page), n = base[r + 1] - base[r];
+  // the requests' offsets and new table entries: a block takes consecutive
+  // requests, a thread a request's offset, a warp a request's entries
+  const uint32_t span = (a.requests + gridDim.x) / gridDim.x;  // of requests + 1 offsets
+  const uint32_t q0 = min(a.requests + 1, blockIdx.x * span), q1 = min(a.requests + 1, q0 + span);
+  for (uint32_t r = q0 + tid; r < q1; r += kPlanThreads) a.offsets[r] = (int32_t)off[r];
+  for (uint32_t r = q0 + warp; r < min(q1, a.requests); r += kPlanWarps) {
+    const uint32_t n = base[r + 1] - base[r];
+    if (!n) continue;
+    const uint32_t first = pages_of((uint32_t)max(a.held[r], 0), a);
     for (uint32_t j = lane; j < n && first + j < a.width; j += 32)
       a.table[(size_t)r * a.width + first + j] = base[r] + j < a.n_free ? a.free_pages[base[r] + j] : -1;
   }
   // the tokens' slots and positions
-  const uint32_t end = min(a.tokens, (blockIdx.x + 1) * kPlanTokens);
-  for (uint32_t i = blockIdx.x * kPlanTokens + tid; i < end; i += kPlanThreads) {
+  const uint32_t begin = blockIdx.x * a.share, end = min(a.tokens, begin + a.share);
+  for (uint32_t i = begin + tid; i - lane < end; i += kPlanThreads) {
+    uint32_t r = request_of(off, a.requests, min(i - lane, total ? total - 1 : 0));
+    if (i >= end) break;
     int64_t slot = -1, mask = 0;
     uint32_t position = 0;
     if (i < total) {
-      const uint32_t r = request_of(off, a.requests, i), local = i - off[r];
-      const uint32_t hu = (uint32_t)max(a.held[r], 0), at = hu + local, column = at / a.page;
-      const uint32_t first = pages_of(hu, a.page);
+      if (off[r + 1] <= i) r = r + 1 + request_of(off + r + 1, a.requests - r - 1, i);
+      const uint32_t local = i - off[r];
+      const uint32_t hu = (uint32_t)max(a.held[r], 0), at = hu + local, column = page_of(at, a);
+      const uint32_t first = pages_of(hu, a);
       int32_t pageid = -1;
       if (column < first) {
         if (column < a.width) pageid = a.table[(size_t)r * a.width + column];
       } else if (column < a.width && base[r] + (column - first) < a.n_free) {
         pageid = a.free_pages[base[r] + (column - first)];
       }
-      if (pageid >= 0) slot = (int64_t)pageid * a.page + at % a.page;
+      if (pageid >= 0) slot = (int64_t)pageid * a.page + (at - column * a.page);
       position = at;
-      if (a.masks) {
+      if (a.masks && local < kTreeNodes) {
         // the node and its ancestors; a parent that is not an earlier node
         // (or a node past 64) leaves the mask empty
-        if (local < kTreeNodes) {
-          uint32_t node = local;
-          unsigned long long m = 0;
-          bool good = true;
-          for (;;) {
-            m |= 1ull << node;
-            const int32_t up = a.parents[off[r] + node];
-            if (up == -1) break;
-            if (up < 0 || (uint32_t)up >= node) {
-              good = false;
-              break;
-            }
-            node = (uint32_t)up;
+        uint32_t node = local;
+        unsigned long long m = 0;
+        bool good = true;
+        for (;;) {
+          m |= 1ull << node;
+          const int32_t up = a.parents[off[r] + node];
+          if (up == -1) break;
+          if (up < 0 || (uint32_t)up >= node) {
+            good = false;
+            break;
           }
-          if (good) {
-            mask = (int64_t)m;
-            position = hu + (uint32_t)__popcll(m) - 1;
-          }
+          node = (uint32_t)up;
+        }
+        if (good) {
+          mask = (int64_t)m;
+          position = hu + (uint32_t)__popcll(m) - 1;
         }
       }
     }
@@ -307,15 +320,17 @@ int iris_page_plan(const int32_t* d_held, const int32_t* d_fresh, uint32_t reque
       tokens > (uint32_t)INT32_MAX || (requests && (!d_held || !d_fresh || (width && !d_table))) ||
       (n_free && !d_free) || (tokens && (!d_slots || !d_positions)) || (tokens && !d_parents != !d_masks))
     return IRIS_EINVAL;
-  PlanArgs a{d_held, d_fresh, d_free, d_parents, requests, page_size, width, n_free, tokens,
+  // two blocks a multiprocessor at most: each repeats the prefix sums
+  const uint32_t rounds = (tokens + 2 * 148 * kPlanThreads - 1) / (2 * 148 * kPlanThreads);
+  const uint32_t share = std::max(1u, rounds) * kPlanThreads;
+  const int32_t shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
+  PlanArgs a{d_held, d_fresh, d_free, d_parents, requests, page_size, width, n_free, tokens, shift, share,
              d_table, d_offsets, d_positions, d_counts, d_slots, d_masks};
   const size_t smem = (size_t)(requests + 1) * 8;
-  if (smem > 40 * 1024) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(page_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kPlanMaxRequests + 1) * 8);
-    if (e != cudaSuccess) return (int)e;
-  }
-  const uint32_t blocks = tokens ? (tokens + kPlanTokens - 1) / kPlanTokens : 1;
+  static std::atomic<bool> allowed[64];
+  const cudaError_t e = allow_smem(page_plan_kernel, allowed);
+  if (e != cudaSuccess) return (int)e;
+  const uint32_t blocks = tokens ? (tokens + share - 1) / share : 1;
   page_plan_kernel<<<blocks, kPlanThreads, smem, (cudaStream_t)stream>>>(a);
   return (int)cudaGetLastError();
 }

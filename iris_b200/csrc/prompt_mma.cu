@@ -421,7 +421,8 @@ cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, const 
                    cudaStream_t stream) {
   const uint32_t smem = RT / 8 * (a.head_dim / 32) * 1024 + 2 * kPromptKeys / 32 * (RT / 8) * 512 +
                         kPromptWarps * kTermList * 4;
-  cudaError_t e = cudaFuncSetAttribute(prompt_mma_kernel<RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<bool> allowed[64];
+  cudaError_t e = allow_smem(prompt_mma_kernel<RT>, allowed);
   if (e != cudaSuccess) return e;
   prompt_items_kernel<<<1, 1024, 0, stream>>>(a, sc, RT);
   e = cudaGetLastError();

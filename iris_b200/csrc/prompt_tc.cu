@@ -652,7 +652,8 @@ cudaError_t launch_prompt_tc(const IrisPromptAttention& a, const PromptTcScratch
       !make_map(&kmap, sc.kp, kPtD, a.tokens, (uint64_t)a.kv_heads * 3, kPtD, (uint64_t)a.tokens * kPtD, kPtKeys, 1) ||
       !make_map(&vmap, sc.vt, sc.tpitch, kPtD, (uint64_t)a.kv_heads * 3, sc.tpitch, (uint64_t)kPtD * sc.tpitch, kPtD, 1))
     return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(prompt_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPtSmem);
+  static std::atomic<bool> allowed[64];
+  cudaError_t e = allow_smem(prompt_tc_kernel, allowed);
   if (e != cudaSuccess) return e;
   e = launch_k(prompt_pack_kernel, dim3(sc.pack_blocks, 4), dim3(kPackThreads), 0, stream, a, sc);
   if (e != cudaSuccess) return e;

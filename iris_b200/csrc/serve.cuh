@@ -4,9 +4,30 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "detnum.cuh"
 
 namespace iris {
+
+// Raises a kernel's dynamic shared memory limit to what a block may have, once
+// per device and not on every launch.
+template <class K>
+inline cudaError_t allow_smem(K* kernel, std::atomic<bool> (&set)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (set[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  int most = 0;
+  cudaFuncAttributes attr;
+  e = cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, kernel);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)attr.sharedSizeBytes);
+  if (e == cudaSuccess) set[dev].store(true, std::memory_order_release);
+  return e;
+}
 
 constexpr uint32_t kTreeNodes = 64;  // drafted nodes a request: a node's visible nodes are one 64-bit word
 

@@ -463,8 +463,8 @@ constexpr uint32_t value_smem(uint32_t d, uint32_t vchunk, uint32_t rows) {
 template <uint32_t NT>
 cudaError_t launch_values(const IrisTreeAttention& a, const TreeScratch& sc, dim3 grid, uint32_t smem,
                           cudaStream_t stream) {
-  const cudaError_t e =
-      cudaFuncSetAttribute(tree_values_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  static std::atomic<bool> allowed[64];
+  const cudaError_t e = allow_smem(tree_values_kernel<NT>, allowed);
   if (e != cudaSuccess) return e;
   return launch_k(tree_values_kernel<NT>, grid, dim3(kValueThreads), smem, stream, a, sc);
 }

@@ -54,18 +54,23 @@ class Accepted(NamedTuple):
     held: torch.Tensor      # [requests] cached tokens now
 
 
-def _need(x: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
-    """The address of a tensor whose last axis is dense; its other axes may have strides."""
-    if x.dtype != dtype or x.dim() != dim or not x.is_cuda or (x.numel() and x.stride(-1) != 1):
-        raise ValueError(f"{name}: a CUDA tensor of {dtype} with {dim} axes, the last one dense, is needed; "
-                         f"got {x.dtype} {tuple(x.shape)} on {x.device} with strides {x.stride()}")
+def _refuse(x: torch.Tensor, name: str, dtype: torch.dtype, dim: int, what: str) -> None:
+    raise ValueError(f"{name}: a CUDA tensor of {dtype} with {dim} axes, {what}, is needed; "
+                     f"got {x.dtype} {tuple(x.shape)} on {x.device} with strides {x.stride()}")
+
+
+def _rows(x: torch.Tensor, name: str) -> int:
+    """The address of int32 rows whose last axis is dense (rows may lie apart)."""
+    if x.dtype != torch.int32 or not x.is_cuda or x.dim() != 2 or (x.stride(1) != 1 and x.numel()):
+        _refuse(x, name, torch.int32, 2, "the last one dense")
     return x.data_ptr()
 
 
 def _dense(x: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
-    if not x.is_contiguous():
-        raise ValueError(f"{name}: a contiguous tensor is needed; got strides {x.stride()}")
-    return _need(x, name, dtype, dim)
+    """The address of a contiguous tensor."""
+    if x.dtype != dtype or not x.is_cuda or x.dim() != dim or not x.is_contiguous():
+        _refuse(x, name, dtype, dim, "contiguous")
+    return x.data_ptr()
 
 
 def _same(count: int, want: int, name: str) -> None:
@@ -74,9 +79,11 @@ def _same(count: int, want: int, name: str) -> None:
 
 
 def _stream(x: torch.Tensor) -> int:
-    if x.device.index != torch.cuda.current_device():
+    """torch's current stream on the tensor's device, which has to be the current one."""
+    index = x.get_device()
+    if index != torch._C._cuda_getDevice():
         raise ValueError(f"tensors are on {x.device}, but cuda:{torch.cuda.current_device()} is the current device")
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free_pages: torch.Tensor, page_size: int,
@@ -87,26 +94,23 @@ def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free
     least the fresh tokens). With `parents` (each drafted node's parent in its
     request, -1 for a root) the plan has the nodes' visibility masks and their
     positions count ancestors only."""
-    requests = held.numel()
+    requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
     ph, pf = _dense(held, "held"), _dense(fresh, "fresh")
     pt, pp = _dense(table, "table", dim=2), _dense(free_pages, "free_pages")
     _same(fresh.numel(), requests, "fresh")
     _same(table.shape[0], requests, "table")
-    dev = held.device
-    offsets = torch.empty(requests + 1, dtype=torch.int32, device=dev)
-    slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-    positions = torch.empty(tokens, dtype=torch.int32, device=dev)
-    counts = torch.empty(4, dtype=torch.int32, device=dev)
-    masks, pm, pa = None, None, None
+    counts, offsets, positions = held.new_empty(4), held.new_empty(requests + 1), held.new_empty(tokens)
+    slots = torch.empty(tokens, dtype=torch.int64, device=held.device)
+    masks, pa, pm = None, None, None
     if parents is not None:
         if parents.numel() < tokens:
             raise ValueError(f"parents: {parents.numel()} entries, expected {tokens}")
         pa = _dense(parents, "parents")
-        masks = torch.empty(tokens, dtype=torch.int64, device=dev)
+        masks = slots.new_empty(tokens)
         pm = masks.data_ptr()
-    check(lib().iris_page_plan(ph, pf, requests, page_size, pt, table.shape[1], pp, free_pages.numel(), pa, tokens,
-                               offsets.data_ptr(), slots.data_ptr(), positions.data_ptr(), pm, counts.data_ptr(),
-                               _stream(held)), "iris_page_plan")
+    check(lib().iris_page_plan(ph, pf, requests, page_size, pt, width, pp, n_free, pa, tokens, offsets.data_ptr(),
+                               slots.data_ptr(), positions.data_ptr(), pm, counts.data_ptr(), _stream(held)),
+          "iris_page_plan")
     return PagePlan(offsets, slots, positions, table, counts, masks)
 
 
@@ -115,7 +119,7 @@ def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     """K and V rows [tokens][kv_dim] into the pools [pages][page_size][kv_dim]
     at their slots; a slot outside the pools (-1) skips its row."""
     tokens, kv_dim = k.shape
-    pk, pv, ps = _need(k, "k", dim=2), _need(v, "v", dim=2), _dense(slots, "slots", torch.int64)
+    pk, pv, ps = _rows(k, "k"), _rows(v, "v"), _dense(slots, "slots", torch.int64)
     ck, cv = _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
     if v.shape != k.shape or k_pages.shape != v_pages.shape or k_pages.shape[2] != kv_dim:
         raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
@@ -137,17 +141,17 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     request r's rows are offsets[r] .. offsets[r + 1] - 1, the longest request
     at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense)."""
     tokens = q.shape[0]
-    pq, pk, pv, po = _need(q, "q", dim=2), _need(k, "k", dim=2), _need(v, "v", dim=2), _dense(offsets, "offsets")
+    pq, pk, pv, po = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _dense(offsets, "offsets")
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
     dim = q.shape[1] // heads
     if k.shape != (tokens, kv_heads * dim) or v.shape != k.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} are not {tokens} rows of {kv_heads} heads of {dim}")
     if out is None:
-        out = torch.empty((tokens, heads * dim), dtype=torch.int32, device=q.device)
+        out = q.new_empty((tokens, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.PromptAttention(pq, pk, pv, po, _need(out, "out", dim=2), q.stride(0), k.stride(0), v.stride(0),
+    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out"), q.stride(0), k.stride(0), v.stride(0),
                              out.stride(0), offsets.numel() - 1, tokens, longest, heads, kv_heads, dim, window,
                              scale_q32)
     L, ref = lib(), C.byref(a)
@@ -167,7 +171,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     cached tokens and the nodes of its mask. `longest`: the most cached tokens
     and nodes a request has together. A node that sees nothing gives zeros."""
     rows, requests = q.shape[0], held.numel()
-    pq, ck, cv = _need(q, "q", dim=2), _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
+    pq, ck, cv = _rows(q, "q"), _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
     pt, ph, po = _dense(table, "table", dim=2), _dense(held, "held"), _dense(offsets, "offsets")
     pm = _dense(masks, "masks", torch.int64)
     pp = _dense(positions, "positions") if positions is not None else None
@@ -182,10 +186,10 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         if x is not None and x.numel() < rows:
             raise ValueError(f"{name}: {x.numel()} entries, expected {rows}")
     if out is None:
-        out = torch.empty((rows, heads * dim), dtype=torch.int32, device=q.device)
+        out = q.new_empty((rows, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _need(out, "out", dim=2), q.stride(0), out.stride(0),
+    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out"), q.stride(0), out.stride(0),
                            k_pages.shape[0], requests, rows, table.shape[1], k_pages.shape[1], nodes, longest, heads,
                            kv_heads, dim, window, scale_q32)
     L, ref = lib(), C.byref(a)
@@ -205,12 +209,12 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     rows, requests = tokens.numel(), held.numel()
     pt, pa, pk = _dense(tokens, "tokens"), _dense(parents, "parents"), _dense(picks, "picks")
     po, ph, tb = _dense(offsets, "offsets"), _dense(held, "held"), _dense(table, "table", dim=2)
-    for x, n, name in ((parents, rows, "parents"), (picks, rows, "picks"), (offsets, requests + 1, "offsets"),
-                       (table[:, :1], requests if table.shape[1] else 0, "table")):
-        _same(x.numel(), n, name)
-    dev = held.device
-    path = torch.empty((requests, path_width), dtype=torch.int32, device=dev)
-    out = torch.empty((3, requests), dtype=torch.int32, device=dev)
+    _same(parents.numel(), rows, "parents")
+    _same(picks.numel(), rows, "picks")
+    _same(offsets.numel(), requests + 1, "offsets")
+    _same(table.shape[0], requests, "table")
+    accepted, after, now = held.new_empty(requests), held.new_empty(requests), held.new_empty(requests)
+    path = held.new_empty((requests, path_width))
     layers, stride, pages, page, kv_dim, ck, cv = 0, 0, 0, 0, 0, None, None
     if k_pages is not None or v_pages is not None:
         if k_pages is None or v_pages is None or k_pages.shape != v_pages.shape:
@@ -218,8 +222,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
         ck, cv = _dense(k_pages, "k_pages", dim=4), _dense(v_pages, "v_pages", dim=4)
         layers, pages, page, kv_dim = k_pages.shape
         stride = pages * page * kv_dim
-    base = out.data_ptr()
-    check(lib().iris_tree_accept(pt, pa, pk, po, requests, rows, ph, path_width, path.data_ptr(), base,
-                                 base + 4 * requests, base + 8 * requests, tb, table.shape[1], page, ck, cv, layers,
-                                 stride, pages, kv_dim, _stream(held)), "iris_tree_accept")
-    return Accepted(path, out[0], out[1], out[2])
+    check(lib().iris_tree_accept(pt, pa, pk, po, requests, rows, ph, path_width, path.data_ptr(), accepted.data_ptr(),
+                                 after.data_ptr(), now.data_ptr(), tb, table.shape[1], page, ck, cv, layers, stride,
+                                 pages, kv_dim, _stream(held)), "iris_tree_accept")
+    return Accepted(path, accepted, after, now)
