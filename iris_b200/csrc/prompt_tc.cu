@@ -32,6 +32,7 @@
 #include "q8.cuh"
 #include "serve_attn.cuh"
 #include "serve_mma.cuh"
+#include "serve_tc.cuh"
 #include "tc.cuh"
 #include "tcgen05.cuh"
 
@@ -59,16 +60,6 @@ static_assert(3 * kPtQPlane <= kPtOperands, "query planes");
 static_assert(8 * kPtRows == 512, "TMEM column groups");
 
 // ---- packing -------------------------------------------------------------------
-
-// Four values as signed base-256 digits, x = c0 + 2^8 c1 + 2^16 c2 with every
-// digit in [-128, 127]: the bytes of x + 0x808080, each less 128. p[3] is not 0
-// where a value is outside [-0x808080, 0x7F7F7F]. With all digits signed, one
-// product takes a plane against several others side by side.
-__device__ __forceinline__ void split_digits(int32_t x, int32_t y, int32_t z, int32_t w, uint32_t (&p)[4]) {
-  split_planes(x + 0x808080, y + 0x808080, z + 0x808080, w + 0x808080, p);
-#pragma unroll
-  for (uint32_t i = 0; i < 3; ++i) p[i] ^= 0x80808080u;
-}
 
 // Rows of 128 values (row r, part g at src + (r / per) * stride + (g * per + r %
 // per) * 128) into planes dst[g][3][rows][128]; flags what is past 24 bits.
@@ -147,37 +138,6 @@ struct PtShared {
   uint32_t recip[kPtRows], first[kPtRows];
   uint32_t item, tmem, dead, wide;
 };
-
-// mbar_wait_bounded that gives up at once after any wait of the block has.
-__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, PtShared& s, unsigned int* fault) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_ns();
-  for (;;) {
-    if (mbar_try_wait_suspend(bar, parity)) return true;
-    if (*(volatile uint32_t*)&s.dead) return false;
-    if (global_ns() - t0 > 1000000000ull) {
-      *(volatile uint32_t*)&s.dead = 1;
-      atomicOr(fault, 1u);
-      return false;
-    }
-  }
-}
-
-// tc_mma and tc_commit issued by the lane with `leader`, without a branch.
-__device__ __forceinline__ void pt_mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, bool acc, bool leader) {
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(ad), "l"(bd), "r"(idesc), "r"((uint32_t)acc), "r"((uint32_t)leader)
-      : "memory");
-}
-__device__ __forceinline__ void pt_commit(uint64_t* bar, bool leader) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_addr(bar)),
-      "r"((uint32_t)leader)
-      : "memory");
-}
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
 
@@ -275,7 +235,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           tma_load_3d(ops + j * kPtQPlane, &qmap, 0, (int32_t)(begin * group + f0), (int32_t)(g * 3 + j), &s.q_full);
         for (uint32_t u = 0; u < 6 * ktiles && ok; ++u, ++ring_n) {
           const uint32_t slot = ring_n % kPtSlots, use = ring_n / kPtSlots;
-          if (use > 0 && !pt_wait(&s.empty[slot], (use - 1) & 1, s, fault)) {
+          if (use > 0 && !tc_wait(&s.empty[slot], (use - 1) & 1, &s.dead, fault)) {
             ok = false;
             break;
           }
@@ -293,7 +253,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     } else if (warp == kPtEpiWarps + 1) {
       // product issuer: the whole warp walks the tiles (so that addresses and
       // descriptors stay uniform), its first lane issues
-      ok = ok && pt_wait(&s.q_full, n_item & 1, s, fault);
+      ok = ok && tc_wait(&s.q_full, n_item & 1, &s.dead, fault);
       tc_fence_after();
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
         // Key plane i against the three query planes side by side (192 rows) is
@@ -305,8 +265,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll 1
         for (uint32_t st = 0; st < 3; ++st, ++ring_n) {
           const uint32_t i = up ? st : 2 - st, slot = ring_n % kPtSlots;
-          ok = ok && pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault);
-          if (st == 1 && kt) ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+          ok = ok && tc_wait(&s.full[slot], (ring_n / kPtSlots) & 1, &s.dead, fault);
+          if (st == 1 && kt) ok = ok && tc_wait(&s.t_free, (n_s - 1) & 1, &s.dead, fault);
           if (!ok) break;
           tc_fence_after();
           const uint64_t key = tc_desc(ring_a + slot * kPtSlot);
@@ -314,52 +274,52 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           // the first product into a diagonal overwrites it: all three of the
           // first plane; then the outermost one of each further plane
           if (st == 0) {
-            pt_mma(col, key, ops_d, tc_idesc_n(true, true, 3 * kPtRows), false, leader);
+            tc_mma_by(col, key, ops_d, tc_idesc_n(true, true, 3 * kPtRows), false, leader);
           } else {
             const uint32_t in = up ? 0 : 1, out = up ? 2 : 0;  // query planes of the other two, and of the outermost
-            pt_mma(col + in * kPtRows, key, ops_d + in * (kPtQPlane / 16), tc_idesc_n(true, true, 2 * kPtRows), true,
+            tc_mma_by(col + in * kPtRows, key, ops_d + in * (kPtQPlane / 16), tc_idesc_n(true, true, 2 * kPtRows), true,
                    leader);
-            pt_mma(col + out * kPtRows, key, ops_d + out * (kPtQPlane / 16), tc_idesc_n(true, true, kPtRows), false,
+            tc_mma_by(col + out * kPtRows, key, ops_d + out * (kPtQPlane / 16), tc_idesc_n(true, true, kPtRows), false,
                    leader);
           }
 #pragma unroll
           for (uint32_t kk = 1; kk < 4; ++kk)
-            pt_mma(col, key + 2 * kk, ops_d + 2 * kk, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
-          pt_commit(&s.empty[slot], leader);
+            tc_mma_by(col, key + 2 * kk, ops_d + 2 * kk, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
+          tc_commit_by(&s.empty[slot], leader);
         }
         if (!ok) break;
-        pt_commit(&s.s_done, leader);
+        tc_commit_by(&s.s_done, leader);
       }
       // the diagonals of the last score tile are read before the value sums take their columns
-      ok = ok && pt_wait(&s.t_free, (n_s - 1) & 1, s, fault);
+      ok = ok && tc_wait(&s.t_free, (n_s - 1) & 1, &s.dead, fault);
       tc_fence_after();
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
         const uint32_t buf = n_w & 1;
-        ok = pt_wait(&s.w_full[buf], (n_w >> 1) & 1, s, fault);
+        ok = tc_wait(&s.w_full[buf], (n_w >> 1) & 1, &s.dead, fault);
         // value plane i against both weight planes (128 rows): diagonals i, i + 1
         const uint64_t w = ops_d + buf * (kPtWBuf / 16);
 #pragma unroll 1
         for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
           const uint32_t slot = ring_n % kPtSlots, col = tmem + i * kPtRows;
-          ok = ok && pt_wait(&s.full[slot], (ring_n / kPtSlots) & 1, s, fault);
+          ok = ok && tc_wait(&s.full[slot], (ring_n / kPtSlots) & 1, &s.dead, fault);
           if (!ok) break;
           tc_fence_after();
           const uint64_t val = tc_desc(ring_a + slot * kPtSlot);
           if (kt == 0 && i) {
-            pt_mma(col, val, w, tc_idesc_n(true, false, kPtRows), true, leader);
-            pt_mma(col + kPtRows, val, w + kPtQPlane / 16, tc_idesc_n(true, false, kPtRows), false, leader);
+            tc_mma_by(col, val, w, tc_idesc_n(true, false, kPtRows), true, leader);
+            tc_mma_by(col + kPtRows, val, w + kPtQPlane / 16, tc_idesc_n(true, false, kPtRows), false, leader);
           } else {
-            pt_mma(col, val, w, tc_idesc_n(true, false, 2 * kPtRows), kt != 0, leader);
+            tc_mma_by(col, val, w, tc_idesc_n(true, false, 2 * kPtRows), kt != 0, leader);
           }
 #pragma unroll
           for (uint32_t kk = 1; kk < 4; ++kk)
-            pt_mma(col, val + 2 * kk, w + 2 * kk, tc_idesc_n(true, false, 2 * kPtRows), true, leader);
-          pt_commit(&s.empty[slot], leader);
+            tc_mma_by(col, val + 2 * kk, w + 2 * kk, tc_idesc_n(true, false, 2 * kPtRows), true, leader);
+          tc_commit_by(&s.empty[slot], leader);
         }
         if (!ok) break;
-        pt_commit(&s.w_empty[buf], leader);
+        tc_commit_by(&s.w_empty[buf], leader);
       }
-      if (ok) pt_commit(&s.v_done, leader);
+      if (ok) tc_commit_by(&s.v_done, leader);
     } else {
       // epilogue warps: TMEM lanes 32 quad .. (keys, then dims), rows 16 cg ..
       const uint32_t quad = warp & 3, cg = warp >> 2;
@@ -374,7 +334,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
       for (uint32_t c = 0; c < 16; ++c) best[c] = INT32_MIN;
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_s) {
-        if (!pt_wait(&s.s_done, n_s & 1, s, fault)) {
+        if (!tc_wait(&s.s_done, n_s & 1, &s.dead, fault)) {
           ok = false;
           break;
         }
@@ -530,7 +490,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       if (ktiles > 1) load_terms(after, 1);
       for (uint32_t kt = 0; kt < ktiles && ok; ++kt, ++n_w) {
         const uint32_t buf = n_w & 1, use = n_w >> 1;
-        if (use > 0 && !pt_wait(&s.w_empty[buf], (use - 1) & 1, s, fault)) {
+        if (use > 0 && !tc_wait(&s.w_empty[buf], (use - 1) & 1, &s.dead, fault)) {
           ok = false;
           break;
         }
@@ -554,12 +514,11 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           for (uint32_t j = 0; j < 8; ++j) all[h] += w[j];
           const uint32_t t0 = __byte_perm(w[0], w[1], 0x5140), t1 = __byte_perm(w[2], w[3], 0x5140);
           const uint32_t u0 = __byte_perm(w[4], w[5], 0x5140), u1 = __byte_perm(w[6], w[7], 0x5140);
-          // 128-byte rows in the 128-byte swizzle: 16-byte pieces exchanged by the row's low bits
-          uint8_t* dst = wb + i * 128 + (((c >> 1) ^ (i & 7)) << 4) + (c & 1) * 8;
+          uint8_t* dst = wb + swizzled(i, 8 * c);
           *(uint2*)dst = make_uint2(__byte_perm(t0, t1, 0x5410), __byte_perm(u0, u1, 0x5410));
           *(uint2*)(dst + kPtQPlane) = make_uint2(__byte_perm(t0, t1, 0x7632), __byte_perm(u0, u1, 0x7632));
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        fence_async_shared();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.w_full[buf]);
       }
@@ -578,7 +537,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * kPtD + 32 * quad + lane]
                     : 0;
       epi_sync();
-      if (ok && pt_wait(&s.v_done, n_item & 1, s, fault)) {
+      if (ok && tc_wait(&s.v_done, n_item & 1, &s.dead, fault)) {
         tc_fence_after();
         uint32_t v[4][16];
 #pragma unroll

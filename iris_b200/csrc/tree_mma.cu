@@ -23,6 +23,7 @@
 #include "serve_attn.cuh"
 #include "serve_mma.cuh"
 #include "tree_mma.cuh"
+#include "tree_tc.cuh"
 
 namespace iris {
 
@@ -30,42 +31,6 @@ namespace {
 
 constexpr uint32_t kTreeThreads = 256, kTreeWarps = kTreeThreads / 32;
 constexpr uint32_t kTreeTile = 32;     // query rows a block works on at a time
-constexpr uint32_t kTreeSegment = 1024;  // keys a warp takes in the second launch
-
-struct TreeScratch {
-  int32_t* scores;     // [rows * heads][pitch], then terms
-  int32_t* chunk_max;  // [rows * heads][chunks]
-  uint64_t* seg_sum;   // [rows * heads][segs]
-  uint32_t* seg_first; // [rows * heads][segs]
-  int64_t* acc;        // [rows * heads][d]
-  int32_t* wsum;       // [rows * heads]
-  uint32_t* done;      // [requests][kv_heads][groups]: finished blocks of the third launch
-  uint32_t pitch, chunk, chunks, segs;
-  uint32_t vchunk, vchunks, groups;  // keys and row groups of the third launch's blocks
-};
-
-// One request's part of the call: its keys from `base` on (a multiple of 64; a
-// window hides all below from every node). Made by whole warps.
-struct TreeRequest {
-  uint32_t begin, nodes, held, keys, group, base, count;
-  __device__ TreeRequest(const IrisTreeAttention& a, uint32_t r) {
-    begin = clamp_offset(a.offsets[r], a.rows);
-    const uint32_t end = clamp_offset(a.offsets[r + 1], a.rows);
-    nodes = end > begin ? min(end - begin, a.nodes) : 0;
-    held = tree_held(a, r);
-    keys = min(held + nodes, a.longest);
-    group = a.heads / a.kv_heads;
-    base = 0;
-    if (a.window) {
-      uint32_t low = held;
-      for (uint32_t i = threadIdx.x & 31; i < nodes; i += 32)
-        low = min(low, window_start((uint32_t)a.positions[begin + i], a.window));
-      base = min(__reduce_min_sync(0xffffffffu, low), keys) / 64 * 64;
-    }
-    count = keys - base;
-  }
-};
-
 __device__ __forceinline__ bool is_visible(const IrisTreeAttention& a, const TreeRequest& q, uint32_t node,
                                            uint32_t key) {
   const uint32_t row = q.begin + node;
@@ -82,10 +47,12 @@ __global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAt
   __shared__ int32_t row_max[kTreeTile];
   __shared__ uint32_t q_wide;
   const uint32_t chunk = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+  pdl_wait();
+  if (sc.flags && !*sc.flags) return;  // the tensor-core launch did the work
   const TreeRequest q(a, r);
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, steps = a.head_dim / 32;
   const uint32_t rows = q.nodes * q.group, key0 = q.base + chunk * sc.chunk;
-  if (chunk == 0) {  // the totals of this request and head start at zero
+  if (chunk == 0 && !sc.flags) {  // the totals of this request and head start at zero
     for (uint32_t i = tid; i < rows * a.head_dim; i += kTreeThreads) {
       const uint32_t f = i / a.head_dim, x = i % a.head_dim;
       const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
@@ -361,6 +328,7 @@ __global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeA
   }
   if (tid == 0) s.wide = 0;
   pdl_wait();
+  if (sc.flags && !sc.flags[1]) return;  // the tensor-core launch did the work
   for (uint32_t i = warp; i < tile; i += kValueWarps) {
     const uint32_t f = f0 + i;
     uint64_t sum = 0;
@@ -433,6 +401,7 @@ uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   const size_t rows = (size_t)a.rows * a.heads;
   sc->chunk = keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 2 * 148);
+  if (tree_tc_usable(a) && sc->chunk < 128) sc->chunk = 128;  // whole key tiles of the tensor-core launch
   sc->chunks = ceil_div(a.longest, sc->chunk);
   sc->groups = ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
   sc->vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->groups, a.longest, 4096, 2 * 148);
@@ -452,6 +421,19 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   sc->acc = (int64_t*)take(rows * a.head_dim * 8);
   sc->wsum = (int32_t*)take(rows * 4);
   sc->done = (uint32_t*)take((size_t)a.requests * a.kv_heads * sc->groups * 4);
+  sc->flags = nullptr;
+  if (tree_tc_usable(a)) {
+    const uint32_t rows_most = a.nodes * (a.heads / a.kv_heads);
+    sc->tc_rows = rows_most <= 64 ? 64 : 128;
+    sc->tc_groups = ceil_div(rows_most, sc->tc_rows);
+    sc->tc_vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->tc_groups, a.longest, 4096, 4 * 148);
+    if (sc->tc_vchunk < 128) sc->tc_vchunk = 128;
+    sc->tc_vchunks = ceil_div(a.longest, sc->tc_vchunk);
+    sc->tc_acc = (int64_t*)take(rows * a.head_dim * 8);
+    sc->tc_wsum = (int32_t*)take(rows * 4);
+    sc->tc_done = (uint32_t*)take((size_t)a.requests * a.kv_heads * sc->tc_groups * 4);
+    sc->flags = (uint32_t*)take(8);
+  }
   return at;
 }
 
@@ -485,11 +467,22 @@ uint64_t tree_mma_workspace(const IrisTreeAttention& a) {
 cudaError_t launch_tree_mma(const IrisTreeAttention& a, uint8_t* workspace, cudaStream_t stream) {
   TreeScratch sc;
   carve(a, workspace, &sc);
-  tree_scores_kernel<<<dim3(sc.chunks, a.kv_heads, a.requests), kTreeThreads, score_smem(a.head_dim), stream>>>(a, sc);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e;
+  if (sc.flags) {
+    e = cudaMemsetAsync(sc.flags, 0, 8, stream);
+    if (e == cudaSuccess) e = launch_tree_tc_scores(a, sc, stream);
+    if (e != cudaSuccess) return e;
+    e = launch_k(tree_scores_kernel, dim3(sc.chunks, a.kv_heads, a.requests), dim3(kTreeThreads),
+                 score_smem(a.head_dim), stream, a, sc);
+  } else {
+    tree_scores_kernel<<<dim3(sc.chunks, a.kv_heads, a.requests), kTreeThreads, score_smem(a.head_dim), stream>>>(a,
+                                                                                                              sc);
+    e = cudaGetLastError();
+  }
   if (e != cudaSuccess) return e;
   e = launch_k(tree_terms_kernel, dim3(ceil_div(a.nodes * a.heads, kTreeWarps), sc.segs, a.requests),
                dim3(kTreeThreads), 0, stream, a, sc);
+  if (e == cudaSuccess && sc.flags) e = launch_tree_tc_values(a, sc, stream);
   if (e != cudaSuccess) return e;
   const uint32_t smem = value_smem(a.head_dim, sc.vchunk, value_rows(a));
   const dim3 grid(sc.vchunks, a.kv_heads * sc.groups, a.requests);

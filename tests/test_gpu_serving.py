@@ -108,12 +108,13 @@ def test_scores_at_the_lowest_value(S, heads, kv_heads, d, step):
         got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 300, heads=heads, kv_heads=kv_heads,
                                  window=window).cpu().numpy()
         assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, 0, window))
-    x = tree_inputs(rng, [150, 0], [9, 5], heads, kv_heads, d, 16, "model", holes=[(0, 3, -1)])
-    x["q"][:] = 1 << 22
-    x["k_pages"][:] = unit + step
-    x["k_pages"][::3] += 9 if step > 1 else -3
-    x["masks"][12] = 0
-    check_tree(S, x, heads, kv_heads, 0, 0, [9, 5])
+    for held, nodes in (([150, 0], [9, 5]), ([600, 0], [20, 13])):
+        x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model", holes=[(0, 3, -1)])
+        x["q"][:] = 1 << 22
+        x["k_pages"][:] = unit + step
+        x["k_pages"][::3] += 9 if step > 1 else -3
+        x["masks"][sum(nodes) - 2] = 0
+        check_tree(S, x, heads, kv_heads, 0, 0, nodes)
 
 
 def test_prompt_attention_over_parts_of_fused_rows_and_a_strided_output(S):
@@ -209,6 +210,14 @@ TREES = [
     ([45], [6], 4, 2, 36, False, 0, 16, "full"),
     ([700], [5], 4, 1, 128, True, 0, 16, "zero"),         # equal scores
     ([1500], [2], 2, 1, 64, True, 0, 16, "equal"),
+    # 24 rows of a K/V head or more, heads of 128 values, 512 keys or more
+    ([600, 0, 33, 515], [13, 7, 0, 24], 8, 2, 128, True, 0, 16, "model"),
+    ([1030, 2], [64, 1], 2, 2, 128, True, 0, 16, "model"),
+    ([520], [64], 8, 1, 128, False, 0, 16, "model"),     # 512 rows
+    ([500, 700], [30, 12], 3, 1, 128, True, 100, 5, "model"),
+    ([530, 64], [9, 30], 4, 1, 128, True, 0, 16, "wide"),
+    ([540], [8], 4, 1, 128, False, 0, 16, "full"),
+    ([900, 100], [6, 8], 4, 1, 128, True, 0, 64, "equal"),
 ]
 
 
@@ -233,6 +242,11 @@ def test_masks_that_leave_rows_empty_and_tables_with_holes(S, d):
     x["table"][1, :] = -1     # nothing of the request is in the pool
     got = check_tree(S, x, 4, 2, scale_of(d), 0, nodes)
     assert not got[4:].any()
+    held, nodes = [0, 700, 40], [14, 12, 3]
+    x = tree_inputs(rng, held, nodes, 4, 2, d, 16, "model", holes=[(1, 0, -1), (1, 30, 10**6), (1, 44, -7)])
+    x["masks"][1], x["masks"][2], x["masks"][20], x["masks"][21] = 0, 1 << 1, 0, -1
+    got = check_tree(S, x, 4, 2, scale_of(d), 0, nodes)
+    assert not got[1].any()
 
 
 def test_tree_attention_of_a_long_context(S):
@@ -240,6 +254,14 @@ def test_tree_attention_of_a_long_context(S):
     held, nodes, heads, kv_heads, d = [20000, 9000], [3, 2], 2, 1, 128
     x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model")
     check_tree(S, x, heads, kv_heads, scale_of(d), 0, nodes)
+
+
+def test_tree_attention_of_wide_trees_over_a_long_context(S):
+    rng = np.random.default_rng(22)
+    held, nodes, heads, kv_heads, d = [9000, 4100], [7, 3], 4, 1, 128
+    x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model")
+    check_tree(S, x, heads, kv_heads, scale_of(d), 0, nodes)
+    check_tree(S, x, heads, kv_heads, scale_of(d), 6000, nodes)
 
 
 def test_drafted_rows_equal_one_by_one_decoding(S):
