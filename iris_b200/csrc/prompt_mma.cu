@@ -32,6 +32,7 @@ constexpr uint32_t kSortRequests = 1024;
 struct PromptScratch {
   uint32_t* order;   // [requests]: the requests, longest first
   uint32_t* tiles;   // [requests + 1]: tiles before each of them
+  uint32_t* tc_tiles;  // the same for prompt_tc_kernel's tiles
   uint32_t* next;    // the item counters of this kernel and of prompt_tc_kernel
   int32_t* scores;   // [blocks][RT][pitch]
   int64_t* acc;      // [blocks][RT][d]: value sums, where several warps or segments add to one
@@ -41,7 +42,8 @@ struct PromptScratch {
 };
 
 // The tiles of each request, longest first (up to 1024 requests; more keep
-// their order), and the item counter.
+// their order), and the item counters. The second block, where there is one,
+// counts the tensor-core kernel's tiles of 64 rows.
 __global__ void __launch_bounds__(1024) prompt_items_kernel(IrisPromptAttention a, PromptScratch sc, uint32_t rt) {
   __shared__ int32_t len_s[kSortRequests];
   __shared__ uint32_t part[32];
@@ -52,8 +54,10 @@ __global__ void __launch_bounds__(1024) prompt_items_kernel(IrisPromptAttention 
     return e > b ? min(e - b, a.longest) : 0u;
   };
   pdl_trigger();
+  uint32_t* tiles = blockIdx.x ? sc.tc_tiles : sc.tiles;
+  if (blockIdx.x) rt = 64;
   if (tid == 0) {
-    sc.next[0] = sc.next[1] = 0;
+    sc.next[blockIdx.x] = 0;
     carry = 0;
   }
   const bool sorted = a.requests <= kSortRequests;
@@ -83,12 +87,12 @@ __global__ void __launch_bounds__(1024) prompt_items_kernel(IrisPromptAttention 
     __syncthreads();
     uint32_t before = carry + incl - n;
     for (uint32_t w = 0; w < warp; ++w) before += part[w];
-    if (r < a.requests) sc.tiles[r] = before;
+    if (r < a.requests) tiles[r] = before;
     __syncthreads();
     if (tid == 1023) carry = before + n;
     __syncthreads();
   }
-  if (tid == 0) sc.tiles[a.requests] = carry;
+  if (tid == 0) tiles[a.requests] = carry;
 }
 
 // One tile: rows f0 .. f0 + RT - 1 of a request's len * group rows (row f is
@@ -385,10 +389,10 @@ constexpr uint32_t kTcLongest = 256;
 bool on_tensor_cores(const IrisPromptAttention& a) { return a.longest >= kTcLongest && prompt_tc_usable(a); }
 
 size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, PromptTcScratch* tc) {
-  const uint32_t rt = row_tile(a), group = a.heads / a.kv_heads;
+  const uint32_t rt = row_tile(a), group = a.heads / a.kv_heads, most = on_tensor_cores(a) ? 64 : rt;
   const uint64_t tiles = ((uint64_t)a.tokens * group + rt - 1) / rt + a.requests;
   sc->blocks = (uint32_t)std::min<uint64_t>(tiles * a.kv_heads, (uint64_t)device_sms());
-  const uint32_t keys = a.window ? std::min<uint64_t>(a.longest, (uint64_t)a.window + rt + 16) : a.longest;
+  const uint32_t keys = a.window ? std::min<uint64_t>(a.longest, (uint64_t)a.window + most + 16) : a.longest;
   sc->pitch = (keys + 15 + 127) / 128 * 128;  // a tile's first key is rounded down to 16, its last up to 128
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -398,15 +402,16 @@ size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, Pro
   };
   sc->next = (uint32_t*)take(8);
   sc->tiles = (uint32_t*)take(((size_t)a.requests + 1) * 4);
+  sc->tc_tiles = (uint32_t*)take(((size_t)a.requests + 1) * 4);
   sc->order = (uint32_t*)take((size_t)a.requests * 4);
-  sc->scores = (int32_t*)take((size_t)sc->blocks * rt * sc->pitch * 4);
+  sc->scores = (int32_t*)take((size_t)sc->blocks * most * sc->pitch * 4);
   sc->acc = (int64_t*)take((size_t)sc->blocks * rt * a.head_dim * 8);
   sc->wide = nullptr;
   sc->flags = 0;
   if (on_tensor_cores(a)) {
     at += prompt_tc_carve(a, base + at, tc);
     tc->order = sc->order;
-    tc->tiles = sc->tiles;
+    tc->tiles = sc->tc_tiles;
     tc->next = sc->next + 1;
     tc->scores = sc->scores;
     tc->pitch = sc->pitch;
@@ -424,7 +429,7 @@ cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, const 
   static std::atomic<bool> allowed[64];
   cudaError_t e = allow_smem(prompt_mma_kernel<RT>, allowed);
   if (e != cudaSuccess) return e;
-  prompt_items_kernel<<<1, 1024, 0, stream>>>(a, sc, RT);
+  prompt_items_kernel<<<sc.flags ? 2 : 1, 1024, 0, stream>>>(a, sc, RT);
   e = cudaGetLastError();
   if (e == cudaSuccess && sc.flags) e = launch_prompt_tc(a, tc, sc.blocks, stream);
   if (e != cudaSuccess) return e;

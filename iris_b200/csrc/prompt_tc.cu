@@ -1,11 +1,12 @@
-// Packed prompt attention on the tcgen05 tensor cores (kind::i8), head_dim 128.
+// Packed prompt attention on the tcgen05 tensor cores (kind::i8), heads of up to
+// 256 values: in one or two chunks (DC) of 128, padded with zeros.
 //
 // The same three phases as prompt_mma.cu, with the contractions on the
 // fifth-generation tensor cores. Operands are packed once a call into K-major
 // byte planes (three signed digits: 24-bit values, nearly; where any operand is wider the kernel
 // leaves the call to prompt_mma_kernel, launched behind it, which then runs):
-// queries [K/V head][plane][token * group + head][128], keys [head][plane]
-// [token][128], values transposed [head][plane][128][token]. A tile of 64 query
+// queries [K/V head][plane][token * group + head][128 DC], keys [head][plane]
+// [token][128 DC], values transposed [head][plane][128 DC][token]. A tile of 64 query
 // rows that share a K/V head goes through
 //   1. scores: 128 keys x 192 rows x 32 dims a product (one key plane against
 //      the three query planes side by side), nine plane pairs into five int32
@@ -40,31 +41,36 @@ namespace iris {
 
 namespace {
 
-constexpr uint32_t kPtD = 128, kPtRows = 64, kPtKeys = 128;
+constexpr uint32_t kPtD = 128, kPtRows = 64, kPtKeys = 128;  // dims of a chunk, query rows, keys of a tile
 constexpr uint32_t kPtEpiWarps = 16, kPtEpi = 32 * kPtEpiWarps, kPtThreads = kPtEpi + 64;
-constexpr uint32_t kPtSlots = 5, kPtSlot = kPtKeys * kPtD;  // one plane of a key or value tile
-constexpr uint32_t kPtQPlane = kPtRows * kPtD;              // one plane of the query rows; of a weight tile
-constexpr uint32_t kPtWBuf = 2 * kPtQPlane;                 // two weight planes
+constexpr uint32_t kPtSlot = kPtKeys * kPtD;     // one plane and chunk of a key or value tile
+constexpr uint32_t kPtQPlane = kPtRows * kPtD;   // one plane and chunk of the query rows; of a weight tile
+constexpr uint32_t kPtWBuf = 2 * kPtQPlane;      // two weight planes
+constexpr uint32_t kPtBlock = kPtRows * kPtKeys;  // scores of a key tile: [row][key]
 constexpr uint32_t kPtFar = kExpTerms - kExpExactBelow;  // distances with a correction bit
 constexpr uint32_t kPtTable = kPtFar / 32;               // words
-constexpr uint32_t kPtBlock = kPtRows * kPtKeys;           // scores of a key tile: [row][key]
-constexpr uint32_t kPtRing = kPtSlots * kPtSlot;
-constexpr uint32_t kPtOperands = 2 * kPtWBuf;  // the query planes (3 x 8 KB), later two weight buffers
-constexpr uint32_t kPtList = kPtOperands / 4 / kPtEpiWarps;  // words of a warp's list of near scores
-constexpr uint32_t kPtNearBits = 18;                         // kExpExactBelow below 2^18, places below 2^14
+constexpr uint32_t kPtNearBits = 18;                     // kExpExactBelow below 2^18, places below 2^14
 constexpr uint32_t kPtLongest = (1u << (32 - kPtNearBits)) - kPtKeys;
-static_assert(kExpExactBelow < 1u << kPtNearBits && kPtList >= 512, "list entries");
+static_assert(kExpExactBelow < 1u << kPtNearBits, "list entries");
 static_assert(kPtLongest + 15 + kPtKeys <= kPvKeys + kPtKeys, "int32 diagonals of the value sums");
-constexpr uint32_t kPtSmem = 1024 + kPtRing + kPtOperands + kPtTable * 4;
-static_assert(3 * kPtQPlane <= kPtOperands, "query planes");
 static_assert(8 * kPtRows == 512, "TMEM column groups");
+
+template <uint32_t DC>
+struct PtLayout {
+  static constexpr uint32_t kSlots = DC == 1 ? 5 : 3;
+  static constexpr uint32_t kRing = kSlots * kPtSlot;
+  static constexpr uint32_t kQuery = 3 * DC * kPtQPlane;  // [chunk][plane][row][128]
+  static constexpr uint32_t kOperands = kQuery > 2 * kPtWBuf ? kQuery : 2 * kPtWBuf;  // the queries, later two weight buffers
+  static constexpr uint32_t kList = kOperands / 4 / kPtEpiWarps;  // words of a warp's list of near scores
+  static constexpr uint32_t kSmem = 1024 + kRing + kOperands + kPtTable * 4;
+  static_assert(kList >= 512, "list entries");
+};
 
 // ---- packing -------------------------------------------------------------------
 
-// Rows of 128 values (row r, part g at src + (r / per) * stride + (g * per + r %
-// per) * 128) into planes dst[g][3][rows][128]; flags what is past 24 bits.
+// Four values (zeros where src is NULL) into three planes; what is past 24 bits.
 __device__ __forceinline__ uint32_t pack_row4(const int32_t* src, uint8_t* dst, uint64_t plane) {
-  const int4 x = *(const int4*)src;
+  const int4 x = src ? *(const int4*)src : make_int4(0, 0, 0, 0);
   uint32_t p[4];
   split_digits(x.x, x.y, x.z, x.w, p);
 #pragma unroll
@@ -76,7 +82,9 @@ constexpr uint32_t kPackThreads = 256;
 
 // blockIdx.y: 0 queries, 1 keys, 2 values (transposed through shared memory, 32
 // tokens x 32 dims a pass), 3 the exponential's correction bits.
+template <uint32_t DC>
 __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAttention a, PromptTcScratch sc) {
+  constexpr uint32_t DP = DC * kPtD;  // dims a packed row
   __shared__ int32_t tile[32][33];
   const uint32_t tid = threadIdx.x, group = a.heads / a.kv_heads;
   pdl_trigger();
@@ -84,27 +92,28 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
   if (blockIdx.y <= 1) {
     const bool keys = blockIdx.y == 1;
     const uint32_t per = keys ? 1 : group;
-    const uint64_t rows = (uint64_t)a.tokens * per, n = rows * a.kv_heads * 32;
+    const uint64_t rows = (uint64_t)a.tokens * per, n = rows * a.kv_heads * (DP / 4);
     const int32_t* src = keys ? a.k : a.q;
     const uint64_t stride = keys ? a.k_stride : a.q_stride;
     uint8_t* dst = keys ? sc.kp : sc.qp;
     for (uint64_t i = (uint64_t)blockIdx.x * kPackThreads + tid; i < n; i += (uint64_t)gridDim.x * kPackThreads) {
-      const uint32_t c = (uint32_t)(i & 31), h = (uint32_t)((i >> 5) % (per * a.kv_heads));
-      const uint64_t token = (i >> 5) / (per * a.kv_heads);
+      const uint32_t c = (uint32_t)(i % (DP / 4)), h = (uint32_t)(i / (DP / 4) % (per * a.kv_heads));
+      const uint64_t token = i / (DP / 4) / (per * a.kv_heads);
       const uint64_t row = token * per + h % per;
-      wide |= pack_row4(src + token * stride + (uint64_t)h * kPtD + 4 * c,
-                        dst + ((uint64_t)(h / per) * 3 * rows + row) * kPtD + 4 * c, rows * kPtD);
+      wide |= pack_row4(4 * c < a.head_dim ? src + token * stride + (uint64_t)h * a.head_dim + 4 * c : nullptr,
+                        dst + ((uint64_t)(h / per) * 3 * rows + row) * DP + 4 * c, rows * DP);
     }
   } else if (blockIdx.y == 2) {
     const uint32_t tx = tid & 31, ty = tid >> 5;
     const uint32_t tts = (a.tokens + 31) / 32;
-    for (uint64_t u = blockIdx.x; u < (uint64_t)tts * 4 * a.kv_heads; u += gridDim.x) {
-      const uint32_t g = (uint32_t)(u % a.kv_heads), d0 = (uint32_t)(u / a.kv_heads % 4) * 32,
-                     t0 = (uint32_t)(u / a.kv_heads / 4) * 32;
+    for (uint64_t u = blockIdx.x; u < (uint64_t)tts * (DP / 32) * a.kv_heads; u += gridDim.x) {
+      const uint32_t g = (uint32_t)(u % a.kv_heads), d0 = (uint32_t)(u / a.kv_heads % (DP / 32)) * 32,
+                     t0 = (uint32_t)(u / a.kv_heads / (DP / 32)) * 32;
       __syncthreads();
       for (uint32_t r = ty; r < 32; r += 8) {
         const uint32_t t = t0 + r;
-        tile[r][tx] = t < a.tokens ? a.v[(uint64_t)t * a.v_stride + g * kPtD + d0 + tx] : 0;
+        tile[r][tx] =
+            t < a.tokens && d0 + tx < a.head_dim ? a.v[(uint64_t)t * a.v_stride + g * a.head_dim + d0 + tx] : 0;
       }
       __syncthreads();
       // thread: dimension tid / 8, four tokens
@@ -114,7 +123,7 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
       wide |= p[3];
 #pragma unroll
       for (uint32_t i = 0; i < 3; ++i)
-        *(uint32_t*)(sc.vt + (((uint64_t)g * 3 + i) * kPtD + d0 + d) * sc.tpitch + t0 + t) = p[i];
+        *(uint32_t*)(sc.vt + (((uint64_t)g * 3 + i) * DP + d0 + d) * sc.tpitch + t0 + t) = p[i];
     }
   } else {
     const uint32_t lane = tid & 31;
@@ -132,7 +141,7 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
 // ---- the attention ----------------------------------------------------------------
 
 struct PtShared {
-  uint64_t full[kPtSlots], empty[kPtSlots], q_full, s_done, t_free, w_full[2], w_empty[2], v_done;
+  uint64_t full[PtLayout<1>::kSlots], empty[PtLayout<1>::kSlots], q_full, s_done, t_free, w_full[2], w_empty[2], v_done;
   uint64_t sum[kPtRows];
   int32_t top[kPtRows], query[kPtRows], wsum[kPtRows];
   uint32_t recip[kPtRows], first[kPtRows];
@@ -154,15 +163,18 @@ __device__ __forceinline__ void terms_by_table(const int4 (&x)[2], int32_t top, 
   }
 }
 
+template <uint32_t DC>
 __global__ void __launch_bounds__(kPtThreads, 1)
     prompt_tc_kernel(IrisPromptAttention a, PromptTcScratch sc, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      unsigned int* fault) {
+  using L = PtLayout<DC>;
+  constexpr uint32_t kPtSlots = L::kSlots, kPtList = L::kList;
   extern __shared__ uint8_t pt_raw[];
   __shared__ __align__(8) PtShared s;
   uint8_t* ring = (uint8_t*)(((uintptr_t)pt_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t* ops = ring + kPtRing;  // query planes, then weight buffers
-  uint32_t* bits = (uint32_t*)(ops + kPtOperands);
+  uint8_t* ops = ring + L::kRing;  // query planes, then weight buffers
+  uint32_t* bits = (uint32_t*)(ops + L::kOperands);
   const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   const bool leader = lane == 0;
   if (tid == 0) {
@@ -230,22 +242,24 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 
     if (warp == kPtEpiWarps) {
       if (lane == 0) {  // TMA producer
-        mbar_arrive_expect_tx(&s.q_full, 3 * kPtQPlane);
-        for (uint32_t j = 0; j < 3; ++j)
-          tma_load_3d(ops + j * kPtQPlane, &qmap, 0, (int32_t)(begin * group + f0), (int32_t)(g * 3 + j), &s.q_full);
-        for (uint32_t u = 0; u < 6 * ktiles && ok; ++u, ++ring_n) {
+        mbar_arrive_expect_tx(&s.q_full, L::kQuery);
+        for (uint32_t j = 0; j < 3 * DC; ++j)
+          tma_load_3d(ops + j * kPtQPlane, &qmap, (int32_t)(j / 3 * kPtD), (int32_t)(begin * group + f0),
+                      (int32_t)(g * 3 + j % 3), &s.q_full);
+        for (uint32_t u = 0; u < 6 * DC * ktiles && ok; ++u, ++ring_n) {
           const uint32_t slot = ring_n % kPtSlots, use = ring_n / kPtSlots;
           if (use > 0 && !tc_wait(&s.empty[slot], (use - 1) & 1, &s.dead, fault)) {
             ok = false;
             break;
           }
           mbar_arrive_expect_tx(&s.full[slot], kPtSlot);
-          const bool vals = u >= 3 * ktiles;
-          const uint32_t v = vals ? u - 3 * ktiles : u, kt = v / 3, t = k0 + kt * kPtKeys;
-          // (every other score tile takes its planes from the last on)
-          const uint32_t plane = g * 3 + (vals || ((n_s + kt) & 1) == 0 ? v % 3 : 2 - v % 3);
-          if (vals) tma_load_3d(ring + slot * kPtSlot, &vmap, (int32_t)t, 0, (int32_t)plane, &s.full[slot]);
-          else tma_load_3d(ring + slot * kPtSlot, &kmap, 0, (int32_t)t, (int32_t)plane, &s.full[slot]);
+          const bool vals = u >= 3 * DC * ktiles;
+          const uint32_t v = vals ? u - 3 * DC * ktiles : u, kt = v / (3 * DC), t = k0 + kt * kPtKeys;
+          // a tile's planes, each in its chunks (every other score tile takes its planes from the last on)
+          const uint32_t j = v / DC % 3, plane = g * 3 + (vals || ((n_s + kt) & 1) == 0 ? j : 2 - j);
+          const int32_t c0 = (int32_t)(v % DC * kPtD);
+          if (vals) tma_load_3d(ring + slot * kPtSlot, &vmap, (int32_t)t, c0, (int32_t)plane, &s.full[slot]);
+          else tma_load_3d(ring + slot * kPtSlot, &kmap, c0, (int32_t)t, (int32_t)plane, &s.full[slot]);
           ++issued[slot];
         }
         n_s += ktiles;
@@ -263,28 +277,30 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const bool up = (n_s & 1) == 0;
         const uint32_t cols = tmem + (up ? 0 : 3 * kPtRows);
 #pragma unroll 1
-        for (uint32_t st = 0; st < 3; ++st, ++ring_n) {
-          const uint32_t i = up ? st : 2 - st, slot = ring_n % kPtSlots;
+        for (uint32_t u = 0; u < 3 * DC; ++u, ++ring_n) {
+          const uint32_t st = u / DC, c = u % DC, i = up ? st : 2 - st, slot = ring_n % kPtSlots;
           ok = ok && tc_wait(&s.full[slot], (ring_n / kPtSlots) & 1, &s.dead, fault);
-          if (st == 1 && kt) ok = ok && tc_wait(&s.t_free, (n_s - 1) & 1, &s.dead, fault);
+          if (u == DC && kt) ok = ok && tc_wait(&s.t_free, (n_s - 1) & 1, &s.dead, fault);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t key = tc_desc(ring_a + slot * kPtSlot);
+          const uint64_t key = tc_desc(ring_a + slot * kPtSlot), qd = ops_d + c * (3 * kPtQPlane / 16);
           const uint32_t col = cols + i * kPtRows;
           // the first product into a diagonal overwrites it: all three of the
           // first plane; then the outermost one of each further plane
-          if (st == 0) {
-            tc_mma_by(col, key, ops_d, tc_idesc_n(true, true, 3 * kPtRows), false, leader);
-          } else {
+          if (c == 0 && st == 0) {
+            tc_mma_by(col, key, qd, tc_idesc_n(true, true, 3 * kPtRows), false, leader);
+          } else if (c == 0) {
             const uint32_t in = up ? 0 : 1, out = up ? 2 : 0;  // query planes of the other two, and of the outermost
-            tc_mma_by(col + in * kPtRows, key, ops_d + in * (kPtQPlane / 16), tc_idesc_n(true, true, 2 * kPtRows), true,
-                   leader);
-            tc_mma_by(col + out * kPtRows, key, ops_d + out * (kPtQPlane / 16), tc_idesc_n(true, true, kPtRows), false,
-                   leader);
+            tc_mma_by(col + in * kPtRows, key, qd + in * (kPtQPlane / 16), tc_idesc_n(true, true, 2 * kPtRows), true,
+                      leader);
+            tc_mma_by(col + out * kPtRows, key, qd + out * (kPtQPlane / 16), tc_idesc_n(true, true, kPtRows), false,
+                      leader);
+          } else {
+            tc_mma_by(col, key, qd, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
           }
 #pragma unroll
           for (uint32_t kk = 1; kk < 4; ++kk)
-            tc_mma_by(col, key + 2 * kk, ops_d + 2 * kk, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
+            tc_mma_by(col, key + 2 * kk, qd + 2 * kk, tc_idesc_n(true, true, 3 * kPtRows), true, leader);
           tc_commit_by(&s.empty[slot], leader);
         }
         if (!ok) break;
@@ -299,8 +315,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         // value plane i against both weight planes (128 rows): diagonals i, i + 1
         const uint64_t w = ops_d + buf * (kPtWBuf / 16);
 #pragma unroll 1
-        for (uint32_t i = 0; i < 3; ++i, ++ring_n) {
-          const uint32_t slot = ring_n % kPtSlots, col = tmem + i * kPtRows;
+        for (uint32_t u = 0; u < 3 * DC; ++u, ++ring_n) {
+          // (dims 128 c .. have four column groups of their own)
+          const uint32_t i = u / DC, c = u % DC, slot = ring_n % kPtSlots, col = tmem + (4 * c + i) * kPtRows;
           ok = ok && tc_wait(&s.full[slot], (ring_n / kPtSlots) & 1, &s.dead, fault);
           if (!ok) break;
           tc_fence_after();
@@ -530,32 +547,40 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if ((lane & 15) == 0) s.wsum[(tid >> 4) + 32 * h] = x;
       }
       // the first maxima's values, ahead of the last products
-      int32_t vf[16];
+      int32_t vf[DC][16];
 #pragma unroll
-      for (uint32_t c = 0; c < 16; ++c)
-        vf[c] = cg * 16 + c < rows
-                    ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * kPtD + 32 * quad + lane]
-                    : 0;
+      for (uint32_t h = 0; h < DC; ++h)
+#pragma unroll
+        for (uint32_t c = 0; c < 16; ++c) {
+          const uint32_t x = h * kPtD + 32 * quad + lane;
+          vf[h][c] = cg * 16 + c < rows && x < a.head_dim
+                         ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * a.head_dim + x]
+                         : 0;
+        }
       epi_sync();
       if (ok && tc_wait(&s.v_done, n_item & 1, &s.dead, fault)) {
         tc_fence_after();
-        uint32_t v[4][16];
 #pragma unroll
-        for (uint32_t d = 0; d < 4; ++d) {
-          tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16, v[d]);
-          tmem_ld8(tmem + ((32 * quad) << 16) + d * kPtRows + cg * 16 + 8, v[d] + 8);
-        }
-        tmem_ld_wait();
-        const uint32_t x = 32 * quad + lane;
+        for (uint32_t h = 0; h < DC; ++h) {
+          uint32_t v[4][16];
 #pragma unroll
-        for (uint32_t c = 0; c < 16; ++c) {
-          const uint32_t i = cg * 16 + c;
-          if (i < rows) {
-            const int32_t y[4] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c]};
-            int64_t total = diagonal_sum(y);
-            mac_wide(total, sub_sat(kOneAct, s.wsum[i]), vf[c]);
-            a.out[(uint64_t)(begin + s.query[i]) * a.out_stride + (g * group + (f0 + i) % group) * kPtD + x] =
-                requantize(total);
+          for (uint32_t d = 0; d < 4; ++d) {
+            const uint32_t col = tmem + ((32 * quad) << 16) + (4 * h + d) * kPtRows + cg * 16;
+            tmem_ld8(col, v[d]);
+            tmem_ld8(col + 8, v[d] + 8);
+          }
+          tmem_ld_wait();
+          const uint32_t x = h * kPtD + 32 * quad + lane;
+#pragma unroll
+          for (uint32_t c = 0; c < 16; ++c) {
+            const uint32_t i = cg * 16 + c;
+            if (i < rows && x < a.head_dim) {
+              const int32_t y[4] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c]};
+              int64_t total = diagonal_sum(y);
+              mac_wide(total, sub_sat(kOneAct, s.wsum[i]), vf[h][c]);
+              a.out[(uint64_t)(begin + s.query[i]) * a.out_stride + (g * group + (f0 + i) % group) * a.head_dim + x] =
+                  requantize(total);
+            }
           }
         }
       } else {
@@ -580,12 +605,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 }  // namespace
 
 bool prompt_tc_usable(const IrisPromptAttention& a) {
-  return a.head_dim == kPtD && a.longest <= kPtLongest && a.tokens >= kPtKeys && (uint64_t)a.tokens * (a.heads / a.kv_heads) < 0x7FFFFFFFull &&
-         (uint64_t)a.kv_heads * 3 < 0x7FFFFFFFull && tensor_map_encoder() != nullptr && device_fault_word() != nullptr;
+  return a.head_dim <= 2 * kPtD && a.longest <= kPtLongest && a.tokens >= kPtKeys &&
+         (uint64_t)a.tokens * (a.heads / a.kv_heads) < 0x7FFFFFFFull && (uint64_t)a.kv_heads * 3 < 0x7FFFFFFFull &&
+         tensor_map_encoder() != nullptr && device_fault_word() != nullptr;
 }
 
 size_t prompt_tc_carve(const IrisPromptAttention& a, uint8_t* base, PromptTcScratch* sc) {
-  const uint64_t group = a.heads / a.kv_heads;
+  const uint64_t group = a.heads / a.kv_heads, dp = a.head_dim <= kPtD ? kPtD : 2 * kPtD;
   sc->tpitch = (a.tokens + 127) / 128 * 128;
   sc->pack_blocks = 148 * 4;
   sc->flags = 4 * sc->pack_blocks;
@@ -595,29 +621,39 @@ size_t prompt_tc_carve(const IrisPromptAttention& a, uint8_t* base, PromptTcScra
     at += (bytes + 255) / 256 * 256;
     return p;
   };
-  sc->qp = take((size_t)a.kv_heads * 3 * a.tokens * group * kPtD);
-  sc->kp = take((size_t)a.kv_heads * 3 * a.tokens * kPtD);
-  sc->vt = take((size_t)a.kv_heads * 3 * kPtD * sc->tpitch);
+  sc->qp = take((size_t)a.kv_heads * 3 * a.tokens * group * dp);
+  sc->kp = take((size_t)a.kv_heads * 3 * a.tokens * dp);
+  sc->vt = take((size_t)a.kv_heads * 3 * dp * sc->tpitch);
   sc->exp_bits = (uint32_t*)take((size_t)kPtTable * 4);
   sc->wide = (uint32_t*)take((size_t)sc->flags * 4);
   return at;
 }
 
-cudaError_t launch_prompt_tc(const IrisPromptAttention& a, const PromptTcScratch& sc, uint32_t blocks,
-                             cudaStream_t stream) {
-  const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads);
+namespace {
+
+template <uint32_t DC>
+cudaError_t launch(const IrisPromptAttention& a, const PromptTcScratch& sc, uint32_t blocks, cudaStream_t stream) {
+  constexpr uint64_t DP = DC * kPtD;
+  const uint64_t rows = (uint64_t)a.tokens * (a.heads / a.kv_heads), planes = (uint64_t)a.kv_heads * 3;
   CUtensorMap qmap, kmap, vmap;
-  if (!make_map(&qmap, sc.qp, kPtD, rows, (uint64_t)a.kv_heads * 3, kPtD, rows * kPtD, kPtRows, 1) ||
-      !make_map(&kmap, sc.kp, kPtD, a.tokens, (uint64_t)a.kv_heads * 3, kPtD, (uint64_t)a.tokens * kPtD, kPtKeys, 1) ||
-      !make_map(&vmap, sc.vt, sc.tpitch, kPtD, (uint64_t)a.kv_heads * 3, sc.tpitch, (uint64_t)kPtD * sc.tpitch, kPtD, 1))
+  if (!make_map(&qmap, sc.qp, DP, rows, planes, DP, rows * DP, kPtRows, 1) ||
+      !make_map(&kmap, sc.kp, DP, a.tokens, planes, DP, (uint64_t)a.tokens * DP, kPtKeys, 1) ||
+      !make_map(&vmap, sc.vt, sc.tpitch, DP, planes, sc.tpitch, DP * sc.tpitch, kPtD, 1))
     return cudaErrorInvalidValue;
   static std::atomic<bool> allowed[64];
-  cudaError_t e = allow_smem(prompt_tc_kernel, allowed);
+  cudaError_t e = allow_smem(prompt_tc_kernel<DC>, allowed);
   if (e != cudaSuccess) return e;
-  e = launch_k(prompt_pack_kernel, dim3(sc.pack_blocks, 4), dim3(kPackThreads), 0, stream, a, sc);
+  e = launch_k(prompt_pack_kernel<DC>, dim3(sc.pack_blocks, 4), dim3(kPackThreads), 0, stream, a, sc);
   if (e != cudaSuccess) return e;
-  return launch_k(prompt_tc_kernel, dim3(blocks), dim3(kPtThreads), kPtSmem, stream, a, sc, qmap, kmap, vmap,
-                  device_fault_word());
+  return launch_k(prompt_tc_kernel<DC>, dim3(blocks), dim3(kPtThreads), PtLayout<DC>::kSmem, stream, a, sc, qmap, kmap,
+                  vmap, device_fault_word());
+}
+
+}  // namespace
+
+cudaError_t launch_prompt_tc(const IrisPromptAttention& a, const PromptTcScratch& sc, uint32_t blocks,
+                             cudaStream_t stream) {
+  return a.head_dim <= kPtD ? launch<1>(a, sc, blocks, stream) : launch<2>(a, sc, blocks, stream);
 }
 
 }  // namespace iris

@@ -19,8 +19,7 @@ struct PromptTcScratch {
   uint32_t pitch;
 };
 
-// head_dim 128, requests of at most 16,256 rows (the int32 diagonals, and the
-// places on the near list).
+// Requests of at most 16,256 rows (the int32 diagonals, and the places on the near list).
 bool prompt_tc_usable(const IrisPromptAttention& a);
 size_t prompt_tc_carve(const IrisPromptAttention& a, uint8_t* base, PromptTcScratch* sc);
 // Packs the operands and runs the attention unless a value is past 24 bits

@@ -309,6 +309,10 @@ template <uint32_t NT>
 __global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
   extern __shared__ __align__(16) uint8_t tree_sm[];
   __shared__ ValueShared s;
+  if (sc.flags) {
+    pdl_wait();
+    if (!sc.flags[1]) return;  // the tensor-core launch did the work
+  }
   const uint32_t dts = a.head_dim / 16, tile = 8 * NT * (dts <= 8 ? 2 : 1);  // rows
   const uint32_t groups = (a.nodes * (a.heads / a.kv_heads) + tile - 1) / tile;
   const uint32_t chunk = blockIdx.x, g = blockIdx.y / groups, f0 = blockIdx.y % groups * tile, r = blockIdx.z;
@@ -327,8 +331,7 @@ __global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeA
     row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
   }
   if (tid == 0) s.wide = 0;
-  pdl_wait();
-  if (sc.flags && !sc.flags[1]) return;  // the tensor-core launch did the work
+  if (!sc.flags) pdl_wait();
   for (uint32_t i = warp; i < tile; i += kValueWarps) {
     const uint32_t f = f0 + i;
     uint64_t sum = 0;
@@ -401,7 +404,8 @@ uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   const size_t rows = (size_t)a.rows * a.heads;
   sc->chunk = keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 2 * 148);
-  if (tree_tc_usable(a) && sc->chunk < 128) sc->chunk = 128;  // whole key tiles of the tensor-core launch
+  if (tree_tc_usable(a))  // whole key tiles of the tensor-core launch, a block a multiprocessor
+    sc->chunk = std::max(128u, keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 2048, 3 * 148));
   sc->chunks = ceil_div(a.longest, sc->chunk);
   sc->groups = ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
   sc->vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->groups, a.longest, 4096, 2 * 148);
@@ -423,10 +427,12 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   sc->done = (uint32_t*)take((size_t)a.requests * a.kv_heads * sc->groups * 4);
   sc->flags = nullptr;
   if (tree_tc_usable(a)) {
+    sc->vchunk = 4096;  // (behind the tensor-core launch: few blocks to find that it did the work)
+    sc->vchunks = ceil_div(a.longest, sc->vchunk);
     const uint32_t rows_most = a.nodes * (a.heads / a.kv_heads);
     sc->tc_rows = rows_most <= 64 ? 64 : 128;
     sc->tc_groups = ceil_div(rows_most, sc->tc_rows);
-    sc->tc_vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->tc_groups, a.longest, 4096, 4 * 148);
+    sc->tc_vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->tc_groups, a.longest, 4096, 3 * 148);
     if (sc->tc_vchunk < 128) sc->tc_vchunk = 128;
     sc->tc_vchunks = ceil_div(a.longest, sc->tc_vchunk);
     sc->tc_acc = (int64_t*)take(rows * a.head_dim * 8);

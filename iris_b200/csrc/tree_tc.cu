@@ -1,5 +1,5 @@
-// Drafted trees on the tcgen05 tensor cores (kind::i8), head_dim 128: the first
-// and third launches of tree_mma.cu with their contractions on the
+// Drafted trees on the tcgen05 tensor cores (kind::i8), head_dim up to 128
+// (narrower heads padded with zeros in shared memory): the first and third launches of tree_mma.cu with their contractions on the
 // fifth-generation tensor cores.
 //
 // Keys and values are read where they lie in their pages, once: sixteen warps
@@ -78,10 +78,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const TreeRequest q(a, r);
   const uint32_t rows_all = q.nodes * q.group, key0 = q.base + chunk * sc.chunk;
   if (chunk == 0 && f0 == 0) {  // the totals of this request and head start at zero
-    for (uint32_t i = tid; i < rows_all * kTtD; i += kTtThreads) {
-      const uint32_t f = i / kTtD, x = i % kTtD;
+    for (uint32_t i = tid; i < rows_all * a.head_dim; i += kTtThreads) {
+      const uint32_t f = i / a.head_dim, x = i % a.head_dim;
       const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-      sc.acc[id * kTtD + x] = sc.tc_acc[id * kTtD + x] = 0;
+      sc.acc[id * a.head_dim + x] = sc.tc_acc[id * a.head_dim + x] = 0;
       if (x == 0) sc.wsum[id] = sc.tc_wsum[id] = 0;
     }
     for (uint32_t i = tid; i < sc.groups; i += kTtThreads) sc.done[((size_t)r * a.kv_heads + g) * sc.groups + i] = 0;
@@ -92,7 +92,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const uint32_t rows = min(kTtRows, rows_all - f0), rts = (rows + kTtTile - 1) / kTtTile;
   const uint32_t count = min(sc.chunk, q.keys - key0), kts = (count + kTtKeys - 1) / kTtKeys;
   const int32_t* table = a.table + (size_t)r * a.width;
-  const size_t kvd = (size_t)a.kv_heads * kTtD;
+  const size_t kvd = (size_t)a.kv_heads * a.head_dim;
+  const bool used = 4 * lane < a.head_dim;  // the lane's four dims
+  const int4 none = make_int4(0, 0, 0, 0);
 
   if (tid == 0) {
     mbar_init(&s.ready, 1);
@@ -111,10 +113,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   uint32_t wide = 0;
   // the query rows: a warp a row and turn, four values a lane
+#pragma unroll 4
   for (uint32_t i = warp; i < rts * kTtTile; i += kTtWarps) {
     const uint32_t f = f0 + min(i, rows - 1);
-    const int4 x = *(const int4*)(a.q + (size_t)(q.begin + f / q.group) * a.q_stride +
-                                  (g * q.group + f % q.group) * kTtD + 4 * lane);
+    const int32_t* src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+    const int4 x = used ? *(const int4*)(src + 4 * lane) : none;
     uint32_t p[4];
     split_digits(x.x, x.y, x.z, x.w, p);
     wide |= p[3];
@@ -130,8 +133,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     if (lane < 8) s.seen[kt & 3][warp * 8 + lane] = row >= 0;
     if (row < 0) row = 0;  // hidden keys are masked: any row will do
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-      x[i] = *(const int4*)(a.k_pages + (size_t)__shfl_sync(0xffffffffu, row, i) * kvd + g * kTtD + 4 * lane);
+    for (uint32_t i = 0; i < 8; ++i) {
+      const int32_t* src = a.k_pages + (size_t)__shfl_sync(0xffffffffu, row, i) * kvd + g * a.head_dim;
+      x[i] = used ? *(const int4*)(src + 4 * lane) : none;
+    }
   };
   auto put_keys = [&](uint32_t kt) {
     uint8_t* dst = keys + (kt & 1) * 3 * kTtPlane;
@@ -221,6 +226,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     const uint32_t at = a.window && there && key >= q.held ? (uint32_t)a.positions[q.begin + node] : place;
     int32_t* out = sc.scores + (key - q.base);
     const bool inside = key - q.base < sc.pitch;
+    int32_t best = INT32_MIN;
 #pragma unroll
     for (uint32_t c = 0; c < 16; ++c) {
       const uint32_t i = rt * kTtTile + cg * 16 + c;
@@ -231,8 +237,9 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
       if (inside) out[s.row_at[i]] = y;
       const int32_t m = __reduce_max_sync(0xffffffffu, y);
-      if (lane == 0) atomicMax(&s.top[i], m);
+      best = lane == c ? m : best;
     }
+    if (lane < 16) atomicMax(&s.top[rt * kTtTile + cg * 16 + lane], best);
   }
   if (wide) s.b.wide = 1;
   __syncthreads();
@@ -272,7 +279,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   if (f0 >= rows || key0 >= q.keys) return;
   const uint32_t count = min(sc.tc_vchunk, (q.keys - key0 + 31) / 32 * 32), stages = (count + kTtKeys - 1) / kTtKeys;
   const int32_t* table = a.table + (size_t)r * a.width;
-  const size_t kvd = (size_t)a.kv_heads * kTtD;
+  const size_t kvd = (size_t)a.kv_heads * a.head_dim;
   for (uint32_t i = tid; i < stages * kTtKeys; i += kTtThreads) {
     const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
     row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
@@ -290,7 +297,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const uint32_t dim = (warp & 3) * 32 + lane;
   int32_t x[2][16];
   auto load_values = [&](uint32_t st) {
-    const int32_t* v = a.v_pages + g * kTtD + dim;
+    const int32_t* v = a.v_pages + g * a.head_dim + (dim < a.head_dim ? dim : 0);  // (dims past the head's are not stored)
 #pragma unroll
     for (uint32_t u = 0; u < 2; ++u) {
       const uint4* row = (const uint4*)(row_s + st * kTtKeys + ((warp >> 2) + 4 * u) * 16);
@@ -306,6 +313,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   };
   load_values(0);
   pdl_wait();
+#pragma unroll 4
   for (uint32_t i = warp; i < RB; i += kTtWarps) {
     const uint32_t f = f0 + i;
     uint64_t sum = 0;
@@ -431,8 +439,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       for (uint32_t c = 0; c < 8; ++c) {
         const uint32_t id = s.id[cg * (RB / 4) + c0 + c];
         const int32_t y[4] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c]};
-        if (id != UINT32_MAX)
-          atomicAdd((unsigned long long*)(sc.tc_acc + (size_t)id * kTtD + 32 * quad + lane),
+        if (id != UINT32_MAX && 32 * quad + lane < a.head_dim)
+          atomicAdd((unsigned long long*)(sc.tc_acc + (size_t)id * a.head_dim + 32 * quad + lane),
                     (unsigned long long)diagonal_sum(y));
       }
     }
@@ -460,11 +468,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       const size_t id = s.id[i];
       const int64_t row = first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
       const int32_t top = sub_sat(kOneAct, __ldcg(sc.tc_wsum + id));
-      int32_t* out = a.out + (size_t)(q.begin + node) * a.out_stride + head * kTtD;
-#pragma unroll
-      for (uint32_t y = lane; y < kTtD; y += 32) {
-        int64_t sum = __ldcg(sc.tc_acc + id * kTtD + y);
-        if (row >= 0) mac_wide(sum, top, a.v_pages[(size_t)row * kvd + g * kTtD + y]);
+      int32_t* out = a.out + (size_t)(q.begin + node) * a.out_stride + head * a.head_dim;
+      for (uint32_t y = lane; y < a.head_dim; y += 32) {
+        int64_t sum = __ldcg(sc.tc_acc + id * a.head_dim + y);
+        if (row >= 0) mac_wide(sum, top, a.v_pages[(size_t)row * kvd + g * a.head_dim + y]);
         out[y] = row >= 0 ? requantize(sum) : 0;
       }
     }
@@ -489,7 +496,7 @@ cudaError_t launch_values(const IrisTreeAttention& a, const TreeScratch& sc, cud
 // From two dozen query rows of a K/V head on (fewer leave the 64-row products
 // idle, and the empty launches behind cost more than they save).
 bool tree_tc_usable(const IrisTreeAttention& a) {
-  return a.head_dim == kTtD && a.nodes * (a.heads / a.kv_heads) >= 24 && a.longest >= 512 &&
+  return a.head_dim <= kTtD && a.nodes * (a.heads / a.kv_heads) >= 24 && a.longest >= 512 &&
          device_fault_word() != nullptr;
 }
 

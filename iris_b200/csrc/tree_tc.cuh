@@ -54,7 +54,7 @@ struct TreeRequest {
   }
 };
 
-// head_dim 128 and trees of enough rows.
+// head_dim up to 128 and trees of enough rows.
 bool tree_tc_usable(const IrisTreeAttention& a);
 // The scores and the value sums; flags are cleared before, terms run between.
 cudaError_t launch_tree_tc_scores(const IrisTreeAttention& a, const TreeScratch& sc, cudaStream_t stream);

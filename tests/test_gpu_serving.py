@@ -74,6 +74,14 @@ PROMPTS = [
     ([270], 2, 1, 128, True, 0, "wide"),
     ([270, 5], 2, 1, 128, False, 0, "full"),
     ([900], 1, 1, 128, True, 0, "equal"),
+    ([300, 33, 1], 2, 1, 256, False, 0, "model"),
+    ([280, 100], 3, 1, 256, False, 60, "model"),
+    ([260], 2, 2, 256, False, 0, "wide"),
+    ([258], 2, 1, 256, True, 0, "full"),
+    ([310, 7], 4, 1, 64, False, 0, "model"),
+    ([256, 31], 4, 2, 96, True, 70, "model"),
+    ([300], 2, 1, 160, True, 0, "model"),
+    ([270], 8, 1, 32, True, 0, "model"),
 ]
 
 
@@ -91,7 +99,8 @@ def test_prompt_attention_equals_the_definition(S, lengths, heads, kv_heads, d, 
     assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, scale, window))
 
 
-@pytest.mark.parametrize("heads,kv_heads,d,step", [(4, 1, 128, 61), (2, 2, 64, 61), (2, 1, 36, 61), (4, 2, 128, 1)])
+@pytest.mark.parametrize("heads,kv_heads,d,step", [(4, 1, 128, 61), (2, 2, 64, 61), (2, 1, 36, 61), (4, 2, 128, 1),
+                                                   (2, 1, 256, 61)])
 def test_scores_at_the_lowest_value(S, heads, kv_heads, d, step):
     """Every score within 16.0 of the lowest one, or saturated at it: what a row
     does not see must not be told by a low score."""
@@ -218,6 +227,9 @@ TREES = [
     ([530, 64], [9, 30], 4, 1, 128, True, 0, 16, "wide"),
     ([540], [8], 4, 1, 128, False, 0, 16, "full"),
     ([900, 100], [6, 8], 4, 1, 128, True, 0, 64, "equal"),
+    ([700, 20], [12, 30], 4, 2, 64, False, 200, 16, "model"),
+    ([600], [10], 4, 1, 96, True, 0, 16, "model"),
+    ([610, 5], [13, 8], 4, 1, 32, True, 0, 16, "wide"),
 ]
 
 
