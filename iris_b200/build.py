@@ -16,9 +16,9 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libiris_b200.so"
-SOURCES = ["q8.cu", "layers.cu", "model.cu", "tp.cu", "step.cu", "tc.cu", "attn_tc.cu", "paging.cu", "serve_attn.cu", "tree_mma.cu", "prompt_mma.cu", "prompt_tc.cu", "tree_tc.cu"]
+SOURCES = ["q8.cu", "layers.cu", "model.cu", "tp.cu", "step.cu", "tc.cu", "attn_tc.cu", "paging.cu", "serve_attn.cu", "tree_mma.cu", "prompt_mma.cu", "prompt_tc.cu", "tree_tc.cu", "tree_cluster.cu"]
 HEADERS = ["common.cuh", "detnum.cuh", "sha256.cuh", "q8.cuh", "gemv.cuh", "layers.cuh", "synth.cuh", "tp.cuh", "step.cuh", "tc.cuh", "tcgen05.cuh",
-           "serve.cuh", "serve_attn.cuh", "serve_mma.cuh", "tree_mma.cuh", "prompt_mma.cuh", "prompt_tc.cuh", "serve_tc.cuh", "tree_tc.cuh"]
+           "serve.cuh", "serve_attn.cuh", "serve_mma.cuh", "tree_mma.cuh", "prompt_mma.cuh", "prompt_tc.cuh", "serve_tc.cuh", "tree_tc.cuh", "tree_cluster.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
          "--expt-relaxed-constexpr"]

@@ -10,6 +10,7 @@
 #include "prompt_mma.cuh"
 #include "serve.cuh"
 #include "serve_attn.cuh"
+#include "tree_cluster.cuh"
 #include "tree_mma.cuh"
 
 namespace iris {
@@ -219,7 +220,7 @@ int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_
 }
 
 uint64_t iris_tree_attention_workspace(const IrisTreeAttention* a) {
-  if (check_tree(a) || !a->rows || !tree_mma_usable(*a)) return 0;
+  if (check_tree(a) || !a->rows || !tree_mma_usable(*a) || tree_cluster_usable(*a)) return 0;
   return tree_mma_workspace(*a);
 }
 
@@ -228,6 +229,7 @@ int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t wo
   if (bad || !a->rows) return bad;
   const uint64_t need = iris_tree_attention_workspace(a);
   if (need && (!aligned16(workspace) || workspace_bytes < need)) return IRIS_ESCRATCH;
+  if (tree_mma_usable(*a) && tree_cluster_usable(*a)) return (int)launch_tree_cluster(*a, (cudaStream_t)stream);
   if (tree_mma_usable(*a)) return (int)launch_tree_mma(*a, (uint8_t*)workspace, (cudaStream_t)stream);
   tree_rows_kernel<<<dim3(a->rows, a->heads), kRowThreads, 0, (cudaStream_t)stream>>>(*a);
   return (int)cudaGetLastError();
