@@ -271,9 +271,16 @@ uint32_t row_tiles(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
-// Blocks of a cluster: sixteen while the clusters leave multiprocessors free.
+// Blocks of a cluster: as many as leave two blocks a multiprocessor over all of
+// them (one for more than eight rows, whose registers allow no second), and 32
+// keys a block. Sixteen only for up to eight rows on a free device (of many
+// clusters, or of blocks that want a multiprocessor each, sixteen are seldom free
+// in one place: 33 against 22 us for sixteen requests of 777 keys).
 uint32_t cluster_blocks(const IrisTreeAttention& a) {
-  return (uint64_t)a.requests * a.kv_heads * 16 <= 148 && a.longest > 256 ? 16 : 8;
+  const uint64_t groups = (uint64_t)a.requests * a.kv_heads, room = row_tiles(a) == 1 ? 2 * 148 : 148;
+  uint32_t n = row_tiles(a) == 1 && groups * 16 <= 148 ? 16 : 8;
+  while (n > 1 && (groups * n > room || (n - 1) * 32 >= a.longest)) n /= 2;
+  return n;
 }
 uint32_t block_span(const IrisTreeAttention& a) {
   const uint32_t n = cluster_blocks(a), each = (a.longest + n - 1) / n;
@@ -313,11 +320,19 @@ cudaError_t launch(const IrisTreeAttention& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Few rows, a span that fits a block, and no more clusters than run at once.
+// Few rows, and a span whose pairs fit a block and keep it no longer than the
+// three launches of tree_mma.cu take: up to 1,024 keys for eight rows (fewer for
+// more), half as many again where the blocks fill the device. Measured, us, here
+// against there (32 query heads, 8 K/V heads of 128): one node over 777 keys 14.8
+// / 22.1, over 12,000 60 / 79, over 30,000 242 / 136; four requests over 12,000
+// 120 / 227; eight nodes over 777 keys 24.5 / 39.1, over 4,000 67 / 57.
 bool tree_cluster_usable(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
-  return rows <= kClusterRows && (uint64_t)row_tiles(a) * 8 * block_span(a) <= kClusterPairs &&
-         (uint64_t)a.requests * a.kv_heads * cluster_blocks(a) <= 4 * 148;
+  if (rows > kClusterRows) return false;
+  const uint32_t tiles = row_tiles(a), span = block_span(a);
+  const uint64_t blocks = (uint64_t)a.requests * a.kv_heads * cluster_blocks(a);
+  return (uint64_t)tiles * 8 * span <= kClusterPairs &&
+         (tiles * span <= 1024 && (span <= 512 || blocks >= 64) || (tiles <= 2 && blocks >= 128 && span <= 1536));
 }
 
 cudaError_t launch_tree_cluster(const IrisTreeAttention& a, cudaStream_t stream) {

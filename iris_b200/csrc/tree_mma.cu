@@ -30,7 +30,6 @@ namespace iris {
 namespace {
 
 constexpr uint32_t kTreeThreads = 256, kTreeWarps = kTreeThreads / 32;
-constexpr uint32_t kTreeTile = 32;     // query rows a block works on at a time
 __device__ __forceinline__ bool is_visible(const IrisTreeAttention& a, const TreeRequest& q, uint32_t node,
                                            uint32_t key) {
   const uint32_t row = q.begin + node;
@@ -38,8 +37,11 @@ __device__ __forceinline__ bool is_visible(const IrisTreeAttention& a, const Tre
                    a.positions ? (uint32_t)a.positions[row] : 0, a.positions + q.begin);
 }
 
-__global__ void __launch_bounds__(kTreeThreads, 2) tree_scores_kernel(IrisTreeAttention a, TreeScratch sc) {
-  constexpr uint32_t NT = kTreeTile / 8;
+// 8 NT query rows at a time; with few rows more blocks share a multiprocessor,
+// for their loads in flight.
+template <uint32_t NT>
+__global__ void __launch_bounds__(kTreeThreads, NT == 1 ? 4 : 2) tree_scores_kernel(IrisTreeAttention a, TreeScratch sc) {
+  constexpr uint32_t kTreeTile = 8 * NT;
   extern __shared__ __align__(16) uint8_t tree_sm[];
   uint2* frag = (uint2*)tree_sm;  // [tile / 8][steps][4][32]
   __shared__ __align__(16) uint64_t row_at[kTreeTile];  // the rows' scores
@@ -306,7 +308,7 @@ __device__ __noinline__ bool tree_chunk_values(const IrisTreeAttention& a, const
 }
 
 template <uint32_t NT>
-__global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
+__global__ void __launch_bounds__(kValueThreads, NT == 1 ? 2 : 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
   extern __shared__ __align__(16) uint8_t tree_sm[];
   __shared__ ValueShared s;
   if (sc.flags) {
@@ -399,6 +401,11 @@ uint32_t value_tiles(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads), halves = a.head_dim <= 128 ? 2 : 1;
   return rows <= 8 * halves ? 1 : rows <= 16 * halves ? 2 : 4;
 }
+// Row tiles of the first launch's blocks.
+uint32_t score_tiles(const IrisTreeAttention& a) {
+  const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
+  return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
 uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a.head_dim <= 128 ? 2 : 1); }
 
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
@@ -443,7 +450,7 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   return at;
 }
 
-constexpr uint32_t score_smem(uint32_t d) { return kTreeTile / 8 * (d / 32) * 4 * 256; }
+uint32_t score_smem(const IrisTreeAttention& a) { return score_tiles(a) * (a.head_dim / 32) * 4 * 256; }
 constexpr uint32_t value_smem(uint32_t d, uint32_t vchunk, uint32_t rows) {
   return vchunk * 4 + 4 * (d / 16) * 4 * 512 + 4 * (rows / 8) * 512;
 }
@@ -478,11 +485,15 @@ cudaError_t launch_tree_mma(const IrisTreeAttention& a, uint8_t* workspace, cuda
     e = cudaMemsetAsync(sc.flags, 0, 8, stream);
     if (e == cudaSuccess) e = launch_tree_tc_scores(a, sc, stream);
     if (e != cudaSuccess) return e;
-    e = launch_k(tree_scores_kernel, dim3(sc.chunks, a.kv_heads, a.requests), dim3(kTreeThreads),
-                 score_smem(a.head_dim), stream, a, sc);
+    e = launch_k(tree_scores_kernel<4>, dim3(sc.chunks, a.kv_heads, a.requests), dim3(kTreeThreads), score_smem(a),
+                 stream, a, sc);
   } else {
-    tree_scores_kernel<<<dim3(sc.chunks, a.kv_heads, a.requests), kTreeThreads, score_smem(a.head_dim), stream>>>(a,
-                                                                                                              sc);
+    const dim3 grid(sc.chunks, a.kv_heads, a.requests);
+    switch (score_tiles(a)) {
+      case 1: tree_scores_kernel<1><<<grid, kTreeThreads, score_smem(a), stream>>>(a, sc); break;
+      case 2: tree_scores_kernel<2><<<grid, kTreeThreads, score_smem(a), stream>>>(a, sc); break;
+      default: tree_scores_kernel<4><<<grid, kTreeThreads, score_smem(a), stream>>>(a, sc); break;
+    }
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return e;

@@ -261,6 +261,19 @@ def test_masks_that_leave_rows_empty_and_tables_with_holes(S, d):
     assert not got[1].any()
 
 
+@pytest.mark.parametrize("requests,nodes,most,heads,kv_heads,d,window", [
+    (24, 1, 90, 8, 8, 64, 0), (9, 1, 300, 4, 4, 128, 0), (5, 2, 700, 16, 4, 128, 40), (3, 4, 500, 8, 1, 32, 0),
+    (2, 1, 1500, 4, 1, 256, 0), (40, 3, 50, 4, 2, 64, 0), (1, 1, 2600, 2, 1, 128, 0)])
+def test_tree_attention_of_few_rows(S, requests, nodes, most, heads, kv_heads, d, window):
+    """Plain decoding and small drafts of one to many requests."""
+    rng = np.random.default_rng(requests * 7 + d)
+    held = [most] + [int(rng.integers(0, most + 1)) for _ in range(requests - 1)]
+    sizes = [nodes] + [int(rng.integers(0, nodes + 1)) for _ in range(requests - 1)]
+    for kind in ("model", "wide" if requests < 10 else "full"):
+        x = tree_inputs(rng, held, sizes, heads, kv_heads, d, 16, kind, holes=[(0, 1, -1)] if most > 40 else ())
+        check_tree(S, x, heads, kv_heads, scale_of(d), window, sizes)
+
+
 def test_tree_attention_of_a_long_context(S):
     rng = np.random.default_rng(21)
     held, nodes, heads, kv_heads, d = [20000, 9000], [3, 2], 2, 1, 128
