@@ -576,6 +576,18 @@ IRIS_HD int32_t softmax_weight_inv(int64_t term, uint64_t sum, uint64_t inv) {
   return requantize((int64_t)q);
 }
 
+// Whether softmax_weight(term, sum) is c or more (1 <= c <= 65536), without a
+// division: the weight is c or more where the quotient rounded to Q32.32 is
+// above c 2^16 - 2^15, or that itself and c even, and such a quotient n / sum (n =
+// term 2^32) is where 2 n >= (2 (c 2^16 - 2^15) - 1) sum for even c, and for odd
+// c where 2 n > (2 (c 2^16 - 2^15) + 1) sum (halves go to the even neighbour).
+IRIS_HD bool softmax_weight_reaches(int64_t term, uint64_t sum, uint32_t c) {
+  const uint64_t m = ((uint64_t)c << 17) - (1u << 16) + (c & 1 ? 1 : -1);
+  const uint64_t hi = mulhi_u64(m, sum), lo = m * sum, n_hi = (uint64_t)term >> 31, n_lo = (uint64_t)term << 33;
+  if (n_hi != hi) return n_hi > hi;
+  return c & 1 ? n_lo > lo : n_lo >= lo;
+}
+
 // ---- gemma-dense functions (ops.rs) -----------------------------------------
 
 // ops.rs:357-377 tanh_act

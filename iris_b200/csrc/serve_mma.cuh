@@ -296,12 +296,8 @@ __device__ __forceinline__ RowTerms row_terms(int32_t* row, uint32_t block, uint
   return out;
 }
 
-// A row's divisor: its exact sum and floor(2^63 / sum) (at most 2^31: the
-// maximum's own term makes the sum at least 2^32); 0 where nothing is seen.
-struct RowSum {
-  uint64_t sum;
-  uint32_t recip;
-};
+// A row's divisor: floor(2^63 / sum) (at most 2^31: the maximum's own term makes
+// the sum at least 2^32); 0 where nothing is seen.
 __device__ __forceinline__ uint32_t sum_recip(uint64_t sum) { return sum ? (uint32_t)(((uint64_t)1 << 63) / sum) : 0; }
 
 // The weight of a term (attention_softmax_raw_weight, ops.rs:269-271:
@@ -310,31 +306,22 @@ __device__ __forceinline__ uint32_t sum_recip(uint64_t sum) { return sum ? (uint
 // floors takes less than 1, the kept top term less than 1/2), and rounding the
 // quotient first moves v by at most 1/4: so the weight is (y + 2^14) >> 15
 // unless a multiple of 2^15 lies within 1/4 below or 2.75 above y + 2^14;
-// there (4 values of 32768) the exact division decides.
-static __device__ __noinline__ int32_t exact_weight(uint32_t term, uint64_t sum) {
-  return softmax_weight((int64_t)kept_term(term), sum);
-}
-// Eight weights of one row: the doubtful ones found together.
+// there (4 values of 32768) the two sides of that multiple are told apart
+// exactly. Eight weights of one row, the doubtful ones found together.
 __device__ __forceinline__ void weights_of(const uint32_t (&term)[8], uint32_t recip, uint64_t sum, int32_t (&w)[8]) {
-  uint32_t y[8], least = 0x7FFF;
+  uint32_t least = 0x7FFF;
 #pragma unroll
   for (uint32_t j = 0; j < 8; ++j) {
-    y[j] = __umulhi(term[j], recip) + (1u << 14);
-    least = min(least, (y[j] + 3) & 0x7FFF);
-    w[j] = (int32_t)(y[j] >> 15);
+    const uint32_t y = __umulhi(term[j], recip) + (1u << 14);
+    least = min(least, (y + 3) & 0x7FFF);
+    w[j] = (int32_t)(y >> 15);
   }
-  if (least <= 3 && recip) {
-#pragma unroll 1
+  if (least <= 3) {
+#pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
-      uint32_t t = 0, z = 0;
-#pragma unroll
-      for (uint32_t o = 0; o < 8; ++o)
-        if (o == j) t = term[o], z = y[o];
-      if (((z + 3) & 0x7FFF) > 3) continue;
-      const int32_t exact = exact_weight(t, sum);
-#pragma unroll
-      for (uint32_t o = 0; o < 8; ++o)
-        if (o == j) w[o] = exact;
+      const uint32_t y = __umulhi(term[j], recip) + (1u << 14) + 3;
+      if ((y & 0x7FFF) <= 3)
+        w[j] = (int32_t)(y >> 15) - !softmax_weight_reaches((int64_t)kept_term(term[j]), sum, y >> 15);
     }
   }
 }
@@ -430,6 +417,5 @@ __device__ __forceinline__ int64_t diagonal_sum(const int32_t (&v)[ND]) {
 #pragma unroll
   for (uint32_t d = 0; d < ND; ++d) s += (int64_t)v[d] << (8 * d);
   return s;
-}
 
 }  // namespace iris

@@ -16,5 +16,13 @@ void serving_exp_terms(uint32_t* term, uint32_t* estimate, uint8_t* doubt, uint3
     want[d] = iris::softmax_exp_term_act(-(int32_t)d, 0);
   }
 }
+// The weights of n terms, by division and as the step (1 to 65536) that is reached and whose successor is not.
+void serving_weights(const int64_t* term, const uint64_t* sum, uint64_t n, int32_t* want, uint8_t* agrees) {
+  for (uint64_t i = 0; i < n; ++i) {
+    const int32_t w = want[i] = iris::softmax_weight(term[i], sum[i]);
+    agrees[i] = (w == 0 || iris::softmax_weight_reaches(term[i], sum[i], w)) &&
+                (w == 65536 || !iris::softmax_weight_reaches(term[i], sum[i], w + 1));
+  }
+}
 uint32_t serving_exact_below() { return iris::kExpExactBelow; }
 }
