@@ -417,5 +417,45 @@ __device__ __forceinline__ int64_t diagonal_sum(const int32_t (&v)[ND]) {
 #pragma unroll
   for (uint32_t d = 0; d < ND; ++d) s += (int64_t)v[d] << (8 * d);
   return s;
+}
+
+// One warp's 16 dimensions over the 32-key steps first, first + by, .. < steps,
+// values straight from their pages (v: the lane's two dimensions; row_s: the
+// keys' pool rows; w: the steps' weights): emit(row, dimension of the 16, sum) for
+// 8 NT rows. Returns whether a value was past 24 bits (P = 3: nothing was
+// emitted then).
+template <uint32_t P, uint32_t NT, class Emit>
+__device__ __forceinline__ bool paged_value_sums(const int32_t* v, size_t kvd, const uint32_t* row_s, const uint2* w,
+                                                 uint32_t first, uint32_t by, uint32_t steps, uint32_t lane,
+                                                 const Emit& emit) {
+  int32_t acc[NT][P + 1][4] = {};
+  int2 x[8], y[8];
+  auto load = [&](int2 (&z)[8], uint32_t st) {
+    const uint32_t* row = row_s + st * 32 + 4 * (lane & 3);
+    const uint4 lo = *(const uint4*)row, hi = *(const uint4*)(row + 16);
+    const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) z[i] = *(const int2*)(v + (size_t)r[i] * kvd);
+  };
+  uint32_t wide = 0;
+  if (first < steps) load(x, first);
+  for (uint32_t st = first; st < steps; st += by) {
+    if (st + by < steps) load(y, st + by);
+    wide |= value_products<P, NT>(x, w + (size_t)st * NT * 64, lane, acc);
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) x[i] = y[i];
+  }
+  if (P == 3 && __any_sync(0xffffffffu, wide != 0)) return true;
+#pragma unroll
+  for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+      int32_t d[P + 1];
+#pragma unroll
+      for (uint32_t j = 0; j < P + 1; ++j) d[j] = acc[n][j][e];
+      emit(8 * n + 2 * (lane & 3) + (e & 1), 2 * (lane >> 2) + (e >> 1), diagonal_sum(d));
+    }
+  return false;
+}
 
 }  // namespace iris

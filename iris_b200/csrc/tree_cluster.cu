@@ -41,41 +41,13 @@ struct ClusterShared {
   uint32_t q_wide;
 };
 
-// This warp's 16 dimensions over the block's keys: sums of 8 NT rows into `sums`
-// [row][d]; whether a value was past 24 bits (P = 3: nothing was written then).
+// cluster sums [row][d] of a warp's 16 dimensions.
 template <uint32_t P, uint32_t NT>
 __device__ __noinline__ bool cluster_values(const IrisTreeAttention& a, const uint32_t* row_s, const uint2* w,
                                             uint32_t steps, uint32_t g, uint32_t dt, int64_t* sums, uint32_t lane) {
-  int32_t acc[NT][P + 1][4] = {};
   const int32_t* v = a.v_pages + g * a.head_dim + 16 * dt + 2 * (lane >> 2);
-  const size_t kvd = (size_t)a.kv_heads * a.head_dim;
-  int2 x[8], y[8];
-  auto load = [&](int2 (&z)[8], uint32_t st) {
-    const uint32_t* row = row_s + st * 32 + 4 * (lane & 3);
-    const uint4 lo = *(const uint4*)row, hi = *(const uint4*)(row + 16);
-    const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) z[i] = *(const int2*)(v + (size_t)r[i] * kvd);
-  };
-  uint32_t wide = 0;
-  load(x, 0);
-  for (uint32_t st = 0; st < steps; ++st) {
-    if (st + 1 < steps) load(y, st + 1);
-    wide |= value_products<P, NT>(x, w + (size_t)st * NT * 64, lane, acc);
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) x[i] = y[i];
-  }
-  if (P == 3 && __any_sync(0xffffffffu, wide != 0)) return true;
-#pragma unroll
-  for (uint32_t n = 0; n < NT; ++n)
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-      int32_t d[P + 1];
-#pragma unroll
-      for (uint32_t j = 0; j < P + 1; ++j) d[j] = acc[n][j][e];
-      sums[(8 * n + 2 * (lane & 3) + (e & 1)) * a.head_dim + 16 * dt + 2 * (lane >> 2) + (e >> 1)] = diagonal_sum(d);
-    }
-  return false;
+  return paged_value_sums<P, NT>(v, (size_t)a.kv_heads * a.head_dim, row_s, w, 0, 1, steps, lane,
+                                 [&](uint32_t row, uint32_t x, int64_t sum) { sums[row * a.head_dim + 16 * dt + x] = sum; });
 }
 
 template <uint32_t NT>

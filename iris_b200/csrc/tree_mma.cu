@@ -189,6 +189,29 @@ __global__ void __launch_bounds__(kTreeThreads) tree_terms_kernel(IrisTreeAttent
   }
 }
 
+// Rows f0 .. f0 + n - 1 of a request and K/V head: the totals, the first maximum's
+// value times what the other weights leave of 1.0, rounded once. Rows that saw
+// nothing give zeros.
+__device__ __forceinline__ void finish_rows(const IrisTreeAttention& a, const int64_t* acc, const int32_t* wsum,
+                                            const TreeRequest& q, const int32_t* table, uint32_t g, uint32_t f0,
+                                            uint32_t n, const uint32_t* ids, const uint32_t* firsts, uint32_t warp,
+                                            uint32_t warps, uint32_t lane) {
+  const size_t kvd = (size_t)a.kv_heads * a.head_dim;
+  for (uint32_t i = warp; i < n; i += warps) {
+    const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group, first = firsts[i];
+    const size_t id = ids[i];
+    const int64_t row =
+        first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
+    const int32_t top = sub_sat(kOneAct, __ldcg(wsum + id));
+    int32_t* out = a.out + (size_t)(q.begin + node) * a.out_stride + head * a.head_dim;
+    for (uint32_t x = lane; x < a.head_dim; x += 32) {
+      int64_t sum = __ldcg(acc + id * a.head_dim + x);
+      if (row >= 0) mac_wide(sum, top, a.v_pages[(size_t)row * kvd + g * a.head_dim + x]);
+      out[x] = row >= 0 ? requantize(sum) : 0;
+    }
+  }
+}
+
 // Values: a block takes up to 16 NT rows (8 NT for heads past 128 values) of one
 // request and K/V head, and a chunk of its keys in stages of 64: the stage's
 // values as byte-plane fragments and its weights go to shared memory, made once
@@ -308,7 +331,7 @@ __device__ __noinline__ bool tree_chunk_values(const IrisTreeAttention& a, const
 }
 
 template <uint32_t NT>
-__global__ void __launch_bounds__(kValueThreads, NT == 1 ? 2 : 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
+__global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeAttention a, TreeScratch sc) {
   extern __shared__ __align__(16) uint8_t tree_sm[];
   __shared__ ValueShared s;
   if (sc.flags) {
@@ -368,20 +391,106 @@ __global__ void __launch_bounds__(kValueThreads, NT == 1 ? 2 : 1) tree_values_ke
   }
   __syncthreads();
   if (!s.last) return;
-  const size_t kvd = (size_t)a.kv_heads * a.head_dim;
-  for (uint32_t i = warp; i < min(tile, rows - f0); i += kValueWarps) {
-    const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group;
-    const size_t id = s.id[i];
-    const uint32_t first = s.first[i];
-    const int64_t row = first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
-    const int32_t top = sub_sat(kOneAct, __ldcg(sc.wsum + id));
-    int32_t* out = a.out + (size_t)(q.begin + node) * a.out_stride + head * a.head_dim;
-    for (uint32_t x = lane; x < a.head_dim; x += 32) {
-      int64_t sum = __ldcg(sc.acc + id * a.head_dim + x);
-      if (row >= 0) mac_wide(sum, top, a.v_pages[(size_t)row * kvd + g * a.head_dim + x]);
-      out[x] = row >= 0 ? requantize(sum) : 0;
+  finish_rows(a, sc.acc, sc.wsum, q, table, g, f0, min(tile, rows - f0), s.id, s.first, warp, kValueWarps, lane);
+}
+
+// Few rows (8 NT at most): values straight from their pages into the products, a
+// chunk of keys a block of eight warps, so that several blocks a multiprocessor
+// keep loads in flight: bound by reading the values.
+template <uint32_t P, uint32_t NT>
+__device__ __noinline__ bool few_values(const IrisTreeAttention& a, const TreeScratch& sc, const uint32_t* row_s,
+                                        const uint2* w, const uint32_t* id_s, uint32_t part, uint32_t shares,
+                                        uint32_t steps, uint32_t g, uint32_t dt, uint32_t lane) {
+  const int32_t* v = a.v_pages + g * a.head_dim + 16 * dt + 2 * (lane >> 2);
+  return paged_value_sums<P, NT>(v, (size_t)a.kv_heads * a.head_dim, row_s, w, part, shares, steps, lane,
+                                 [&](uint32_t row, uint32_t x, int64_t sum) {
+                                   if (id_s[row] != UINT32_MAX)
+                                     atomicAdd((unsigned long long*)(sc.acc + (size_t)id_s[row] * a.head_dim + 16 * dt + x),
+                                               (unsigned long long)sum);
+                                 });
+}
+
+template <uint32_t NT>
+__global__ void __launch_bounds__(kTreeThreads, 2)
+    tree_few_values_kernel(IrisTreeAttention a, TreeScratch sc) {
+  constexpr uint32_t R = 8 * NT;
+  extern __shared__ __align__(16) uint8_t tree_sm[];
+  uint32_t* row_s = (uint32_t*)tree_sm;         // [vchunk] pool rows
+  uint2* wts = (uint2*)(row_s + sc.vchunk);     // [vchunk / 32][NT][2][32]
+  __shared__ uint64_t sum_s[R];
+  __shared__ uint32_t recip_s[R], first_s[R], id_s[R], last_s;
+  __shared__ int32_t wsum_s[R];
+  const uint32_t chunk = blockIdx.x, g = blockIdx.y, r = blockIdx.z;
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const TreeRequest q(a, r);
+  const uint32_t rows = q.nodes * q.group, s0 = chunk * sc.vchunk, key0 = q.base + s0;
+  const uint32_t chunks = (q.count + sc.vchunk - 1) / sc.vchunk, segs = (q.count + kTreeSegment - 1) / kTreeSegment;
+  if (!rows || key0 >= q.keys) return;
+  const uint32_t count = min(sc.vchunk, (q.keys - key0 + 31) / 32 * 32), steps = count / 32;
+  const int32_t* table = a.table + (size_t)r * a.width;
+  for (uint32_t i = tid; i < count; i += kTreeThreads) {
+    const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
+    row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
+  }
+  if (tid < R) wsum_s[tid] = 0;
+  pdl_wait();
+#pragma unroll
+  for (uint32_t i = warp; i < R; i += kTreeWarps) {
+    uint64_t sum = 0;
+    uint32_t first = UINT32_MAX, id = UINT32_MAX;
+    if (i < rows) {
+      id = (q.begin + i / q.group) * a.heads + g * q.group + i % q.group;
+      for (uint32_t x = lane; x < segs; x += 32) {
+        sum += sc.seg_sum[(size_t)id * sc.segs + x];
+        first = min(first, sc.seg_first[(size_t)id * sc.segs + x]);
+      }
+      sum = (uint64_t)warp_sum_i64((int64_t)sum);
+      first = __reduce_min_sync(0xffffffffu, first);
+    }
+    if (lane == 0) {
+      sum_s[i] = sum;
+      recip_s[i] = sum_recip(sum);
+      first_s[i] = first;
+      id_s[i] = id;
     }
   }
+  __syncthreads();
+  for (uint32_t u = warp; u < NT * steps; u += kTreeWarps) {
+    const uint32_t n = u % NT, st = u / NT, i = 8 * n + (lane >> 2), at = s0 + st * 32 + 4 * (lane & 3);
+    uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+    if (id_s[i] != UINT32_MAX) {
+      const int32_t* t = sc.scores + (size_t)id_s[i] * sc.pitch + at;
+      lo = __ldcg((const uint4*)t);
+      hi = __ldcg((const uint4*)(t + 16));
+    }
+    const uint32_t e[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    int32_t w[8], all = 0;
+    weights_of(e, recip_s[i], sum_s[i], w);
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) {
+      if (at + (j >> 2) * 16 + (j & 3) == first_s[i]) w[j] = 0;  // its weight comes last
+      all += w[j];
+    }
+    put_weight_fragment(wts + (size_t)(st * NT + n) * 64, lane, w);
+    all += __shfl_xor_sync(0xffffffffu, all, 1);
+    all += __shfl_xor_sync(0xffffffffu, all, 2);
+    if ((lane & 3) == 0 && all) atomicAdd(&wsum_s[i], all);
+  }
+  __syncthreads();
+  const uint32_t dts = a.head_dim / 16, shares = max(1u, kTreeWarps / dts);  // warps a 16-dimension tile
+  for (uint32_t u = warp; u < dts * shares; u += kTreeWarps)
+    if (few_values<3, NT>(a, sc, row_s, wts, id_s, u / dts, shares, steps, g, u % dts, lane))
+      few_values<4, NT>(a, sc, row_s, wts, id_s, u / dts, shares, steps, g, u % dts, lane);
+  if (tid < R && id_s[tid] != UINT32_MAX && wsum_s[tid]) atomicAdd(sc.wsum + id_s[tid], wsum_s[tid]);
+  // the last block of these rows writes the outputs
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    last_s = atom_add_acq_rel(sc.done + (size_t)r * gridDim.y + g, 1u) + 1 == chunks;
+    __threadfence();
+  }
+  __syncthreads();
+  if (last_s) finish_rows(a, sc.acc, sc.wsum, q, table, g, 0, min(R, rows), id_s, first_s, warp, kTreeWarps, lane);
 }
 
 uint32_t ceil_div(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
@@ -395,17 +504,18 @@ uint32_t keys_a_block(uint64_t groups, uint32_t longest, uint32_t most, uint32_t
   return chunk;
 }
 
-// Row tiles a warp of the third launch takes (8 rows each): as few as hold the
-// call's largest tree, so that a few rows do not pay for 64.
+// Row tiles a warp of the third launch takes (8 rows each, two warps a tile of
+// dimensions for up to 128 of them): 32 rows do not pay for 64.
 uint32_t value_tiles(const IrisTreeAttention& a) {
-  const uint32_t rows = a.nodes * (a.heads / a.kv_heads), halves = a.head_dim <= 128 ? 2 : 1;
-  return rows <= 8 * halves ? 1 : rows <= 16 * halves ? 2 : 4;
+  return a.head_dim <= 128 && a.nodes * (a.heads / a.kv_heads) <= 32 ? 2 : 4;
 }
 // Row tiles of the first launch's blocks.
 uint32_t score_tiles(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
+// Up to sixteen rows take their values straight from the pages.
+bool few_rows(const IrisTreeAttention& a) { return a.nodes * (a.heads / a.kv_heads) <= 16; }
 uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a.head_dim <= 128 ? 2 : 1); }
 
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
@@ -414,8 +524,9 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   if (tree_tc_usable(a))  // whole key tiles of the tensor-core launch, a block a multiprocessor
     sc->chunk = std::max(128u, keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 2048, 3 * 148));
   sc->chunks = ceil_div(a.longest, sc->chunk);
-  sc->groups = ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
-  sc->vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->groups, a.longest, 4096, 2 * 148);
+  sc->groups = few_rows(a) ? 1 : ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
+  sc->vchunk = few_rows(a) ? keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 4 * 148)
+                           : keys_a_block((uint64_t)a.requests * a.kv_heads * sc->groups, a.longest, 4096, 2 * 148);
   sc->vchunks = ceil_div(a.longest, sc->vchunk);
   sc->segs = ceil_div(a.longest, kTreeSegment);
   sc->pitch = ceil_div(a.longest, 64) * 64;
@@ -501,13 +612,17 @@ cudaError_t launch_tree_mma(const IrisTreeAttention& a, uint8_t* workspace, cuda
                dim3(kTreeThreads), 0, stream, a, sc);
   if (e == cudaSuccess && sc.flags) e = launch_tree_tc_values(a, sc, stream);
   if (e != cudaSuccess) return e;
+  if (few_rows(a)) {
+    const dim3 few(sc.vchunks, a.kv_heads, a.requests);
+    const uint32_t few_smem = sc.vchunk * 4 + sc.vchunk / 32 * score_tiles(a) * 512;
+    return score_tiles(a) == 1
+               ? launch_k(tree_few_values_kernel<1>, few, dim3(kTreeThreads), few_smem, stream, a, sc)
+               : launch_k(tree_few_values_kernel<2>, few, dim3(kTreeThreads), few_smem, stream, a, sc);
+  }
   const uint32_t smem = value_smem(a.head_dim, sc.vchunk, value_rows(a));
   const dim3 grid(sc.vchunks, a.kv_heads * sc.groups, a.requests);
-  switch (value_tiles(a)) {
-    case 1: return launch_values<1>(a, sc, grid, smem, stream);
-    case 2: return launch_values<2>(a, sc, grid, smem, stream);
-    default: return launch_values<4>(a, sc, grid, smem, stream);
-  }
+  return value_tiles(a) == 2 ? launch_values<2>(a, sc, grid, smem, stream)
+                             : launch_values<4>(a, sc, grid, smem, stream);
 }
 
 }  // namespace iris
