@@ -28,6 +28,7 @@ namespace {
 constexpr uint32_t kPromptThreads = 512, kPromptWarps = kPromptThreads / 32;
 constexpr uint32_t kPromptKeys = 128;  // keys of a weight tile
 constexpr uint32_t kSortRequests = 1024;
+constexpr uint32_t kFewRequests = 32;  // whose tiles a block counts itself, with 148 blocks' worth of tiles at most
 
 struct PromptScratch {
   uint32_t* order;   // [requests]: the requests, longest first
@@ -258,20 +259,42 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
     for (uint32_t i = tid; i < sc.flags; i += kPromptThreads) wide |= sc.wide[i];
     if (!__syncthreads_or(wide != 0)) return;
   }
-  const uint32_t items = sc.tiles[a.requests] * a.kv_heads;
-  for (;;) {
+  // Few requests: every block counts the tiles itself, and takes every so manyth
+  // of them; else the list of prompt_items_kernel, handed out one by one.
+  __shared__ uint32_t few_tiles[kFewRequests + 1];
+  const bool few = sc.order == nullptr;
+  if (few && warp == 0) {
+    uint32_t n = 0;
+    if (lane < a.requests) {
+      const uint32_t b = clamp_offset(a.offsets[lane], a.tokens), e = clamp_offset(a.offsets[lane + 1], a.tokens);
+      n = e > b ? (uint32_t)(((uint64_t)min(e - b, a.longest) * (a.heads / a.kv_heads) + RT - 1) / RT) : 0;
+    }
+    uint32_t incl = n;
+#pragma unroll
+    for (uint32_t d = 1; d < 32; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    few_tiles[lane] = incl - n;
+    if (lane == 31) few_tiles[32] = incl;
+  }
+  __syncthreads();
+  const uint32_t* tiles = few ? few_tiles : sc.tiles;
+  const uint32_t items = (few ? few_tiles[32] : sc.tiles[a.requests]) * a.kv_heads;
+  for (uint32_t mine = blockIdx.x;; mine += gridDim.x) {
     __syncthreads();  // the tile before is done with the shared memory
-    if (tid == 0) s.item = atomicAdd(sc.next, 1u);
+    if (!few && tid == 0) s.item = atomicAdd(sc.next, 1u);
     __syncthreads();
-    const uint32_t item = s.item;
+    const uint32_t item = few ? mine : s.item;
     if (item >= items) return;
     PromptTile p;
     p.g = item % a.kv_heads;
-    const uint32_t at = item / a.kv_heads, rank = request_of(sc.tiles, a.requests, at), r = sc.order[rank];
+    const uint32_t at = item / a.kv_heads, rank = request_of(tiles, few ? 32u : a.requests, at);
+    const uint32_t r = few ? rank : sc.order[rank];
     p.begin = clamp_offset(a.offsets[r], a.tokens);
     p.len = min(clamp_offset(a.offsets[r + 1], a.tokens) - p.begin, a.longest);
     p.group = a.heads / a.kv_heads;
-    p.f0 = (sc.tiles[rank + 1] - 1 - at) * RT;  // a request's last tile, the longest, first
+    p.f0 = (tiles[rank + 1] - 1 - at) * RT;  // a request's last tile, the longest, first
     p.rows = min(RT, p.len * p.group - p.f0);
     const uint32_t q0 = p.f0 / p.group, q1 = (p.f0 + p.rows - 1) / p.group;
     p.base = window_start(q0, a.window) / 16 * 16;
@@ -400,6 +423,15 @@ size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, Pro
     at += up256(bytes);
     return p;
   };
+  // a tile a block: nothing to balance, and no launch for the list
+  if (!on_tensor_cores(a) && a.requests <= kFewRequests && tiles * a.kv_heads <= (uint64_t)device_sms()) {
+    sc->next = sc->order = sc->tiles = nullptr;
+    sc->scores = (int32_t*)take((size_t)sc->blocks * rt * sc->pitch * 4);
+    sc->acc = (int64_t*)take((size_t)sc->blocks * rt * a.head_dim * 8);
+    sc->wide = nullptr;
+    sc->flags = 0;
+    return at;
+  }
   sc->next = (uint32_t*)take(8);
   sc->tiles = (uint32_t*)take(((size_t)a.requests + 1) * 4);
   sc->tc_tiles = (uint32_t*)take(((size_t)a.requests + 1) * 4);
@@ -429,6 +461,10 @@ cudaError_t launch(const IrisPromptAttention& a, const PromptScratch& sc, const 
   static std::atomic<bool> allowed[64];
   cudaError_t e = allow_smem(prompt_mma_kernel<RT>, allowed);
   if (e != cudaSuccess) return e;
+  if (!sc.order) {
+    prompt_mma_kernel<RT><<<sc.blocks, kPromptThreads, smem, stream>>>(a, sc);
+    return cudaGetLastError();
+  }
   prompt_items_kernel<<<sc.flags ? 2 : 1, 1024, 0, stream>>>(a, sc, RT);
   e = cudaGetLastError();
   if (e == cudaSuccess && sc.flags) e = launch_prompt_tc(a, tc, sc.blocks, stream);
