@@ -406,10 +406,18 @@ size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 // cover 16 dimensions x 32 rows, sixteen warps).
 uint32_t row_tile(const IrisPromptAttention& a) { return a.head_dim <= 128 ? 64 : 32; }
 
-// The tensor-core kernel's packing and its two further launches pay from
-// requests of a few hundred rows on.
-constexpr uint32_t kTcLongest = 256;
-bool on_tensor_cores(const IrisPromptAttention& a) { return a.longest >= kTcLongest && prompt_tc_usable(a); }
+// The tensor-core kernel's packing and its two further launches pay for one
+// long request, whose tiles wait for their longest, or where there is much to
+// multiply. Measured, us, there against here: 32 query heads, 8 K/V heads of 128:
+// 384 rows 81 / 70, 512 rows 93 / 101, 1,024 rows 195 / 298, thirty-two requests of
+// 130 455 / 507; 8 heads and 1 of 256: 512 rows 81 / 61, 1,024 rows 115 / 120, four
+// requests of 256 68 / 65, of 512 128 / 152; 4 heads and 1 of 64: 512 rows 65 / 60,
+// 1,024 rows 89 / 104, sixteen requests of 256 85 / 75.
+bool on_tensor_cores(const IrisPromptAttention& a) {
+  const uint64_t pairs = (uint64_t)a.tokens * a.longest;
+  return (a.longest >= 1024 || (a.longest >= 128 && pairs / 1024 * a.heads * a.head_dim >= 1u << 20)) &&
+         prompt_tc_usable(a);
+}
 
 size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, PromptTcScratch* tc) {
   const uint32_t rt = row_tile(a), group = a.heads / a.kv_heads, most = on_tensor_cores(a) ? 64 : rt;

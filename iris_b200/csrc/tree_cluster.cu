@@ -28,7 +28,6 @@ namespace cg = cooperative_groups;
 
 constexpr uint32_t kTcThreads = 256, kTcWarps = kTcThreads / 32;
 constexpr uint32_t kClusterRows = 32;          // most rows
-constexpr uint32_t kClusterPairs = 16 * 1024;  // most rows x keys of a block
 
 struct ClusterShared {
   int32_t top[kClusterRows];       // this block's, then the cluster's
@@ -243,15 +242,25 @@ uint32_t row_tiles(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
   return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
 }
-// Blocks of a cluster: as many as leave two blocks a multiprocessor over all of
-// them (one for more than eight rows, whose registers allow no second), and 32
-// keys a block. Sixteen only for up to eight rows on a free device (of many
-// clusters, or of blocks that want a multiprocessor each, sixteen are seldom free
-// in one place: 33 against 22 us for sixteen requests of 777 keys).
+// Blocks a multiprocessor holds: two of up to eight rows; more rows' registers
+// allow no second.
+uint32_t blocks_a_sm(const IrisTreeAttention& a) { return row_tiles(a) == 1 ? 2 : 1; }
+// Blocks of a cluster: as many as are on the device at once, and 32 keys a
+// block. A cluster's blocks lie together, so that fifteen clusters of eight blocks
+// a multiprocessor each find room, 33 of four, 74 of two; two blocks a
+// multiprocessor 33, 71 and 148 (four drafts of sixteen requests over 777 keys, 4
+// query heads of 64: sixteen clusters of eight 30.7 us, of four 20.1; one node of
+// four requests over 4,000 keys, 32 heads and 8 of 128: 32 clusters of eight 49 us,
+// of four 74). Sixteen only for up to eight rows on a free device: of many such
+// clusters few are free in one place (33 against 22 us for sixteen requests of 777
+// keys).
 uint32_t cluster_blocks(const IrisTreeAttention& a) {
-  const uint64_t groups = (uint64_t)a.requests * a.kv_heads, room = row_tiles(a) == 1 ? 2 * 148 : 148;
-  uint32_t n = row_tiles(a) == 1 && groups * 16 <= 148 ? 16 : 8;
-  while (n > 1 && (groups * n > room || (n - 1) * 32 >= a.longest)) n /= 2;
+  const uint64_t groups = (uint64_t)a.requests * a.kv_heads;
+  const bool two = blocks_a_sm(a) == 2;
+  if (two && groups * 16 <= 148 && 15 * 32 < a.longest) return 16;
+  const auto room = [&](uint32_t n) { return n == 8 ? (two ? 33u : 15u) : n == 4 ? (two ? 71u : 33u) : (two ? 148u : 74u); };
+  uint32_t n = 8;
+  while (n > 1 && (groups > room(n) || (n - 1) * 32 >= a.longest)) n /= 2;
   return n;
 }
 uint32_t block_span(const IrisTreeAttention& a) {
@@ -292,19 +301,22 @@ cudaError_t launch(const IrisTreeAttention& a, cudaStream_t stream) {
 
 }  // namespace
 
-// Few rows, and a span whose pairs fit a block and keep it no longer than the
-// three launches of tree_mma.cu take: up to 1,024 keys for eight rows (fewer for
-// more), half as many again where the blocks fill the device. Measured, us, here
-// against there (32 query heads, 8 K/V heads of 128): one node over 777 keys 14.8
-// / 22.1, over 12,000 60 / 79, over 30,000 242 / 136; four requests over 12,000
-// 120 / 227; eight nodes over 777 keys 24.5 / 39.1, over 4,000 67 / 57.
+// Few rows, and spans of keys that a block is done with before the three launches
+// of tree_mma.cu are: up to 256; where the blocks fill much of the device, all at
+// once, up to 1,536 for eight rows, 1,024 for sixteen, 512 for more. Measured, us,
+// here against there: 32 query heads, 8 K/V heads of 128: one node over 777 keys
+// 14.8 / 20.7, over 8,000 35 / 54, over 30,000 242 / 106; four requests over
+// 12,000 119 / 147, sixteen over 2,000 86 / 107, over 4,000 264 / 181, forty over
+// 777 130 / 118; four nodes over 8,000 64 / 84; eight nodes over 777 24.3 / 38.3,
+// four requests of them over 2,000 58 / 96. 8 query heads, 1 K/V head of 256: one
+// node over 4,000 25.1 / 24.6, over 8,000 39.5 / 26.9; four over 4,000 71 / 42,
+// eight requests of them 85 / 129.
 bool tree_cluster_usable(const IrisTreeAttention& a) {
   const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
   if (rows > kClusterRows) return false;
-  const uint32_t tiles = row_tiles(a), span = block_span(a);
+  const uint32_t tiles = row_tiles(a), span = block_span(a), most = tiles == 1 ? 1536 : tiles == 2 ? 1024 : 512;
   const uint64_t blocks = (uint64_t)a.requests * a.kv_heads * cluster_blocks(a);
-  return (uint64_t)tiles * 8 * span <= kClusterPairs &&
-         (tiles * span <= 1024 && (span <= 512 || blocks >= 64) || (tiles <= 2 && blocks >= 128 && span <= 1536));
+  return span <= 256 || (span <= most && blocks >= 64 && blocks <= 148 * blocks_a_sm(a));
 }
 
 cudaError_t launch_tree_cluster(const IrisTreeAttention& a, cudaStream_t stream) {

@@ -493,10 +493,16 @@ cudaError_t launch_values(const IrisTreeAttention& a, const TreeScratch& sc, cud
 
 }  // namespace
 
-// From two dozen query rows of a K/V head on (fewer leave the 64-row products
-// idle, and the empty launches behind cost more than they save).
+// From 33 query rows of a K/V head on, 128 keys and more; for 17 to 32, which
+// leave half of the 64-row products idle, only where much is to read. Measured, us,
+// here against the mma.sync kernels (32 query heads, 8 K/V heads of 128): sixteen
+// nodes over 256 keys 44.7 / 49.1, over 8,000 117 / 166; thirty-two nodes of sixteen
+// requests over 8,000 1,101 / 1,962; eight nodes over 8,000 93 / 90, of sixteen
+// requests over 777 128 / 122, over 2,000 196 / 201, over 8,000 542 / 616.
 bool tree_tc_usable(const IrisTreeAttention& a) {
-  return a.head_dim <= kTtD && a.nodes * (a.heads / a.kv_heads) >= 24 && a.longest >= 512 &&
+  const uint32_t rows = a.nodes * (a.heads / a.kv_heads);
+  const uint64_t keys = (uint64_t)a.requests * a.kv_heads * a.longest;
+  return a.head_dim <= kTtD && a.longest >= 128 && (rows > 32 || (rows > 16 && keys >= 1u << 18)) &&
          device_fault_word() != nullptr;
 }
 
