@@ -99,6 +99,37 @@ def test_prompt_attention_equals_the_definition(S, lengths, heads, kv_heads, d, 
     assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, scale, window))
 
 
+@pytest.mark.parametrize("lengths,heads,kv_heads,d,scaled,window,kind", [c for c in PROMPTS if sum(c[0]) >= 128])
+def test_prompt_attention_with_room_for_longer_requests(S, lengths, heads, kv_heads, d, scaled, window, kind):
+    """`longest` is a bound: with a loose one other kernels are chosen, for the same result."""
+    rng = np.random.default_rng(sum(lengths) + d + 1)
+    n = sum(lengths)
+    q = values(rng, (n, heads * d), kind)
+    k = values(rng, (n, kv_heads * d), kind)
+    v = values(rng, (n, kv_heads * d), "full" if kind == "full" else "wide" if sum(lengths) % 2 else "model")
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    scale = scale_of(d) if scaled else 0
+    for longest in (1100, 20000):
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), longest, heads=heads, kv_heads=kv_heads,
+                                 scale_q32=scale, window=window).cpu().numpy()
+        assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, scale, window))
+
+
+def test_weights_at_the_edge_between_two_values(S):
+    """Many rows of many keys: among their weights some lie within 2^-15 of the
+    edge between two values (one row of these inputs has one at 554.49996)."""
+    for lengths, heads, kv_heads, d in (([5, 64, 63, 65, 1], 8, 2, 128), ([500, 501], 8, 2, 64), ([1300], 4, 1, 32)):
+        rng = np.random.default_rng(sum(lengths) + d)
+        n = sum(lengths)
+        q, k = (values(rng, (n, w * d), "model") for w in (heads, kv_heads))
+        v = values(rng, (n, kv_heads * d), "wide")
+        offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+        for longest in (max(lengths), 2000):
+            got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), longest, heads=heads, kv_heads=kv_heads,
+                                     scale_q32=scale_of(d)).cpu().numpy()
+            assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, scale_of(d), 0))
+
+
 @pytest.mark.parametrize("heads,kv_heads,d,step", [(4, 1, 128, 61), (2, 2, 64, 61), (2, 1, 36, 61), (4, 2, 128, 1),
                                                    (2, 1, 256, 61)])
 def test_scores_at_the_lowest_value(S, heads, kv_heads, d, step):
@@ -238,6 +269,19 @@ def test_tree_attention_equals_the_definition(S, held, nodes, heads, kv_heads, d
     rng = np.random.default_rng(sum(held) + d + page)
     x = tree_inputs(rng, held, nodes, heads, kv_heads, d, page, kind)
     check_tree(S, x, heads, kv_heads, scale_of(d) if scaled else 0, window, nodes)
+
+
+@pytest.mark.parametrize("held,nodes,heads,kv_heads,d,scaled,window,page,kind", TREES)
+def test_tree_attention_with_room_for_longer_requests(S, held, nodes, heads, kv_heads, d, scaled, window, page, kind):
+    """`longest` and `nodes` are bounds: with loose ones other kernels are chosen, for the same result."""
+    rng = np.random.default_rng(sum(held) + d + page + 1)
+    x = tree_inputs(rng, held, nodes, heads, kv_heads, d, page, kind)
+    wide = np.full((len(held), (1 << 18) // page + 1), -1, np.int32)
+    wide[:, :x["table"].shape[1]] = x["table"]
+    x["table"] = wide
+    for most, longest in ((max(nodes), 3000), (max(nodes), (1 << 18) // (len(held) * kv_heads)), (64, 1500)):
+        check_tree(S, x, heads, kv_heads, scale_of(d) if scaled else 0, window, [most],
+                   max(longest, int((x["held"] + np.diff(x["offsets"])).max())))
 
 
 @pytest.mark.parametrize("d", [36, 128])
