@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           for (uint32_t c = 0; c < 8; ++c) {
             const int32_t x[5] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c],
                                   (int32_t)v[4][c]};
-            carry_diagonals(x, &hi[h * 8 + c], &lo[h * 8 + c]);
+            sum_digits<DC * kPtD>(x, &hi[h * 8 + c], &lo[h * 8 + c]);
           }
         }
         tc_fence_before();

@@ -138,11 +138,12 @@ __device__ __forceinline__ uint32_t key_products(const int32_t* k0, const int32_
 // times the scale down 32 bits, then down 16 to nearest even (one addition, as
 // in mul_sat), saturated where the high word is past 16 bits.
 __device__ __forceinline__ int32_t score_of(int32_t hi, uint32_t lo, uint32_t scale) {
-  uint64_t s = ((uint64_t)(uint32_t)hi << 32) | lo;
-  if (scale) s = (uint64_t)((int64_t)hi * (int32_t)scale) + __umulhi(lo, scale);
-  s += 0x7FFF + (((uint32_t)s >> 16) & 1);
+  // half added first; on a tie that leaves 16 zeros, and the even neighbour has no low bit
+  uint64_t s = (((uint64_t)(uint32_t)hi << 32) | lo) + 0x8000;
+  if (scale) s = (uint64_t)((int64_t)hi * (int32_t)scale) + (__umulhi(lo, scale) + 0x8000u);
   const int32_t top = (int32_t)(s >> 32);
-  const int32_t low = (int32_t)__funnelshift_r((uint32_t)s, (uint32_t)top, 16);
+  int32_t low = (int32_t)__funnelshift_r((uint32_t)s, (uint32_t)top, 16);
+  if (((uint32_t)s & 0xFFFFu) == 0) low &= ~1;
   return (uint32_t)(top + 0x8000) < 0x10000u ? low : (top >> 31) ^ INT32_MAX;
 }
 // Five diagonals: carried byte by byte, the low 32 bits from the bytes left behind.

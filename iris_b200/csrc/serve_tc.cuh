@@ -51,6 +51,19 @@ __device__ __forceinline__ void split_digits(int32_t x, int32_t y, int32_t z, in
   for (uint32_t i = 0; i < 3; ++i) p[i] ^= 0x80808080u;
 }
 
+// The 64-bit sum of five diagonals of signed digits over D dims: for up to 128,
+// two diagonals together are below 2^31 (2^21 + 2^8 2^22, 3 2^21 + 2^8 2^22).
+template <uint32_t D>
+__device__ __forceinline__ void sum_digits(const int32_t (&v)[5], int32_t* hi, uint32_t* lo) {
+  if (D > 128) {
+    carry_diagonals(v, hi, lo);
+    return;
+  }
+  const int64_t s = (int64_t)(v[2] + v[3] * 256) * 65536 + (v[0] + v[1] * 256);
+  *hi = (int32_t)(s >> 32) + v[4];
+  *lo = (uint32_t)s;
+}
+
 // Byte offset of byte x of row y in a tile of 128-byte rows in the 128-byte
 // swizzle: 16-byte pieces exchanged by the row's low bits.
 __device__ __forceinline__ uint32_t swizzled(uint32_t y, uint32_t x) { return y * 128 + (((x >> 4) ^ (y & 7)) << 4) + (x & 15); }

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 #pragma unroll
         for (uint32_t c = 0; c < 8; ++c) {
           const int32_t w[5] = {(int32_t)v[0][c], (int32_t)v[1][c], (int32_t)v[2][c], (int32_t)v[3][c], (int32_t)v[4][c]};
-          carry_diagonals(w, &hi[h * 8 + c], &lo[h * 8 + c]);
+          sum_digits<kTtD>(w, &hi[h * 8 + c], &lo[h * 8 + c]);
         }
       }
     }
