@@ -24,7 +24,8 @@ namespace iris {
 
 namespace {
 
-constexpr uint32_t kTtD = 128, kTtKeys = 128, kTtThreads = 512, kTtWarps = kTtThreads / 32;
+constexpr uint32_t kTtD = 128, kTtKeys = 128, kTtWarps = 16, kTtWork = 32 * kTtWarps;
+constexpr uint32_t kTtThreads = kTtWork + 32;         // and one warp that issues the products
 constexpr uint32_t kTtTile = 64;                      // query rows of a score tile
 constexpr uint32_t kTtRows = 256;                     // query rows a scores block holds
 constexpr uint32_t kTtPlane = kTtKeys * kTtD;         // bytes of a key or value plane
@@ -59,11 +60,11 @@ __device__ __forceinline__ void tt_free(const TtBlock& s, uint32_t warp, uint32_
 struct TtScores {
   TtBlock b;
   uint64_t ready;             // a score tile's products are done
+  uint64_t taken;             // and out of TMEM, the next tile's keys in shared memory
   uint64_t row_at[kTtRows];   // the rows' scores
   uint64_t mask[kTtRows];     // the nodes a row sees
   uint32_t position[kTtRows];
   int32_t top[kTtRows];
-  uint8_t seen[4][kTtKeys];   // whether a key's page is in the pool
 };
 
 __global__ void __launch_bounds__(kTtThreads, 1)
@@ -98,6 +99,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 
   if (tid == 0) {
     mbar_init(&s.ready, 1);
+    mbar_init(&s.taken, kTtWarps);
     s.b.dead = 0;
     s.b.wide = 0;
     mbar_fence_init();
@@ -112,25 +114,35 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     s.top[i] = INT32_MIN;
   }
   uint32_t wide = 0;
+  const bool works = warp < kTtWarps;  // (the last warp issues)
   // the query rows: a warp a row and turn, four values a lane
-#pragma unroll 4
-  for (uint32_t i = warp; i < rts * kTtTile; i += kTtWarps) {
-    const uint32_t f = f0 + min(i, rows - 1);
-    const int32_t* src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
-    const int4 x = used ? *(const int4*)(src + 4 * lane) : none;
-    uint32_t p[4];
-    split_digits(x.x, x.y, x.z, x.w, p);
-    wide |= p[3];
-    uint8_t* dst = qs + i / kTtTile * 3 * kTtQPlane + swizzled(i % kTtTile, 4 * lane);
+  if (works) {
+#pragma unroll 1
+    for (uint32_t i0 = warp; i0 < rts * kTtTile; i0 += 4 * kTtWarps) {
+      int4 x[4];
 #pragma unroll
-    for (uint32_t j = 0; j < 3; ++j) *(uint32_t*)(dst + j * kTtQPlane) = p[j];
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t f = f0 + min(i0 + u * kTtWarps, rows - 1);
+        const int32_t* src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+        x[u] = used ? *(const int4*)(src + 4 * lane) : none;
+      }
+#pragma unroll
+      for (uint32_t u = 0; u < 4; ++u) {
+        const uint32_t i = i0 + u * kTtWarps;  // (a row tile is four turns of the warps)
+        uint32_t p[4];
+        split_digits(x[u].x, x[u].y, x[u].z, x[u].w, p);
+        wide |= p[3];
+        uint8_t* dst = qs + i / kTtTile * 3 * kTtQPlane + swizzled(i % kTtTile, 4 * lane);
+#pragma unroll
+        for (uint32_t j = 0; j < 3; ++j) *(uint32_t*)(dst + j * kTtQPlane) = p[j];
+      }
+    }
   }
   // the keys of a tile: a warp takes eight of them, four values a lane
   int4 x[8];
   auto load_keys = [&](uint32_t kt) {
     const uint32_t mine = kt * kTtKeys + warp * 8 + (lane & 7);
     int64_t row = mine < count ? page_row(table, a.width, a.page_size, a.pages, key0 + mine) : -1;
-    if (lane < 8) s.seen[kt & 3][warp * 8 + lane] = row >= 0;
     if (row < 0) row = 0;  // hidden keys are masked: any row will do
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -150,52 +162,69 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       for (uint32_t j = 0; j < 3; ++j) *(uint32_t*)(dst + j * kTtPlane + at) = p[j];
     }
   };
-  load_keys(0);
-  put_keys(0);
-  if (kts > 1) load_keys(1);
+  // whether the key of a lane's scores is there, its page in the pool
+  const uint32_t quad = warp & 3, cg = warp >> 2, tiles = kts * rts;
+  auto is_there = [&](uint32_t kt) {
+    const uint32_t k = kt * kTtKeys + 32 * quad + lane;
+    return k < count && page_row(table, a.width, a.page_size, a.pages, key0 + k) >= 0;
+  };
+  bool there = false, there_next = false;
+  if (works) {
+    load_keys(0);
+    there = is_there(0);
+    put_keys(0);
+    if (kts > 1) {
+      load_keys(1);
+      there_next = is_there(1);
+    }
+  }
   fence_async_shared();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.b.tmem;
-  const uint64_t keys_d = tc_desc(smem_addr(keys)), qs_d = tc_desc(smem_addr(qs));
-  const bool leader = tid == 0;
-  // one score tile's products: plane i of the keys against all three of the
-  // rows is diagonals i, i + 1, i + 2; a diagonal's first product overwrites it
-  auto issue = [&](uint32_t kt, uint32_t rt) {
-    const uint64_t kd = keys_d + (kt & 1) * (3 * kTtPlane / 16), qd = qs_d + rt * (3 * kTtQPlane / 16);
+  if (!works) {
+    // one score tile's products: plane i of the keys against all three of the
+    // rows is diagonals i, i + 1, i + 2; a diagonal's first product overwrites it
+    const uint64_t keys_d = tc_desc(smem_addr(keys)), qs_d = tc_desc(smem_addr(qs));
+    const bool leader = lane == 0;
+    for (uint32_t n = 0; n < tiles; ++n) {
+      if (n && !tc_wait(&s.taken, (n - 1) & 1, &s.b.dead, fault)) break;
+      __syncwarp();
+      tc_fence_after();
+      const uint32_t kt = n / rts, rt = n % rts;
+      const uint64_t kd = keys_d + (kt & 1) * (3 * kTtPlane / 16), qd = qs_d + rt * (3 * kTtQPlane / 16);
 #pragma unroll
-    for (uint32_t i = 0; i < 3; ++i) {
-      const uint64_t key = kd + i * (kTtPlane / 16);
-      const uint32_t col = tmem + i * kTtTile;
-      if (i == 0) {
-        tc_mma_by(col, key, qd, tc_idesc_n(true, true, 3 * kTtTile), false, leader);
-      } else {
-        tc_mma_by(col, key, qd, tc_idesc_n(true, true, 2 * kTtTile), true, leader);
-        tc_mma_by(col + 2 * kTtTile, key, qd + 2 * (kTtQPlane / 16), tc_idesc_n(true, true, kTtTile), false, leader);
+      for (uint32_t i = 0; i < 3; ++i) {
+        const uint64_t key = kd + i * (kTtPlane / 16);
+        const uint32_t col = tmem + i * kTtTile;
+        if (i == 0) {
+          tc_mma_by(col, key, qd, tc_idesc_n(true, true, 3 * kTtTile), false, leader);
+        } else {
+          tc_mma_by(col, key, qd, tc_idesc_n(true, true, 2 * kTtTile), true, leader);
+          tc_mma_by(col + 2 * kTtTile, key, qd + 2 * (kTtQPlane / 16), tc_idesc_n(true, true, kTtTile), false, leader);
+        }
+#pragma unroll
+        for (uint32_t kk = 1; kk < 4; ++kk)
+          tc_mma_by(col, key + 2 * kk, qd + 2 * kk, tc_idesc_n(true, true, 3 * kTtTile), true, leader);
       }
-#pragma unroll
-      for (uint32_t kk = 1; kk < 4; ++kk)
-        tc_mma_by(col, key + 2 * kk, qd + 2 * kk, tc_idesc_n(true, true, 3 * kTtTile), true, leader);
+      tc_commit_by(&s.ready, leader);
     }
-    tc_commit_by(&s.ready, leader);
-  };
-  if (warp == 0) issue(0, 0);
-  const uint32_t quad = warp & 3, cg = warp >> 2, tiles = kts * rts;
-  for (uint32_t n = 0; n < tiles; ++n) {
-    const uint32_t kt = n / rts, rt = n % rts;
-    // With a key tile's last row tile the next keys, loaded one tile ahead, go
-    // to the other buffer (its products were waited for before).
-    const bool turn = rt + 1 == rts;
-    if (turn && kt + 1 < kts) {
-      put_keys(kt + 1);
-      fence_async_shared();
-    }
-    const bool ok = tc_wait(&s.ready, n & 1, &s.b.dead, fault);
-    tc_fence_after();
-    uint32_t lo[16];
-    int32_t hi[16];
-    if (ok) {
+  } else {
+    for (uint32_t n = 0; n < tiles; ++n) {
+      const uint32_t kt = n / rts, rt = n % rts;
+      // With a key tile's last row tile the next keys, loaded one tile ahead, go
+      // to the other buffer (its products were waited for before).
+      const bool turn = rt + 1 == rts;
+      if (turn && kt + 1 < kts) {
+        put_keys(kt + 1);
+        fence_async_shared();
+      }
+      if (!tc_wait(&s.ready, n & 1, &s.b.dead, fault)) break;
+      __syncwarp();
+      tc_fence_after();
+      uint32_t lo[16];
+      int32_t hi[16];
 #pragma unroll
       for (uint32_t h = 0; h < 2; ++h) {
         uint32_t v[5][8];
@@ -208,38 +237,44 @@ __global__ void __launch_bounds__(kTtThreads, 1)
           sum_digits<kTtD>(w, &hi[h * 8 + c], &lo[h * 8 + c]);
         }
       }
-    }
-    tc_fence_before();
-    // the diagonals are read, the next tile's keys in shared memory
-    if (__syncthreads_or(!ok)) break;
-    if (warp == 0 && n + 1 < tiles) {
-      tc_fence_after();
-      issue((n + 1) / rts, (n + 1) % rts);
-    }
-    if (turn && kt + 2 < kts) load_keys(kt + 2);
-    const uint32_t k = kt * kTtKeys + 32 * quad + lane, key = key0 + k;
-    const bool there = k < count && s.seen[kt & 3][32 * quad + lane];
-    const bool open = !a.window && __all_sync(0xffffffffu, there && key < q.held);
-    // a node's key: its bit in the rows' masks, and its position
-    const uint32_t node = key - q.held, place = key < q.held ? key : 0;
-    const uint64_t bit = key < q.held ? ~0ull : node < kTreeNodes ? 1ull << node : 0;
-    const uint32_t at = a.window && there && key >= q.held ? (uint32_t)a.positions[q.begin + node] : place;
-    int32_t* out = sc.scores + (key - q.base);
-    const bool inside = key - q.base < sc.pitch;
-    int32_t best = INT32_MIN;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.taken);
+      int32_t y[16];
+      scores_of(hi, lo, a.scale_q32, y);
+      const uint32_t k = kt * kTtKeys + 32 * quad + lane, key = key0 + k;
+      if (a.window || !__all_sync(0xffffffffu, there && key < q.held)) {
+        // a node's key: its bit in the rows' masks, and its position
+        const uint32_t node = key - q.held;
+        const uint64_t bit = key < q.held ? ~0ull : node < kTreeNodes ? 1ull << node : 0;
+        const uint32_t at = key < q.held ? key : a.window && there ? (uint32_t)a.positions[q.begin + node] : 0;
 #pragma unroll
-    for (uint32_t c = 0; c < 16; ++c) {
-      const uint32_t i = rt * kTtTile + cg * 16 + c;
-      int32_t y = score_of(hi[c], lo[c], a.scale_q32);
-      if (!open) {
-        const bool visible = there && (key < q.held || (s.mask[i] & bit)) && (!a.window || at + a.window > s.position[i]);
-        if (!visible) y = INT32_MIN;
+        for (uint32_t c = 0; c < 16; ++c) {
+          const uint32_t i = rt * kTtTile + cg * 16 + c;
+          if (!there || !(key < q.held || (s.mask[i] & bit)) || (a.window && at + a.window <= s.position[i])) y[c] = INT32_MIN;
+        }
       }
-      if (inside) out[s.row_at[i]] = y;
-      const int32_t m = __reduce_max_sync(0xffffffffu, y);
-      best = lane == c ? m : best;
+      int32_t* out = sc.scores + (key - q.base);
+      if (key - q.base < sc.pitch) {
+#pragma unroll
+        for (uint32_t c = 0; c < 16; ++c) out[s.row_at[rt * kTtTile + cg * 16 + c]] = y[c];
+      }
+      __syncwarp();
+      int32_t best = INT32_MIN;
+#pragma unroll
+      for (uint32_t c = 0; c < 16; ++c) {
+        const int32_t m = __reduce_max_sync(0xffffffffu, y[c]);
+        best = lane == c ? m : best;
+      }
+      if (lane < 16) atomicMax(&s.top[rt * kTtTile + cg * 16 + lane], best);
+      if (turn) {
+        there = there_next;
+        if (kt + 2 < kts) {
+          load_keys(kt + 2);
+          there_next = is_there(kt + 2);
+        }
+      }
     }
-    if (lane < 16) atomicMax(&s.top[rt * kTtTile + cg * 16 + lane], best);
   }
   if (wide) s.b.wide = 1;
   __syncthreads();
@@ -254,6 +289,7 @@ template <uint32_t RB>
 struct TtValues {
   TtBlock b;
   uint64_t done[2];  // the products of a stage's buffers
+  uint64_t full[2];  // a stage's values and weights are in shared memory
   uint64_t sum[RB];
   uint32_t recip[RB], first[RB], id[RB];  // id: the row's place in the scratch, UINT32_MAX past the last
   int32_t wsum[RB];
@@ -264,7 +300,7 @@ struct TtValues {
 template <uint32_t RB>
 __global__ void __launch_bounds__(kTtThreads, 1)
     tree_tc_values_kernel(IrisTreeAttention a, TreeScratch sc, unsigned int* fault) {
-  constexpr uint32_t kWPlane = RB * kTtKeys, kUnits = RB * 16 / kTtThreads;  // a thread's units of eight weights
+  constexpr uint32_t kWPlane = RB * kTtKeys, kUnits = RB * 16 / kTtWork;  // a thread's units of eight weights
   extern __shared__ uint8_t tt_raw[];
   __shared__ __align__(16) TtValues<RB> s;
   uint8_t* vals = aligned_1024(tt_raw);                       // two stages of three planes [dim][128 keys]
@@ -287,6 +323,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   if (tid == 0) {
     mbar_init(&s.done[0], 1);
     mbar_init(&s.done[1], 1);
+    mbar_init(&s.full[0], kTtWarps);
+    mbar_init(&s.full[1], kTtWarps);
     s.b.dead = 0;
     s.b.wide = 0;
     mbar_fence_init();
@@ -311,10 +349,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
     }
   };
-  load_values(0);
+  const bool works = warp < kTtWarps;  // (the last warp issues)
+  if (works) load_values(0);
   pdl_wait();
 #pragma unroll 4
-  for (uint32_t i = warp; i < RB; i += kTtWarps) {
+  for (uint32_t i = warp; works && i < RB; i += kTtWarps) {
     const uint32_t f = f0 + i;
     uint64_t sum = 0;
     uint32_t first = UINT32_MAX, id = UINT32_MAX;
@@ -339,8 +378,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s.b.tmem;
-  const uint64_t vals_d = tc_desc(smem_addr(vals)), wts_d = tc_desc(smem_addr(wts));
-  const bool leader = tid == 0;
   uint4 t[kUnits][2];
   // unit u of a thread: eight keys of row tid / 16 + 32 u
   auto load_terms = [&](uint32_t st) {
@@ -355,13 +392,44 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
     }
   };
-  load_terms(0);
+  if (works) load_terms(0);
   uint32_t wide = 0;
   int32_t total[kUnits] = {};
   bool ok = true;
-  for (uint32_t st = 0; st < stages; ++st) {
+  if (!works) {
+    // value plane i against both weight planes: diagonals i, i + 1
+    const uint64_t vals_d = tc_desc(smem_addr(vals)), wts_d = tc_desc(smem_addr(wts));
+    const bool leader = lane == 0;
+    for (uint32_t st = 0; st < stages; ++st) {
+      const uint32_t buf = st & 1;
+      if (!tc_wait(&s.full[buf], (st >> 1) & 1, &s.b.dead, fault)) break;
+      __syncwarp();
+      tc_fence_after();
+      const uint64_t vd = vals_d + buf * (3 * kTtPlane / 16), wd = wts_d + buf * (2 * kWPlane / 16);
+#pragma unroll
+      for (uint32_t i = 0; i < 3; ++i) {
+        const uint64_t val = vd + i * (kTtPlane / 16);
+        const uint32_t col = tmem + i * RB;
+        if (st == 0 && i) {
+          tc_mma_by(col, val, wd, tc_idesc_n(true, false, RB), true, leader);
+          tc_mma_by(col + RB, val, wd + kWPlane / 16, tc_idesc_n(true, false, RB), false, leader);
+        } else {
+          tc_mma_by(col, val, wd, tc_idesc_n(true, false, 2 * RB), st != 0, leader);
+        }
+#pragma unroll
+        for (uint32_t kk = 1; kk < 4; ++kk)
+          tc_mma_by(col, val + 2 * kk, wd + 2 * kk, tc_idesc_n(true, false, 2 * RB), true, leader);
+      }
+      tc_commit_by(&s.done[buf], leader);
+    }
+  }
+  for (uint32_t st = 0; works && st < stages; ++st) {
     const uint32_t buf = st & 1;
-    if (st >= 2) ok = tc_wait(&s.done[buf], ((st >> 1) - 1) & 1, &s.b.dead, fault);
+    if (st >= 2) {
+      ok = tc_wait(&s.done[buf], ((st >> 1) - 1) & 1, &s.b.dead, fault);
+      if (!ok) break;
+      __syncwarp();
+    }
     uint8_t* vb = vals + buf * 3 * kTtPlane;
     uint8_t* wb = wts + buf * 2 * kWPlane;
 #pragma unroll
@@ -397,30 +465,11 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       *(uint2*)(dst + kWPlane) = make_uint2(__byte_perm(t0, t1, 0x7632), __byte_perm(u0, u1, 0x7632));
     }
     fence_async_shared();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s.full[buf]);
     if (st + 1 < stages) {
       load_values(st + 1);
       load_terms(st + 1);
-    }
-    if (__syncthreads_or(!ok)) break;
-    if (warp == 0) {
-      // value plane i against both weight planes: diagonals i, i + 1
-      tc_fence_after();
-      const uint64_t vd = vals_d + buf * (3 * kTtPlane / 16), wd = wts_d + buf * (2 * kWPlane / 16);
-#pragma unroll
-      for (uint32_t i = 0; i < 3; ++i) {
-        const uint64_t val = vd + i * (kTtPlane / 16);
-        const uint32_t col = tmem + i * RB;
-        if (st == 0 && i) {
-          tc_mma_by(col, val, wd, tc_idesc_n(true, false, RB), true, leader);
-          tc_mma_by(col + RB, val, wd + kWPlane / 16, tc_idesc_n(true, false, RB), false, leader);
-        } else {
-          tc_mma_by(col, val, wd, tc_idesc_n(true, false, 2 * RB), st != 0, leader);
-        }
-#pragma unroll
-        for (uint32_t kk = 1; kk < 4; ++kk)
-          tc_mma_by(col, val + 2 * kk, wd + 2 * kk, tc_idesc_n(true, false, 2 * RB), true, leader);
-      }
-      tc_commit_by(&s.done[buf], leader);
     }
   }
   if (wide) s.b.wide = 1;
@@ -428,7 +477,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   if (ok) ok = tc_wait(&s.done[(stages - 1) & 1], ((stages - 1) >> 1) & 1, &s.b.dead, fault);
   tc_fence_after();
   const uint32_t quad = warp & 3, cg = warp >> 2;
-  if (ok) {
+  if (ok && works) {
 #pragma unroll 1
     for (uint32_t c0 = 0; c0 < RB / 4; c0 += 8) {
       uint32_t v[4][8];
@@ -446,7 +495,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     }
   }
 #pragma unroll
-  for (uint32_t u = 0; u < kUnits; ++u) {
+  for (uint32_t u = 0; works && u < kUnits; ++u) {
     int32_t y = total[u];
 #pragma unroll
     for (uint32_t o = 1; o <= 8; o <<= 1) y += __shfl_xor_sync(0xffffffffu, y, o);
@@ -463,7 +512,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   __syncthreads();
   if (s.last) {
-    for (uint32_t i = warp; i < min(RB, rows - f0); i += kTtWarps) {
+    for (uint32_t i = warp; i < min(RB, rows - f0); i += kTtThreads / 32) {
       const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group, first = s.first[i];
       const size_t id = s.id[i];
       const int64_t row = first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
