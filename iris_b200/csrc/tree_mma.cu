@@ -504,6 +504,24 @@ uint32_t keys_a_block(uint64_t groups, uint32_t longest, uint32_t most, uint32_t
   return chunk;
 }
 
+// The same for the tensor-core launches, whose blocks have a multiprocessor each
+// and start with work of `start` tenths of a tile of 128 keys: one request is cut
+// so that its blocks fill whole waves (sixty-four nodes over 12,000 keys: chunks of
+// 128 keys 340 us, by this rule 223); several, whose lengths differ, into
+// two waves or more.
+uint32_t tc_keys_a_block(uint32_t requests, uint64_t groups, uint32_t longest, uint32_t start, uint32_t most) {
+  if (requests > 1) return std::max(128u, keys_a_block(requests * groups, longest, most, 2 * 148));
+  const uint32_t tiles = ceil_div(longest, 128), least = (uint32_t)((groups + 147) / 148);
+  uint32_t best = 1;
+  uint64_t cost = UINT64_MAX;
+  for (uint32_t waves = least; waves < least + 8; ++waves) {
+    const uint32_t t = std::min<uint64_t>(ceil_div(tiles, (uint32_t)std::min<uint64_t>(148 * waves / groups, tiles)), most / 128);
+    const uint64_t blocks = groups * ceil_div(tiles, t), c = (blocks + 147) / 148 * (10 * t + start);
+    if (c < cost) cost = c, best = t;
+  }
+  return best * 128;
+}
+
 // Row tiles a warp of the third launch takes (8 rows each, two warps a tile of
 // dimensions for up to 128 of them): 32 rows do not pay for 64.
 uint32_t value_tiles(const IrisTreeAttention& a) {
@@ -521,8 +539,8 @@ uint32_t value_rows(const IrisTreeAttention& a) { return value_tiles(a) * 8 * (a
 size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
   const size_t rows = (size_t)a.rows * a.heads;
   sc->chunk = keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 2 * 148);
-  if (tree_tc_usable(a))  // whole key tiles of the tensor-core launch, a block a multiprocessor
-    sc->chunk = std::max(128u, keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 2048, 3 * 148));
+  if (tree_tc_usable(a))  // whole key tiles of the tensor-core launch
+    sc->chunk = tc_keys_a_block(a.requests, a.kv_heads * ceil_div(a.nodes * (a.heads / a.kv_heads), kTreeTcRows), a.longest, 13, 4096);
   sc->chunks = ceil_div(a.longest, sc->chunk);
   sc->groups = few_rows(a) ? 1 : ceil_div(a.nodes * (a.heads / a.kv_heads), value_rows(a));
   sc->vchunk = few_rows(a) ? keys_a_block((uint64_t)a.requests * a.kv_heads, a.longest, 512, 4 * 148)
@@ -550,8 +568,7 @@ size_t carve(const IrisTreeAttention& a, uint8_t* base, TreeScratch* sc) {
     const uint32_t rows_most = a.nodes * (a.heads / a.kv_heads);
     sc->tc_rows = rows_most <= 64 ? 64 : 128;
     sc->tc_groups = ceil_div(rows_most, sc->tc_rows);
-    sc->tc_vchunk = keys_a_block((uint64_t)a.requests * a.kv_heads * sc->tc_groups, a.longest, 4096, 3 * 148);
-    if (sc->tc_vchunk < 128) sc->tc_vchunk = 128;
+    sc->tc_vchunk = tc_keys_a_block(a.requests, (uint64_t)a.kv_heads * sc->tc_groups, a.longest, 20, 4096);
     sc->tc_vchunks = ceil_div(a.longest, sc->tc_vchunk);
     sc->tc_acc = (int64_t*)take(rows * a.head_dim * 8);
     sc->tc_wsum = (int32_t*)take(rows * 4);

@@ -27,7 +27,7 @@ namespace {
 constexpr uint32_t kTtD = 128, kTtKeys = 128, kTtWarps = 16, kTtWork = 32 * kTtWarps;
 constexpr uint32_t kTtThreads = kTtWork + 32;         // and one warp that issues the products
 constexpr uint32_t kTtTile = 64;                      // query rows of a score tile
-constexpr uint32_t kTtRows = 256;                     // query rows a scores block holds
+constexpr uint32_t kTtRows = kTreeTcRows;             // query rows a scores block holds
 constexpr uint32_t kTtPlane = kTtKeys * kTtD;         // bytes of a key or value plane
 constexpr uint32_t kTtQPlane = kTtTile * kTtD;
 

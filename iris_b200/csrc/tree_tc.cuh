@@ -31,6 +31,7 @@ struct TreeScratch {
 };
 
 constexpr uint32_t kTreeSegment = 1024;  // keys a warp takes in the second launch
+constexpr uint32_t kTreeTcRows = 256;    // query rows of a tensor-core scores block
 
 // One request's part of the call: its keys from `base` on (a multiple of 64; a
 // window hides all below from every node). Made by whole warps.
