@@ -80,13 +80,13 @@ __global__ void __launch_bounds__(kTcThreads) tree_cluster_kernel(IrisTreeAttent
     s.sum[tid] = 0;
     s.first[tid] = UINT32_MAX;
     s.wsum[tid] = 0;
-    s.node[tid] = std::min(tid, rows - 1) / q.group;
+    s.node[tid] = q.node_of(std::min(tid, rows - 1));
   }
   if (tid == 0) s.q_wide = 0;
   __syncthreads();
   for (uint32_t u = warp; u < NT * steps; u += kTcWarps) {
     const uint32_t nt = u / steps, f = std::min(8 * nt + (lane >> 2), rows - 1);  // (rows past the last repeat it)
-    const int32_t* src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+    const int32_t* src = a.q + (size_t)(q.begin + q.node_of(f)) * a.q_stride + q.head_of(f, g) * a.head_dim;
     if (put_query_fragment(frag, steps, nt, u % steps, lane, src)) s.q_wide = 1;
   }
   __syncthreads();
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kTcThreads) tree_cluster_kernel(IrisTreeAttent
       mac_wide(sum, rest, a.v_pages[(size_t)row * kvd + g * a.head_dim + x]);
       y = requantize(sum);
     }
-    a.out[(size_t)(q.begin + f / q.group) * a.out_stride + (g * q.group + f % q.group) * a.head_dim + x] = y;
+    a.out[(size_t)(q.begin + q.node_of(f)) * a.out_stride + q.head_of(f, g) * a.head_dim + x] = y;
   }
   cluster.sync();  // the others' reads of this block's sums are over
 }

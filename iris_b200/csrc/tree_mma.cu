@@ -55,11 +55,10 @@ __global__ void __launch_bounds__(kTreeThreads, NT == 1 ? 4 : 2) tree_scores_ker
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, steps = a.head_dim / 32;
   const uint32_t rows = q.nodes * q.group, key0 = q.base + chunk * sc.chunk;
   if (chunk == 0 && !sc.flags) {  // the totals of this request and head start at zero
-    for (uint32_t i = tid; i < rows * a.head_dim; i += kTreeThreads) {
-      const uint32_t f = i / a.head_dim, x = i % a.head_dim;
-      const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-      sc.acc[id * a.head_dim + x] = 0;
-      if (x == 0) sc.wsum[id] = 0;
+    for (uint32_t f = warp; f < rows; f += kTreeWarps) {
+      const size_t id = (size_t)(q.begin + q.node_of(f)) * a.heads + q.head_of(f, g);
+      for (uint32_t x = lane; x < a.head_dim; x += 32) sc.acc[id * a.head_dim + x] = 0;
+      if (lane == 0) sc.wsum[id] = 0;
     }
     for (uint32_t i = tid; i < sc.groups; i += kTreeThreads) sc.done[((size_t)r * a.kv_heads + g) * sc.groups + i] = 0;
   }
@@ -72,7 +71,7 @@ __global__ void __launch_bounds__(kTreeThreads, NT == 1 ? 4 : 2) tree_scores_ker
     if (f0) __syncthreads();
     if (tid < kTreeTile) {
       // (rows past the last one repeat it)
-      const uint32_t f = min(f0 + tid, rows - 1), node = f / q.group, head = g * q.group + f % q.group;
+      const uint32_t f = min(f0 + tid, rows - 1), node = q.node_of(f), head = q.head_of(f, g);
       row_node[tid] = node;
       row_at[tid] = ((size_t)(q.begin + node) * a.heads + head) * sc.pitch;
       row_max[tid] = INT32_MIN;
@@ -81,7 +80,7 @@ __global__ void __launch_bounds__(kTreeThreads, NT == 1 ? 4 : 2) tree_scores_ker
     __syncthreads();
     for (uint32_t u = warp; u < NT * steps; u += kTreeWarps) {
       const uint32_t nt = u / steps, i = 8 * nt + (lane >> 2), f = min(f0 + i, rows - 1);
-      const int32_t* src = a.q + (size_t)(q.begin + row_node[i]) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+      const int32_t* src = a.q + (size_t)(q.begin + row_node[i]) * a.q_stride + q.head_of(f, g) * a.head_dim;
       if (put_query_fragment(frag, steps, nt, u % steps, lane, src)) q_wide = 1;
     }
     __syncthreads();
@@ -198,7 +197,7 @@ __device__ __forceinline__ void finish_rows(const IrisTreeAttention& a, const in
                                             uint32_t warps, uint32_t lane) {
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
   for (uint32_t i = warp; i < n; i += warps) {
-    const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group, first = firsts[i];
+    const uint32_t node = q.node_of(f0 + i), head = q.head_of(f0 + i, g), first = firsts[i];
     const size_t id = ids[i];
     const int64_t row =
         first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
@@ -362,7 +361,7 @@ __global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeA
     uint64_t sum = 0;
     uint32_t first = UINT32_MAX, id = UINT32_MAX;
     if (f < rows) {
-      id = (q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
+      id = (q.begin + q.node_of(f)) * a.heads + q.head_of(f, g);
       for (uint32_t x = lane; x < segs; x += 32) {
         sum += sc.seg_sum[(size_t)id * sc.segs + x];
         first = min(first, sc.seg_first[(size_t)id * sc.segs + x]);
@@ -439,7 +438,7 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
     uint64_t sum = 0;
     uint32_t first = UINT32_MAX, id = UINT32_MAX;
     if (i < rows) {
-      id = (q.begin + i / q.group) * a.heads + g * q.group + i % q.group;
+      id = (q.begin + q.node_of(i)) * a.heads + q.head_of(i, g);
       for (uint32_t x = lane; x < segs; x += 32) {
         sum += sc.seg_sum[(size_t)id * sc.segs + x];
         first = min(first, sc.seg_first[(size_t)id * sc.segs + x]);
@@ -610,7 +609,8 @@ cudaError_t launch_tree_mma(const IrisTreeAttention& a, uint8_t* workspace, cuda
   carve(a, workspace, &sc);
   cudaError_t e;
   if (sc.flags) {
-    e = cudaMemsetAsync(sc.flags, 0, 8, stream);
+    // totals, counters and flags, one behind another, start at zero
+    e = cudaMemsetAsync(sc.acc, 0, (size_t)((uint8_t*)(sc.flags + 2) - (uint8_t*)sc.acc), stream);
     if (e == cudaSuccess) e = launch_tree_tc_scores(a, sc, stream);
     if (e != cudaSuccess) return e;
     e = launch_k(tree_scores_kernel<4>, dim3(sc.chunks, a.kv_heads, a.requests), dim3(kTreeThreads), score_smem(a),

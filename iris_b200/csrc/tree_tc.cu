@@ -78,17 +78,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const uint32_t f0 = blockIdx.y % row_groups * kTtRows;
   const TreeRequest q(a, r);
   const uint32_t rows_all = q.nodes * q.group, key0 = q.base + chunk * sc.chunk;
-  if (chunk == 0 && f0 == 0) {  // the totals of this request and head start at zero
-    for (uint32_t i = tid; i < rows_all * a.head_dim; i += kTtThreads) {
-      const uint32_t f = i / a.head_dim, x = i % a.head_dim;
-      const size_t id = (size_t)(q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
-      sc.acc[id * a.head_dim + x] = sc.tc_acc[id * a.head_dim + x] = 0;
-      if (x == 0) sc.wsum[id] = sc.tc_wsum[id] = 0;
-    }
-    for (uint32_t i = tid; i < sc.groups; i += kTtThreads) sc.done[((size_t)r * a.kv_heads + g) * sc.groups + i] = 0;
-    for (uint32_t i = tid; i < sc.tc_groups; i += kTtThreads)
-      sc.tc_done[((size_t)r * a.kv_heads + g) * sc.tc_groups + i] = 0;
-  }
   if (key0 >= q.keys || f0 >= rows_all) return;
   const uint32_t rows = min(kTtRows, rows_all - f0), rts = (rows + kTtTile - 1) / kTtTile;
   const uint32_t count = min(sc.chunk, q.keys - key0), kts = (count + kTtKeys - 1) / kTtKeys;
@@ -106,7 +95,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   tt_alloc(s.b, warp, 512);
   for (uint32_t i = tid; i < rts * kTtTile; i += kTtThreads) {  // (rows past the last one repeat it)
-    const uint32_t f = f0 + min(i, rows - 1), node = f / q.group, head = g * q.group + f % q.group;
+    const uint32_t f = f0 + min(i, rows - 1), node = q.node_of(f), head = q.head_of(f, g);
     const uint32_t row = q.begin + node;
     s.row_at[i] = ((size_t)row * a.heads + head) * sc.pitch;
     s.mask[i] = (uint64_t)a.masks[row] & node_bits(q.nodes);
@@ -123,7 +112,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
 #pragma unroll
       for (uint32_t u = 0; u < 4; ++u) {
         const uint32_t f = f0 + min(i0 + u * kTtWarps, rows - 1);
-        const int32_t* src = a.q + (size_t)(q.begin + f / q.group) * a.q_stride + (g * q.group + f % q.group) * a.head_dim;
+        const int32_t* src = a.q + (size_t)(q.begin + q.node_of(f)) * a.q_stride + q.head_of(f, g) * a.head_dim;
         x[u] = used ? *(const int4*)(src + 4 * lane) : none;
       }
 #pragma unroll
@@ -140,10 +129,22 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   }
   // the keys of a tile: a warp takes eight of them, four values a lane
   int4 x[8];
+  // (the table's entries are read a tile ahead of the keys)
+  const uint32_t quad = warp & 3, cg = warp >> 2, tiles = kts * rts;
+  auto table_at = [&](uint32_t t) {
+    const uint32_t column = (key0 + t) / a.page_size;
+    return t < count && column < a.width ? table[column] : -1;
+  };
+  int32_t id_key = -1, id_score = -1;  // of the lane's key to load, and of the key of its scores
+  auto look_up = [&](uint32_t kt) {
+    if (kt >= kts) return;
+    id_key = table_at(kt * kTtKeys + warp * 8 + (lane & 7));
+    id_score = table_at(kt * kTtKeys + 32 * quad + lane);
+  };
   auto load_keys = [&](uint32_t kt) {
-    const uint32_t mine = kt * kTtKeys + warp * 8 + (lane & 7);
-    int64_t row = mine < count ? page_row(table, a.width, a.page_size, a.pages, key0 + mine) : -1;
-    if (row < 0) row = 0;  // hidden keys are masked: any row will do
+    const uint32_t at = key0 + kt * kTtKeys + warp * 8 + (lane & 7);
+    // hidden keys are masked: any row will do
+    const int64_t row = id_key < 0 || (uint64_t)id_key >= a.pages ? 0 : (int64_t)id_key * a.page_size + at % a.page_size;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
       const int32_t* src = a.k_pages + (size_t)__shfl_sync(0xffffffffu, row, i) * kvd + g * a.head_dim;
@@ -163,19 +164,18 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     }
   };
   // whether the key of a lane's scores is there, its page in the pool
-  const uint32_t quad = warp & 3, cg = warp >> 2, tiles = kts * rts;
-  auto is_there = [&](uint32_t kt) {
-    const uint32_t k = kt * kTtKeys + 32 * quad + lane;
-    return k < count && page_row(table, a.width, a.page_size, a.pages, key0 + k) >= 0;
-  };
+  auto in_pool = [&] { return id_score >= 0 && (uint64_t)id_score < a.pages; };
   bool there = false, there_next = false;
   if (works) {
+    look_up(0);
     load_keys(0);
-    there = is_there(0);
+    there = in_pool();
+    look_up(1);
     put_keys(0);
     if (kts > 1) {
       load_keys(1);
-      there_next = is_there(1);
+      there_next = in_pool();
+      look_up(2);
     }
   }
   fence_async_shared();
@@ -271,7 +271,8 @@ __global__ void __launch_bounds__(kTtThreads, 1)
         there = there_next;
         if (kt + 2 < kts) {
           load_keys(kt + 2);
-          there_next = is_there(kt + 2);
+          there_next = in_pool();
+          look_up(kt + 3);
         }
       }
     }
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     uint64_t sum = 0;
     uint32_t first = UINT32_MAX, id = UINT32_MAX;
     if (f < rows) {
-      id = (q.begin + f / q.group) * a.heads + g * q.group + f % q.group;
+      id = (q.begin + q.node_of(f)) * a.heads + q.head_of(f, g);
       for (uint32_t y = lane; y < segs; y += 32) {
         sum += sc.seg_sum[(size_t)id * sc.segs + y];
         first = min(first, sc.seg_first[(size_t)id * sc.segs + y]);
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __syncthreads();
   if (s.last) {
     for (uint32_t i = warp; i < min(RB, rows - f0); i += kTtThreads / 32) {
-      const uint32_t node = (f0 + i) / q.group, head = g * q.group + (f0 + i) % q.group, first = s.first[i];
+      const uint32_t node = q.node_of(f0 + i), head = q.head_of(f0 + i, g), first = s.first[i];
       const size_t id = s.id[i];
       const int64_t row = first < q.count ? page_row(table, a.width, a.page_size, a.pages, q.base + first) : -1;
       const int32_t top = sub_sat(kOneAct, __ldcg(sc.tc_wsum + id));

@@ -37,6 +37,7 @@ constexpr uint32_t kTreeTcRows = 256;    // query rows of a tensor-core scores b
 // window hides all below from every node). Made by whole warps.
 struct TreeRequest {
   uint32_t begin, nodes, held, keys, group, base, count;
+  uint32_t inverse;  // of the group, rounded up: floor(f inverse / 2^32) is f / group for f and group up to 2^16
   __device__ TreeRequest(const IrisTreeAttention& a, uint32_t r) {
     begin = clamp_offset(a.offsets[r], a.rows);
     const uint32_t end = clamp_offset(a.offsets[r + 1], a.rows);
@@ -44,6 +45,7 @@ struct TreeRequest {
     held = tree_held(a, r);
     keys = min(held + nodes, a.longest);
     group = a.heads / a.kv_heads;
+    inverse = 0xFFFFFFFFu / group + 1;
     base = 0;
     if (a.window) {
       uint32_t low = held;
@@ -53,6 +55,9 @@ struct TreeRequest {
     }
     count = keys - base;
   }
+  // The node of a K/V head's row f (node * group + head), and its query head.
+  __device__ uint32_t node_of(uint32_t f) const { return group == 1 ? f : __umulhi(f, inverse); }
+  __device__ uint32_t head_of(uint32_t f, uint32_t g) const { return g * group + f - node_of(f) * group; }
 };
 
 // head_dim up to 128 and trees of enough rows.
