@@ -25,7 +25,8 @@ namespace {
 // request by one search, which a lane repeats only where its token is past it.
 // Bound by latency: 4,001 requests and a million tokens move 12 MB.
 constexpr uint32_t kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
-constexpr uint32_t kPlanMaxRequests = 16384;  // two prefix sums of 4 bytes a request in shared memory
+constexpr uint32_t kPlanMaxRequests = 16384;  // two prefix sums and the lengths, 4 bytes a request each, in shared memory
+constexpr uint32_t kPlanAhead = 4;            // tokens of a lane whose pages are read together
 
 struct PlanArgs {
   const int32_t *held, *fresh, *free_pages, *parents;
@@ -45,6 +46,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
   extern __shared__ uint32_t plan_sm[];
   uint32_t* off = plan_sm;                    // [requests + 1]
   uint32_t* base = plan_sm + a.requests + 1;  // [requests + 1]
+  uint32_t* held = base + a.requests + 1;     // [requests]
   __shared__ unsigned long long part[kPlanWarps];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t bad = 0;
@@ -57,6 +59,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     const uint32_t after = pages_of(hu + fu, a);
     if (after > a.width) bad |= IRIS_PLAN_WIDTH;
     off[r] = fu;
+    held[r] = hu;
     base[r] = after - pages_of(hu, a);
   }
   __syncthreads();
@@ -107,39 +110,54 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
   for (uint32_t r = q0 + warp; r < min(q1, a.requests); r += kPlanWarps) {
     const uint32_t n = base[r + 1] - base[r];
     if (!n) continue;
-    const uint32_t first = pages_of((uint32_t)max(a.held[r], 0), a);
+    const uint32_t first = pages_of(held[r], a);
     for (uint32_t j = lane; j < n && first + j < a.width; j += 32)
       a.table[(size_t)r * a.width + first + j] = base[r] + j < a.n_free ? a.free_pages[base[r] + j] : -1;
   }
-  // the tokens' slots and positions
-  const uint32_t begin = blockIdx.x * a.share, end = min(a.tokens, begin + a.share);
-  for (uint32_t i = begin + tid; i - lane < end; i += kPlanThreads) {
-    uint32_t r = request_of(off, a.requests, min(i - lane, total ? total - 1 : 0));
-    if (i >= end) break;
-    int64_t slot = -1, mask = 0;
-    uint32_t position = 0;
-    if (i < total) {
-      if (off[r + 1] <= i) r = r + 1 + request_of(off + r + 1, a.requests - r - 1, i);
-      const uint32_t local = i - off[r];
-      const uint32_t hu = (uint32_t)max(a.held[r], 0), at = hu + local, column = page_of(at, a);
-      const uint32_t first = pages_of(hu, a);
-      int32_t pageid = -1;
-      if (column < first) {
-        if (column < a.width) pageid = a.table[(size_t)r * a.width + column];
-      } else if (column < a.width && base[r] + (column - first) < a.n_free) {
-        pageid = a.free_pages[base[r] + (column - first)];
+  // the tokens' slots and positions: a warp's consecutive ones, kPlanAhead at a
+  // time a lane, whose requests are steps from the last one's
+  const uint32_t begin = blockIdx.x * a.share + warp * (a.share / kPlanWarps);
+  const uint32_t end = min(a.tokens, begin + a.share / kPlanWarps);
+  uint32_t r = begin < end && total ? request_of(off, a.requests, min(begin, total - 1)) : 0;
+  for (uint32_t i0 = begin; i0 < end; i0 += 32 * kPlanAhead) {
+    uint32_t own[kPlanAhead], at[kPlanAhead];
+    int32_t id[kPlanAhead];
+#pragma unroll
+    for (uint32_t u = 0; u < kPlanAhead; ++u) {
+      const uint32_t i = i0 + 32 * u + lane;
+      id[u] = -1;
+      at[u] = 0;
+      if (i < min(total, end)) {
+#pragma unroll
+        for (uint32_t step = 0; step < 2; ++step) r += off[r + 1] <= i;
+        if (off[r + 1] <= i) r += 1 + request_of(off + r + 1, a.requests - r - 1, i);
+        at[u] = held[r] + i - off[r];
+        const uint32_t column = page_of(at[u], a), first = pages_of(held[r], a);
+        if (column < a.width) {
+          const uint32_t fresh = base[r] + (column - first);
+          if (column < first) id[u] = a.table[(size_t)r * a.width + column];
+          else if (fresh < a.n_free) id[u] = a.free_pages[fresh];
+        }
       }
-      if (pageid >= 0) slot = (int64_t)pageid * a.page + (at - column * a.page);
-      position = at;
-      if (a.masks && local < kTreeNodes) {
+      own[u] = r;
+      r = __shfl_sync(0xffffffffu, r, 31);
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < kPlanAhead; ++u) {
+      const uint32_t i = i0 + 32 * u + lane;
+      if (i >= end) break;
+      int64_t mask = 0;
+      uint32_t position = at[u];
+      if (a.masks && i < total && i - off[own[u]] < kTreeNodes) {
         // the node and its ancestors; a parent that is not an earlier node
         // (or a node past 64) leaves the mask empty
-        uint32_t node = local;
+        const uint32_t first = off[own[u]];
+        uint32_t node = i - first;
         unsigned long long m = 0;
         bool good = true;
         for (;;) {
           m |= 1ull << node;
-          const int32_t up = a.parents[off[r] + node];
+          const int32_t up = a.parents[first + node];
           if (up == -1) break;
           if (up < 0 || (uint32_t)up >= node) {
             good = false;
@@ -149,13 +167,13 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
         }
         if (good) {
           mask = (int64_t)m;
-          position = hu + (uint32_t)__popcll(m) - 1;
+          position = held[own[u]] + (uint32_t)__popcll(m) - 1;
         }
       }
+      a.slots[i] = id[u] < 0 ? -1 : (int64_t)id[u] * a.page + (at[u] - page_of(at[u], a) * a.page);
+      a.positions[i] = (int32_t)position;
+      if (a.masks) a.masks[i] = mask;
     }
-    a.slots[i] = slot;
-    a.positions[i] = (int32_t)position;
-    if (a.masks) a.masks[i] = mask;
   }
 }
 
@@ -326,7 +344,7 @@ int iris_page_plan(const int32_t* d_held, const int32_t* d_fresh, uint32_t reque
   const int32_t shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   PlanArgs a{d_held, d_fresh, d_free, d_parents, requests, page_size, width, n_free, tokens, shift, share,
              d_table, d_offsets, d_positions, d_counts, d_slots, d_masks};
-  const size_t smem = (size_t)(requests + 1) * 8;
+  const size_t smem = (size_t)(requests + 1) * 8 + (size_t)requests * 4;
   static std::atomic<bool> allowed[64];
   const cudaError_t e = allow_smem(page_plan_kernel, allowed);
   if (e != cudaSuccess) return (int)e;
