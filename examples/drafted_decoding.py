@@ -139,6 +139,7 @@ def decode(model: Model, prompts: list[list[int]], count: int, nodes: int, seed:
         for r, (path, after) in enumerate(zip(done.path.tolist(), done.next.tolist())):
             if trees[r][0]:
                 out[r] += [trees[r][0][i] for i in path[1:] if i >= 0] + [after]
+    serving.stall_check()
     return [o[:count] for o in out], steps
 
 

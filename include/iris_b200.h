@@ -570,6 +570,11 @@ int iris_tree_accept(const int32_t* d_tokens, const int32_t* d_parents, const in
                      const int32_t* d_table, uint32_t width, uint32_t page_size, int32_t* d_k_pages,
                      int32_t* d_v_pages, uint32_t layers, uint64_t layer_stride, uint64_t pages, uint32_t kv_dim,
                      void* stream);
+/* The attentions above wait for their own copies and products with a bound. A
+ * wait that gave up (about a second) leaves that call's output rows undefined.
+ * Waits for `stream`, then IRIS_ESTALL if any kernel of the library on the
+ * current device gave up since the last check (which clears it), else 0. */
+int iris_stall_check(void* stream);
 
 /* Message for any status this library returns. */
 const char* iris_error(int code);

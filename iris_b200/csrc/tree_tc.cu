@@ -1,6 +1,7 @@
 // Drafted trees on the tcgen05 tensor cores (kind::i8), head_dim up to 128
-// (narrower heads padded with zeros in shared memory): the first and third launches of tree_mma.cu with their contractions on the
-// fifth-generation tensor cores.
+// (narrower heads padded with zeros in shared memory): the first and third
+// launches of tree_mma.cu with their contractions on the fifth-generation tensor
+// cores.
 //
 // Keys and values are read where they lie in their pages, once: sixteen warps
 // turn 128 of them into swizzled planes of signed base-256 digits in shared
@@ -10,8 +11,16 @@
 // (128 x 192 x 32 a product) into five int32 diagonals in TMEM, all row tiles of a
 // head against a tile of keys before the next. Values: a transposed value plane
 // against both weight planes of 64 or 128 rows into four diagonals that stay in
-// TMEM over the block's keys. One thread issues the products; every wait is
-// bounded and a give-up ends the block and is recorded in the fault word.
+// TMEM over the block's keys. A seventeenth warp issues the products (a warp that
+// also worked on the scores held the others up: 777 against 732 us in all); every
+// wait is bounded and a give-up ends the block and is recorded in the fault word.
+//
+// 64 and 48 nodes over 32,001 and 20,011 keys (32 query heads, 8 of 128 values): 251
+// us for the scores, 248 us for the values, of 701. The scores are bound by
+// their integer arithmetic and the splitting of the keys (without the score's
+// stores, the maxima, or three quarters of the products they take 1 to 5 % less), the
+// values by the reading of the terms (the scratch is 384 MB there) and the weights'
+// arithmetic; the products' unit is busy a tenth of the time.
 #include <algorithm>
 
 #include "../../include/iris_b200.h"

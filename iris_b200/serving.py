@@ -226,3 +226,10 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
                                  after.data_ptr(), now.data_ptr(), tb, table.shape[1], page, ck, cv, layers, stride,
                                  pages, kv_dim, _stream(held)), "iris_tree_accept")
     return Accepted(path, accepted, after, now)
+
+
+def stall_check() -> None:
+    """Waits for torch's current stream; raises IrisError if a kernel of the
+    library gave up a bounded wait since the last check (its rows are then
+    undefined)."""
+    check(lib().iris_stall_check(torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())), "iris_stall_check")

@@ -539,3 +539,9 @@ def test_another_stream_and_a_captured_step(S):
     dev["tokens"].copy_(cuda(rng.integers(0, 3, rows).astype(np.int32)))
     g.replay()
     check(*again)
+
+
+def test_no_wait_gave_up(S):
+    """The bounded waits of every call above held; the check reports a status, not a leftover."""
+    S.stall_check()
+    S.stall_check()
