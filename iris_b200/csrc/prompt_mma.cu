@@ -12,7 +12,7 @@
 // its item, which mostly stays in L2. Tiles are handed out longest first; few
 // tiles, a block each, are counted by the blocks themselves in one launch.
 // Bound by the chain of its phases on a few rows (five requests of up to 96 rows, 4
-// heads of 64, 29 us; two launches more 39 us) and by the products and the score and
+// heads of 64, 27 us; with the list in a launch of its own 39 us) and by the products and the score and
 // exponential arithmetic on many (512 rows, 32 heads of 128, 101 us; prompt_tc.cu
 // takes over there).
 #include <algorithm>
@@ -322,43 +322,41 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
     }
     __syncthreads();
 
-    // 1. scores, 16 keys a warp; hidden ones carry the lowest score
+    // 1. scores, 16 keys x 32 rows a warp and turn; hidden ones carry the lowest score
     const bool q_wide = s.wide != 0;
     const int32_t* k = a.k + (uint64_t)p.begin * a.k_stride + p.g * a.head_dim;
     const uint32_t last_key = p.base + p.count - 1;
-    for (uint32_t t0 = 16 * warp; t0 < p.count; t0 += 16 * kPromptWarps) {
+    for (uint32_t u = warp; u / (NT / 4) * 16 < p.count; u += kPromptWarps) {
+      const uint32_t t0 = u / (NT / 4) * 16, nt0 = u % (NT / 4) * 4;
       const uint32_t ka = p.base + t0 + (lane >> 2), kb = ka + 8;
       const int32_t* pa = k + (uint64_t)min(ka, last_key) * a.k_stride;
       const int32_t* pb = k + (uint64_t)min(kb, last_key) * a.k_stride;
       // keys that every row sees
       const bool open = p.base + t0 + 15 <= q0 && (!a.window || p.base + t0 >= window_start(q1, a.window));
-#pragma unroll 1
-      for (uint32_t nt0 = 0; nt0 < NT; nt0 += 4) {
-        int32_t x[4][4];
-        key_scores<4>(pa, pb, tile, q_wide, nt0, lane, a.scale_q32, x);
-        int32_t* out = scores + (uint64_t)(8 * nt0 + 2 * (lane & 3)) * sc.pitch + t0 + (lane >> 2);
+      int32_t x[4][4];
+      key_scores<4>(pa, pb, tile, q_wide, nt0, lane, a.scale_q32, x);
+      int32_t* out = scores + (uint64_t)(8 * nt0 + 2 * (lane & 3)) * sc.pitch + t0 + (lane >> 2);
 #pragma unroll
-        for (uint32_t n = 0; n < 4; ++n)
+      for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
-          for (uint32_t e = 0; e < 4; ++e) {
-            if (!open) {
-              const int32_t q = s.query[8 * (nt0 + n) + 2 * (lane & 3) + (e & 1)];
-              const uint32_t key = e >> 1 ? kb : ka;
-              if (q < 0 || key > (uint32_t)q || key < window_start((uint32_t)q, a.window)) x[n][e] = INT32_MIN;
-            }
-            __stcg(out + (8 * n + (e & 1)) * sc.pitch + 8 * (e >> 1), x[n][e]);
+        for (uint32_t e = 0; e < 4; ++e) {
+          if (!open) {
+            const int32_t q = s.query[8 * (nt0 + n) + 2 * (lane & 3) + (e & 1)];
+            const uint32_t key = e >> 1 ? kb : ka;
+            if (q < 0 || key > (uint32_t)q || key < window_start((uint32_t)q, a.window)) x[n][e] = INT32_MIN;
           }
+          __stcg(out + (8 * n + (e & 1)) * sc.pitch + 8 * (e >> 1), x[n][e]);
+        }
 #pragma unroll
-        for (uint32_t n = 0; n < 4; ++n)
+      for (uint32_t n = 0; n < 4; ++n)
 #pragma unroll
-          for (uint32_t e = 0; e < 2; ++e) {
-            int32_t m = max(x[n][e], x[n][e + 2]);
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
-            m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            if (lane < 4) atomicMax(&s.top[8 * (nt0 + n) + 2 * lane + e], m);
-          }
-      }
+        for (uint32_t e = 0; e < 2; ++e) {
+          int32_t m = max(x[n][e], x[n][e + 2]);
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+          if (lane < 4) atomicMax(&s.top[8 * (nt0 + n) + 2 * lane + e], m);
+        }
     }
     __syncthreads();
 
@@ -366,18 +364,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
     // 16.0 of the lowest score that mark does not tell hidden keys, and the
     // causal range is asked again.
     const uint32_t written = (p.count + 15) / 16 * 16, padded = (p.count + 31) / 32 * 32;
+    int4 x[2];  // a row's first scores, loaded during the row before
+    row_load(x, scores + (uint64_t)warp * sc.pitch, 128, 0, written, lane);
     for (uint32_t i = warp; i < RT; i += kPromptWarps) {
       const int32_t top = s.top[i], q = s.query[i];
       int32_t* row = scores + (uint64_t)i * sc.pitch;
+      const int32_t* next = i + kPromptWarps < RT ? row + (uint64_t)kPromptWarps * sc.pitch : nullptr;
       uint64_t sum = 0;
       uint32_t first = UINT32_MAX;
       if (q >= 0 && top >= INT32_MIN + (1 << 20)) {
-        int4 x[2];
-        row_load(x, row, 128, 0, written, lane);
-        const RowTerms r = row_terms(row, 128, written, padded, top, lists + warp * kTermList, lane, x, nullptr);
+        const RowTerms r = row_terms(row, 128, written, padded, top, lists + warp * kTermList, lane, x, next);
         sum = r.sum;
         first = r.first;
-      } else if (q >= 0) {
+      } else if (next) {
+        row_load(x, next, 128, 0, written, lane);
+      }
+      if (q >= 0 && top < INT32_MIN + (1 << 20)) {
         for (uint32_t t = lane; t < padded; t += 32) {
           const uint32_t key = p.base + t;
           const bool gone = t >= p.count || key > (uint32_t)q || key < window_start((uint32_t)q, a.window);
@@ -392,11 +394,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
       __syncwarp();
       if (lane == 0) {
         s.sum[i] = sum;
-        s.recip[i] = sum_recip(sum);
         s.first[i] = first;
         if (q >= 0) __stcg(row + first, 0);  // its weight comes last
       }
     }
+    __syncwarp();
+    if (lane < RT / kPromptWarps) s.recip[warp + lane * kPromptWarps] = sum_recip(s.sum[warp + lane * kPromptWarps]);
     __syncthreads();
 
     // 3. weights and value sums
