@@ -541,6 +541,52 @@ def test_another_stream_and_a_captured_step(S):
     check(*again)
 
 
+def test_a_pool_of_more_than_32_bits_of_values(S):
+    """Pages past 2^32 values into the pools: appended, attended over and moved as in a small pool."""
+    import torch
+    rng = np.random.default_rng(31)
+    heads, kv_heads, d, page, pages = 16, 8, 128, 16, 270000  # 17.7 GB a pool
+    width = kv_heads * d
+    assert (pages - 1) * page * width > 1 << 32
+    free, _ = torch.cuda.mem_get_info()
+    if free < 45 << 30:
+        pytest.skip("needs 45 GB")
+    big_k, big_v = (torch.empty((pages, page, width), dtype=torch.int32, device="cuda") for _ in range(2))
+    for held, nodes in ((700, 1), (300, 6), (700, 12), (700, 40), (4200, 3)):
+        x = tree_inputs(rng, [held], [nodes], heads, kv_heads, d, page, "model", spare=0)
+        n = held + nodes
+        used = x["table"].shape[1]
+        ids = (pages - used + rng.permutation(used)).astype(np.int32)  # the pool's last pages
+        ids[0] = 3
+        rows = [int(x["table"][0, t // page]) * page + t % page for t in range(n)]
+        slots = np.array([int(ids[t // page]) * page + t % page for t in range(n)], np.int64)
+        k, v = (x[name].reshape(-1, width)[rows] for name in ("k_pages", "v_pages"))
+        S.page_append(cuda(k), cuda(v), cuda(slots), big_k, big_v)
+        args = [cuda(x[name]) for name in ("held", "offsets", "masks")]
+        small = S.tree_attention(cuda(x["q"]), cuda(x["k_pages"]), cuda(x["v_pages"]), cuda(x["table"]), *args, nodes, n,
+                                 heads=heads, kv_heads=kv_heads, scale_q32=scale_of(d))
+        large = S.tree_attention(cuda(x["q"]), big_k, big_v, cuda(ids[None]), *args, nodes, n, heads=heads,
+                                 kv_heads=kv_heads, scale_q32=scale_of(d))
+        assert torch.equal(small, large)
+        # every node accepted along its last path, in both pools
+        tokens = np.arange(nodes, dtype=np.int32)
+        picks = np.full(nodes, -5, np.int32)
+        at = nodes - 1
+        while x["parents"][at] >= 0:
+            picks[x["parents"][at]] = at
+            at = x["parents"][at]
+        pools = [cuda(x["k_pages"])[None], cuda(x["v_pages"])[None]]
+        for pk, pv, table in ((*pools, x["table"]), (big_k[None], big_v[None], ids[None])):
+            done = S.tree_accept(cuda(tokens), cuda(x["parents"]), cuda(picks), args[1], args[0], cuda(table), nodes,
+                                 k_pages=pk, v_pages=pv)
+        moved = int(done.held[0])
+        assert moved == held + bin(int(x["masks"][nodes - 1]) & (1 << 64) - 1).count("1")
+        for small_pool, big in zip(pools, (big_k, big_v)):
+            a = small_pool.view(-1, width)[torch.tensor(rows[:moved], device="cuda")]
+            b = big.view(-1, width)[torch.from_numpy(slots[:moved]).cuda()]
+            assert torch.equal(a, b)
+
+
 def test_no_wait_gave_up(S):
     """The bounded waits of every call above held; the check reports a status, not a leftover."""
     S.stall_check()
