@@ -281,11 +281,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
       if (lane >= d) incl += o;
     }
     few_tiles[lane] = incl - n;
-    if (lane == 31) few_tiles[32] = incl;
+    if (lane == 31) few_tiles[kFewRequests] = incl;
   }
   __syncthreads();
   const uint32_t* tiles = few ? few_tiles : sc.tiles;
-  const uint32_t items = (few ? few_tiles[32] : sc.tiles[a.requests]) * a.kv_heads;
+  const uint32_t items = (few ? few_tiles[kFewRequests] : sc.tiles[a.requests]) * a.kv_heads;
   for (uint32_t mine = blockIdx.x;; mine += gridDim.x) {
     __syncthreads();  // the tile before is done with the shared memory
     if (!few && tid == 0) s.item = atomicAdd(sc.next, 1u);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_mma_kernel(IrisPromp
     if (item >= items) return;
     PromptTile p;
     p.g = item % a.kv_heads;
-    const uint32_t at = item / a.kv_heads, rank = request_of(tiles, few ? 32u : a.requests, at);
+    const uint32_t at = item / a.kv_heads, rank = request_of(tiles, few ? kFewRequests : a.requests, at);
     const uint32_t r = few ? rank : sc.order[rank];
     p.begin = clamp_offset(a.offsets[r], a.tokens);
     p.len = min(clamp_offset(a.offsets[r + 1], a.tokens) - p.begin, a.longest);
