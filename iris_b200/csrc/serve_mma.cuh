@@ -134,19 +134,6 @@ __device__ __forceinline__ uint32_t key_products(const int32_t* k0, const int32_
   return wide;
 }
 
-// The score of a sum hi 2^32 + lo (serve_score), scale below 2^31: the sum
-// times the scale down 32 bits, then down 16 to nearest even, saturated where the
-// high word is past 16 bits. Half is added first (with the scale in one step); on a
-// tie that leaves 16 zeros, and the even neighbour has no low bit.
-template <bool kScaled>
-__device__ __forceinline__ int32_t score_by(int32_t hi, uint32_t lo, uint32_t scale) {
-  const uint64_t s = kScaled ? (uint64_t)((int64_t)hi * (int32_t)scale) + (__umulhi(lo, scale) + 0x8000u)
-                             : (((uint64_t)(uint32_t)hi << 32) | lo) + 0x8000;
-  const int32_t top = (int32_t)(s >> 32);
-  int32_t low = (int32_t)__funnelshift_r((uint32_t)s, (uint32_t)top, 16);
-  if (((uint32_t)s & 0xFFFFu) == 0) low &= ~1;
-  return (uint32_t)(top + 0x8000) < 0x10000u ? low : (top >> 31) ^ INT32_MAX;
-}
 __device__ __forceinline__ int32_t score_of(int32_t hi, uint32_t lo, uint32_t scale) {
   return scale ? score_by<true>(hi, lo, scale) : score_by<false>(hi, lo, scale);
 }

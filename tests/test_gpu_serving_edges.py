@@ -1,0 +1,56 @@
+"""The serving operators on the GPU at the edges of their ranges, against the
+plain 64-bit restatements (tests/serving_reference.py)."""
+import numpy as np
+import pytest
+
+import serving_reference as ref
+from test_gpu_serving import cuda, scale_of, tree_inputs, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def S():
+    from iris_b200 import build
+    build.build()
+    from iris_b200 import _lib, serving
+    assert _lib.lib().q8gpu_init() == 0, "no usable CUDA device"
+    return serving
+
+
+def run_tree(S, x, heads, kv_heads, scale, window, nodes, longest, out=None):
+    return S.tree_attention(*(cuda(x[n]) for n in ("q", "k_pages", "v_pages", "table", "held", "offsets", "masks")),
+                            nodes, longest, heads=heads, kv_heads=kv_heads, scale_q32=scale, window=window,
+                            positions=cuda(x["positions"]) if window else None, out=out).cpu().numpy()
+
+
+def tree_rows(x, heads, kv_heads, scale, window):
+    return ref.trees(x["q"], x["k_pages"], x["v_pages"], x["table"], x["held"], x["offsets"],
+                     [int(m) & (1 << 64) - 1 for m in x["masks"]], x["positions"], heads, kv_heads, scale, window)
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256, 36])
+def test_a_sum_at_the_top_of_64_bits_is_the_highest_score(S, d):
+    """A key whose unscaled sum is 2^63 - 1 among keys of small ones: its score is the highest there is."""
+    rng = np.random.default_rng(d)
+    heads, kv_heads = 2, 1
+    row = np.zeros(d, np.int32)
+    row[:3] = -2**31, -2**31, 2**31 - 1
+    best, other = np.zeros(d, np.int32), np.zeros(d, np.int32)
+    best[:3] = -2**31, -(2**31 - 1), 1
+    other[2] = 1
+    assert int((row.astype(object) * best.astype(object)).sum()) == 2**63 - 1
+    n = 90
+    q, k, v = np.tile(row, (n, heads)), np.tile(other, (n, 1)), values(rng, (n, d), "model")
+    k[0] = best
+    offsets = np.array([0, n], np.int32)
+    got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), n, heads=heads, kv_heads=kv_heads).cpu().numpy()
+    assert np.array_equal(got, ref.prompts(q, k, v, offsets, heads, kv_heads, 0, 0))
+    assert np.array_equal(got[-1], np.tile(v[0], heads))
+    for held, nodes in ((50, 1), (50, 9), (1500, 3), (400, 40)):  # in clusters, on mma.sync, on the tensor cores
+        x = tree_inputs(rng, [held], [nodes], heads, kv_heads, d, 16, "model")
+        x["q"][:] = np.tile(row, heads)
+        x["k_pages"][:] = other
+        x["k_pages"][x["table"][0, 1], 3] = best
+        got = run_tree(S, x, heads, kv_heads, 0, 0, nodes, held + nodes)
+        assert np.array_equal(got, tree_rows(x, heads, kv_heads, 0, 0)), (held, nodes)
