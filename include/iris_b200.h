@@ -515,7 +515,7 @@ int iris_page_append(const int32_t* d_k, const int32_t* d_v, uint64_t k_stride, 
  * its request's rows up to i, the last `window` of them where window is not 0.
  * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]
  * (a fused q|k|v row's parts may be passed with its stride). longest: no
- * request is longer. scale_q32: the score scale (mistral.rs:148-160), 0 for
+ * request is longer (more than tokens counts as tokens). scale_q32: the score scale (mistral.rs:148-160), 0 for
  * unscaled scores (gemma-dense). head_dim a multiple of 4, at most 256. */
 typedef struct {
   const int32_t *q, *k, *v;

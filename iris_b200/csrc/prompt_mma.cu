@@ -431,8 +431,8 @@ size_t carve(const IrisPromptAttention& a, uint8_t* base, PromptScratch* sc, Pro
   const uint32_t rt = row_tile(a), group = a.heads / a.kv_heads, most = on_tensor_cores(a) ? 64 : rt;
   const uint64_t tiles = ((uint64_t)a.tokens * group + rt - 1) / rt + a.requests;
   sc->blocks = (uint32_t)std::min<uint64_t>(tiles * a.kv_heads, (uint64_t)device_sms());
-  const uint32_t keys = a.window ? std::min<uint64_t>(a.longest, (uint64_t)a.window + most + 16) : a.longest;
-  sc->pitch = (keys + 15 + 127) / 128 * 128;  // a tile's first key is rounded down to 16, its last up to 128
+  const uint64_t keys = a.window ? std::min<uint64_t>(a.longest, (uint64_t)a.window + most + 16) : a.longest;
+  sc->pitch = (uint32_t)((keys + 15 + 127) / 128 * 128);  // a tile's first key is rounded down to 16, its last up to 128
   size_t at = 0;
   auto take = [&](size_t bytes) {
     uint8_t* p = base + at;

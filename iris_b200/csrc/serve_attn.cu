@@ -4,6 +4,8 @@
 // scores of mistral.rs:130-145 or the unscaled ones, and the weighted value
 // sums of tensor.rs:530-536), so a drafted or packed row equals the row that
 // decoding the same tokens one at a time gives, bit for bit.
+#include <algorithm>
+
 #include "../../include/iris_b200.h"
 #include "common.cuh"
 #include "layers.cuh"
@@ -187,6 +189,13 @@ int check_prompt(const IrisPromptAttention* a) {
   return 0;
 }
 
+// No request is longer than all rows together: a looser bound would choose
+// kernels and size the scratch for requests that cannot be.
+IrisPromptAttention bounded(IrisPromptAttention a) {
+  a.longest = std::min(a.longest, a.tokens);
+  return a;
+}
+
 int check_tree(const IrisTreeAttention* a) {
   if (!a || !heads_ok(a->heads, a->kv_heads, a->head_dim) || a->rows > (uint32_t)INT32_MAX) return IRIS_EINVAL;
   if (!a->rows) return 0;
@@ -209,17 +218,20 @@ using namespace iris;
 extern "C" {
 
 uint64_t iris_prompt_attention_workspace(const IrisPromptAttention* a) {
-  if (check_prompt(a) || !a->tokens || !prompt_mma_usable(*a)) return 0;
-  return prompt_mma_workspace(*a);
+  if (check_prompt(a) || !a->tokens) return 0;
+  const IrisPromptAttention b = bounded(*a);
+  return prompt_mma_usable(b) ? prompt_mma_workspace(b) : 0;
 }
 
 int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_t workspace_bytes, void* stream) {
   const int bad = check_prompt(a);
   if (bad || !a->tokens) return bad;
-  const uint64_t need = iris_prompt_attention_workspace(a);
+  const IrisPromptAttention b = bounded(*a);
+  const bool mma = prompt_mma_usable(b);
+  const uint64_t need = mma ? prompt_mma_workspace(b) : 0;
   if (need && (!aligned16(workspace) || workspace_bytes < need)) return IRIS_ESCRATCH;
-  if (prompt_mma_usable(*a)) return (int)launch_prompt_mma(*a, (uint8_t*)workspace, (cudaStream_t)stream);
-  prompt_rows_kernel<<<dim3(a->tokens, a->heads), kRowThreads, 0, (cudaStream_t)stream>>>(*a);
+  if (mma) return (int)launch_prompt_mma(b, (uint8_t*)workspace, (cudaStream_t)stream);
+  prompt_rows_kernel<<<dim3(b.tokens, b.heads), kRowThreads, 0, (cudaStream_t)stream>>>(b);
   return (int)cudaGetLastError();
 }
 

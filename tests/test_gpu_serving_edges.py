@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import serving_reference as ref
-from test_gpu_serving import cuda, scale_of, tree_inputs, values
+from test_gpu_serving import PROMPTS, cuda, scale_of, tree_inputs, values
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,43 @@ def test_a_sum_at_the_top_of_64_bits_is_the_highest_score(S, d):
         x["k_pages"][x["table"][0, 1], 3] = best
         got = run_tree(S, x, heads, kv_heads, 0, 0, nodes, held + nodes)
         assert np.array_equal(got, tree_rows(x, heads, kv_heads, 0, 0)), (held, nodes)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,d", [([5, 64, 300, 1], 8, 2, 128), ([130], 4, 1, 256), ([40, 3], 4, 2, 32),
+                                                      ([50, 90], 4, 2, 36)])
+def test_any_bound_on_the_prompts_gives_the_same_rows(S, lengths, heads, kv_heads, d):
+    rng = np.random.default_rng(d)
+    n = sum(lengths)
+    q, k, v = (values(rng, (n, w * d), "model") for w in (heads, kv_heads, kv_heads))
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    for window in (0, 24):
+        want = ref.prompts(q, k, v, offsets, heads, kv_heads, scale_of(d), window)
+        for longest in (max(lengths), n, n + 1, 20000, 1 << 31, 0xFFFFFF72, 0xFFFFFFFF):
+            got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), longest, heads=heads, kv_heads=kv_heads,
+                                     scale_q32=scale_of(d), window=window).cpu().numpy()
+            assert np.array_equal(got, want), (window, longest)
+
+
+@pytest.mark.parametrize("lengths,heads,kv_heads,d,scaled,window,kind",
+                         [c for c in PROMPTS if c[3] % 32 == 0 and sum(c[0]) < 500])
+def test_prompts_behind_a_long_one(S, lengths, heads, kv_heads, d, scaled, window, kind):
+    """With a request of 1,024 rows among them the others go through the tensor cores' tiles too."""
+    rng = np.random.default_rng(sum(lengths) + d + 2)
+    lengths = [*lengths[:1], 1024, *lengths[1:]]
+    n = sum(lengths)
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    scale = scale_of(d) if scaled else 0
+    for values_kind in ("model", "full" if kind == "full" else "wide"):
+        q, k = (values(rng, (n, w * d), kind) for w in (heads, kv_heads))
+        v = values(rng, (n, kv_heads * d), values_kind)
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 1024, heads=heads, kv_heads=kv_heads,
+                                 scale_q32=scale, window=window).cpu().numpy()
+        a, b = offsets[1], offsets[2]
+        short = np.r_[0:a, b:n]
+        at = np.concatenate([offsets[:2], offsets[3:] - 1024])
+        assert np.array_equal(got[short], ref.prompts(q[short], k[short], v[short], at, heads, kv_heads, scale, window))
+        for i in [0, 1, 63, 127, 128, 500, 1023]:
+            lo = a + (max(0, i + 1 - window) if window else 0)
+            for h in range(heads):
+                c, g = slice(h * d, (h + 1) * d), slice(h * kv_heads // heads * d, (h * kv_heads // heads + 1) * d)
+                assert np.array_equal(got[a + i, c], ref.attend(q[a + i, c], k[lo:a + i + 1, g], v[lo:a + i + 1, g], scale)), i

@@ -38,3 +38,28 @@ def test_scores_at_both_ends_of_the_sums(edges, scale):
     got, want = np.zeros(len(sums), np.int32), np.zeros(len(sums), np.int32)
     edges.edge_scores(at(sums), C.c_uint64(len(sums)), C.c_uint32(scale), at(got), at(want))
     assert np.array_equal(got, want)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from iris_b200 import build
+    build.build()
+    from iris_b200 import _lib
+    return _lib
+
+
+@pytest.mark.parametrize("tokens,heads,kv_heads,d,window", [
+    (1, 4, 1, 64, 0), (300, 4, 2, 128, 0), (300, 8, 1, 256, 96), (5000, 32, 8, 128, 0), (5000, 4, 2, 32, 17)])
+def test_a_loose_bound_on_the_prompts_needs_no_more_scratch(lib, tokens, heads, kv_heads, d, window):
+    """`longest` past the number of rows sizes the scratch as that number does, up to the last 32-bit one."""
+    a = 1 << 20
+
+    def need(longest):
+        p = lib.PromptAttention(a, a, a, a, a, heads * d, kv_heads * d, kv_heads * d, heads * d, 3, tokens, longest,
+                                heads, kv_heads, d, window, 1)
+        return lib.lib().iris_prompt_attention_workspace(C.byref(p))
+
+    rows = tokens + 15 if not window else min(tokens, window)
+    assert need(tokens) >= rows * 4
+    for longest in (tokens + 1, 1 << 31, 0xFFFFFF72, 0xFFFFFF80, 0xFFFFFFFF):
+        assert need(longest) == need(tokens), longest
