@@ -610,6 +610,10 @@ IRIS_HD bool softmax_weight_reaches(int64_t term, uint64_t sum, uint32_t c) {
   return c & 1 ? n_lo > lo : n_lo >= lo;
 }
 
+// A first maximum's place among `count` keys (1 or more), for reading its value:
+// inside them also where none was found (UINT32_MAX).
+IRIS_HD uint32_t place_within(uint32_t first, uint32_t count) { return first < count ? first : count - 1; }
+
 // ---- gemma-dense functions (ops.rs) -----------------------------------------
 
 // ops.rs:357-377 tanh_act

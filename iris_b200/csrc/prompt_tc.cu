@@ -158,6 +158,17 @@ struct PtShared {
 };
 
 __device__ __forceinline__ void epi_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kPtEpi) : "memory"); }
+// The same barrier, and whether `x` holds for every epilogue warp.
+__device__ __forceinline__ bool epi_all(bool x) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbar.red.and.pred q, 1, %2, p;\n\t"
+      "selp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(all)
+      : "r"((uint32_t)x), "n"(kPtEpi)
+      : "memory");
+  return all != 0;
+}
 
 // The terms of eight scores, 0 below kExpExactBelow, and their distances.
 __device__ __forceinline__ void terms_by_table(const int4 (&x)[2], int32_t top, const uint32_t* bits, uint32_t (&e)[8],
@@ -405,7 +416,10 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int32_t x = __reduce_max_sync(0xffffffffu, best[c]);
         if (lane == 0) atomicMax(&s.top[cg * 16 + c], x);
       }
-      epi_sync();
+      // After a give-up the scratch holds no scores, the maxima no places, and the
+      // queries' copies may still be landing under the lists: nothing more is done.
+      ok = epi_all(ok);
+      if (!ok) continue;
       // 2. terms in place, a row a warp (hidden keys: see prompt_mma.cu)
       const uint32_t padded = ktiles * kPtKeys;
       uint32_t* list = (uint32_t*)ops + warp * kPtList;  // (the query planes are done with)
@@ -563,7 +577,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (uint32_t c = 0; c < 16; ++c) {
           const uint32_t x = h * kPtD + 32 * quad + lane;
           vf[h][c] = cg * 16 + c < rows && x < a.head_dim
-                         ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * a.head_dim + x]
+                         ? a.v[(uint64_t)(k0 + place_within(s.first[cg * 16 + c], count)) * a.v_stride + g * a.head_dim + x]
                          : 0;
         }
       epi_sync();

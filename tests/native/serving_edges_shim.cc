@@ -12,4 +12,5 @@ void edge_scores(const int64_t* sum, uint64_t n, uint32_t scale, int32_t* got, i
     want[i] = scale ? iris::scaled_score_finish(sum[i], scale) : iris::requantize(sum[i]);
   }
 }
+uint32_t edge_place_within(uint32_t first, uint32_t count) { return iris::place_within(first, count); }
 }

@@ -63,3 +63,11 @@ def test_a_loose_bound_on_the_prompts_needs_no_more_scratch(lib, tokens, heads, 
     assert need(tokens) >= rows * 4
     for longest in (tokens + 1, 1 << 31, 0xFFFFFF72, 0xFFFFFF80, 0xFFFFFFFF):
         assert need(longest) == need(tokens), longest
+
+
+def test_a_place_that_was_not_found_is_read_inside_the_keys(edges):
+    """A row whose maximum was never found (a wait that gave up) has the place 2^32 - 1."""
+    for count in (1, 2, 127, 16256):
+        for first in (0, 1, count - 1, count, 0xFFFFFFFF):
+            got = edges.edge_place_within(C.c_uint32(first), C.c_uint32(count))
+            assert got == (first if first < count else count - 1)
