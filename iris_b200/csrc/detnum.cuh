@@ -435,9 +435,9 @@ IRIS_HD int32_t scaled_score_finish(int64_t sum, uint32_t scale_q32) {
 // 2^32 + lo in 32-bit halves, for scales of 1 to 2^31 - 1: the sum times the scale
 // down 32 bits, then down 16 to nearest even. Half is added first (with the scale
 // in one step); on a tie that leaves 16 zeros, and the even neighbour has no low
-// bit. Adding half to an unscaled sum within half of 2^63 turns its sign, so a score
-// past 32 bits takes its side from hi.
-template <bool kScaled>
+// bit. Adding half to an unscaled sum within half of 2^63 turns its sign: where
+// such sums can be (kAny), a score past 32 bits takes its side from hi.
+template <bool kScaled, bool kAny>
 IRIS_HD int32_t score_by(int32_t hi, uint32_t lo, uint32_t scale) {
 #if defined(__CUDA_ARCH__)
   const uint64_t s = kScaled ? (uint64_t)((int64_t)hi * (int32_t)scale) + (__umulhi(lo, scale) + 0x8000u)
@@ -450,7 +450,7 @@ IRIS_HD int32_t score_by(int32_t hi, uint32_t lo, uint32_t scale) {
 #endif
   const int32_t top = (int32_t)(uint32_t)(s >> 32);
   if (((uint32_t)s & 0xFFFFu) == 0) low &= ~1;
-  return (uint32_t)top + 0x8000u < 0x10000u ? low : (hi >> 31) ^ INT32_MAX;
+  return (uint32_t)top + 0x8000u < 0x10000u ? low : ((kAny && !kScaled ? hi : top) >> 31) ^ INT32_MAX;
 }
 
 // ---- softmax (ops.rs:233-276, 508-556) -------------------------------------

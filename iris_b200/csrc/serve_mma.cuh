@@ -134,17 +134,20 @@ __device__ __forceinline__ uint32_t key_products(const int32_t* k0, const int32_
   return wide;
 }
 
+// The score of a sum hi 2^32 + lo, by scale or without (0); sums of 24-bit
+// operands stay below 2^62.
+template <bool kAny = false>
 __device__ __forceinline__ int32_t score_of(int32_t hi, uint32_t lo, uint32_t scale) {
-  return scale ? score_by<true>(hi, lo, scale) : score_by<false>(hi, lo, scale);
+  return scale ? score_by<true, kAny>(hi, lo, scale) : score_by<false, kAny>(hi, lo, scale);
 }
 template <uint32_t N>
 __device__ __forceinline__ void scores_of(const int32_t (&hi)[N], const uint32_t (&lo)[N], uint32_t scale, int32_t (&y)[N]) {
   if (scale) {
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) y[i] = score_by<true>(hi[i], lo[i], scale);
+    for (uint32_t i = 0; i < N; ++i) y[i] = score_by<true, false>(hi[i], lo[i], scale);
   } else {
 #pragma unroll
-    for (uint32_t i = 0; i < N; ++i) y[i] = score_by<false>(hi[i], lo[i], scale);
+    for (uint32_t i = 0; i < N; ++i) y[i] = score_by<false, false>(hi[i], lo[i], scale);
   }
 }
 // Five diagonals: carried byte by byte, the low 32 bits from the bytes left behind.
@@ -164,7 +167,7 @@ __device__ __forceinline__ int32_t diagonal_score(const int32_t (&v)[7], uint32_
   uint64_t s = 0;
 #pragma unroll
   for (uint32_t d = 0; d < 7; ++d) s += (uint64_t)(int64_t)v[d] << (8 * d);
-  return score_of((int32_t)(s >> 32), (uint32_t)s, scale);
+  return score_of<true>((int32_t)(s >> 32), (uint32_t)s, scale);
 }
 
 template <uint32_t NT>

@@ -8,7 +8,7 @@ void edge_scores(const int64_t* sum, uint64_t n, uint32_t scale, int32_t* got, i
   for (uint64_t i = 0; i < n; ++i) {
     const int32_t hi = (int32_t)(uint32_t)((uint64_t)sum[i] >> 32);
     const uint32_t lo = (uint32_t)(uint64_t)sum[i];
-    got[i] = scale ? iris::score_by<true>(hi, lo, scale) : iris::score_by<false>(hi, lo, scale);
+    got[i] = scale ? iris::score_by<true, true>(hi, lo, scale) : iris::score_by<false, true>(hi, lo, scale);
     want[i] = scale ? iris::scaled_score_finish(sum[i], scale) : iris::requantize(sum[i]);
   }
 }
