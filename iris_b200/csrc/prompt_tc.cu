@@ -416,10 +416,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int32_t x = __reduce_max_sync(0xffffffffu, best[c]);
         if (lane == 0) atomicMax(&s.top[cg * 16 + c], x);
       }
-      // After a give-up the scratch holds no scores, the maxima no places, and the
-      // queries' copies may still be landing under the lists: nothing more is done.
+      // After a give-up the scratch holds no scores, and the queries' copies may still
+      // be landing under the lists: no row is worked on then.
       ok = epi_all(ok);
-      if (!ok) continue;
       // 2. terms in place, a row a warp (hidden keys: see prompt_mma.cu)
       const uint32_t padded = ktiles * kPtKeys;
       uint32_t* list = (uint32_t*)ops + warp * kPtList;  // (the query planes are done with)
@@ -433,7 +432,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       int4 x[2];
       load(x, scores + warp * kPtKeys, 0);
       for (uint32_t i = warp; i < kPtRows; i += kPtEpiWarps) {
-        const int32_t top = s.top[i], q = s.query[i];
+        const int32_t top = s.top[i], q = ok ? s.query[i] : -1;
         const bool ask = top < INT32_MIN + (1 << 20);
         int32_t* row = scores + i * kPtKeys;  // key t at (t / 128) blocks + t % 128
         uint64_t sum = 0;
@@ -505,7 +504,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         __syncwarp();
         if (lane == 0) {
           s.sum[i] = sum;
-          s.first[i] = first;
+          s.first[i] = place_within(first, count);
           if (q >= 0 && first < padded) __stcg(row + (first / kPtKeys) * kPtBlock + first % kPtKeys, 0);  // its weight comes last
         }
       }
@@ -576,8 +575,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
 #pragma unroll
         for (uint32_t c = 0; c < 16; ++c) {
           const uint32_t x = h * kPtD + 32 * quad + lane;
-          vf[h][c] = cg * 16 + c < rows && x < a.head_dim
-                         ? a.v[(uint64_t)(k0 + place_within(s.first[cg * 16 + c], count)) * a.v_stride + g * a.head_dim + x]
+          vf[h][c] = ok && cg * 16 + c < rows && x < a.head_dim
+                         ? a.v[(uint64_t)(k0 + s.first[cg * 16 + c]) * a.v_stride + g * a.head_dim + x]
                          : 0;
         }
       epi_sync();
