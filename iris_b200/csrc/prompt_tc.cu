@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kPackThreads) prompt_pack_kernel(IrisPromptAtt
 // ---- the attention ----------------------------------------------------------------
 
 struct PtShared {
-  uint64_t full[PtLayout<1>::kSlots], empty[PtLayout<1>::kSlots], q_full, s_done, t_free, w_full[2], w_empty[2], v_done;
+  uint64_t full[PtLayout<1>::kSlots], empty[PtLayout<1>::kSlots], q_full, s_done, t_free, w_full[2], w_empty[2], v_done, drained;
   uint64_t sum[kPtRows];
   int32_t top[kPtRows], query[kPtRows], wsum[kPtRows];
   uint32_t recip[kPtRows], first[kPtRows];
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&s.w_empty[i], 1);
     }
     mbar_init(&s.v_done, 1);
+    mbar_init(&s.drained, 1);
     s.dead = 0;
     s.wide = 0;
     mbar_fence_init();
@@ -612,10 +613,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     }
     __syncwarp();
   }
-  // every issued copy has landed before the block exits
-  if (warp == kPtEpiWarps && lane == 0)
+  // every issued copy has landed, and every product is done, before the block exits
+  if (warp == kPtEpiWarps && lane == 0) {
+    if (n_item) mbar_wait_bounded(&s.q_full, (n_item - 1) & 1, fault);
     for (uint32_t i = 0; i < kPtSlots; ++i)
       if (issued[i]) mbar_wait_bounded(&s.full[i], (issued[i] - 1) & 1, fault);
+  }
+  if (warp == kPtEpiWarps + 1 && s.dead) tc_drain(&s.drained, leader, fault);
   tc_fence_before();
   __syncthreads();
   if (warp == kPtEpiWarps) {

@@ -38,6 +38,14 @@ __device__ __forceinline__ void tc_commit_by(uint64_t* bar, bool leader) {
       "r"((uint32_t)leader)
       : "memory");
 }
+// After a give-up: waits, with a bound, until the products that this warp issued are
+// done (bar: initialised for one arrival, unused before), so that none runs on in
+// shared memory and accumulators that the block gives back.
+__device__ __forceinline__ void tc_drain(uint64_t* bar, bool leader, unsigned int* fault) {
+  tc_commit_by(bar, leader);
+  __syncwarp();
+  mbar_wait_bounded(bar, 0, fault);
+}
 // Shared-memory writes of this thread made visible to the tensor cores' reads.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -45,6 +45,7 @@ __device__ __forceinline__ uint8_t* aligned_1024(uint8_t* p) {
 }
 
 struct TtBlock {  // TMEM and its waits
+  uint64_t drained;
   uint32_t tmem, dead, wide;
 };
 
@@ -55,7 +56,9 @@ __device__ __forceinline__ void tt_alloc(TtBlock& s, uint32_t warp, uint32_t col
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
 }
-__device__ __forceinline__ void tt_free(const TtBlock& s, uint32_t warp, uint32_t cols) {
+// The last warp issued the products.
+__device__ __forceinline__ void tt_free(TtBlock& s, uint32_t warp, uint32_t cols, unsigned int* fault) {
+  if (warp == kTtWarps && s.dead) tc_drain(&s.drained, (threadIdx.x & 31) == 0, fault);
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -98,6 +101,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   if (tid == 0) {
     mbar_init(&s.ready, 1);
     mbar_init(&s.taken, kTtWarps);
+    mbar_init(&s.b.drained, 1);
     s.b.dead = 0;
     s.b.wide = 0;
     mbar_fence_init();
@@ -290,7 +294,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   __syncthreads();
   for (uint32_t i = tid; i < rows; i += kTtThreads) sc.chunk_max[s.row_at[i] / sc.pitch * sc.chunks + chunk] = s.top[i];
   if (tid == 0 && s.b.wide) atomicOr(sc.flags, 1u);
-  tt_free(s.b, warp, 512);
+  tt_free(s.b, warp, 512, fault);
 }
 
 // ---- values -----------------------------------------------------------------------
@@ -335,6 +339,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
     mbar_init(&s.done[1], 1);
     mbar_init(&s.full[0], kTtWarps);
     mbar_init(&s.full[1], kTtWarps);
+    mbar_init(&s.b.drained, 1);
     s.b.dead = 0;
     s.b.wide = 0;
     mbar_fence_init();
@@ -535,7 +540,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       }
     }
   }
-  tt_free(s.b, warp, 4 * RB);
+  tt_free(s.b, warp, 4 * RB, fault);
 }
 
 uint32_t scores_smem(uint32_t row_tiles) { return 1024 + 2 * 3 * kTtPlane + row_tiles * 3 * kTtQPlane; }
