@@ -209,6 +209,13 @@ int check_tree(const IrisTreeAttention* a) {
   return 0;
 }
 
+// Positions have 31 bits: a wider window hides nothing, and the kernels add a
+// window to an index in 32 bits.
+IrisTreeAttention bounded(IrisTreeAttention a) {
+  if (a.window > (uint32_t)INT32_MAX) a.window = 0;
+  return a;
+}
+
 }  // namespace
 
 }  // namespace iris
@@ -236,18 +243,21 @@ int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_
 }
 
 uint64_t iris_tree_attention_workspace(const IrisTreeAttention* a) {
-  if (check_tree(a) || !a->rows || !tree_mma_usable(*a) || tree_cluster_usable(*a)) return 0;
-  return tree_mma_workspace(*a);
+  if (check_tree(a) || !a->rows) return 0;
+  const IrisTreeAttention b = bounded(*a);
+  return tree_mma_usable(b) && !tree_cluster_usable(b) ? tree_mma_workspace(b) : 0;
 }
 
 int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t workspace_bytes, void* stream) {
   const int bad = check_tree(a);
   if (bad || !a->rows) return bad;
-  const uint64_t need = iris_tree_attention_workspace(a);
+  const IrisTreeAttention b = bounded(*a);
+  const bool mma = tree_mma_usable(b), cluster = mma && tree_cluster_usable(b);
+  const uint64_t need = mma && !cluster ? tree_mma_workspace(b) : 0;
   if (need && (!aligned16(workspace) || workspace_bytes < need)) return IRIS_ESCRATCH;
-  if (tree_mma_usable(*a) && tree_cluster_usable(*a)) return (int)launch_tree_cluster(*a, (cudaStream_t)stream);
-  if (tree_mma_usable(*a)) return (int)launch_tree_mma(*a, (uint8_t*)workspace, (cudaStream_t)stream);
-  tree_rows_kernel<<<dim3(a->rows, a->heads), kRowThreads, 0, (cudaStream_t)stream>>>(*a);
+  if (cluster) return (int)launch_tree_cluster(b, (cudaStream_t)stream);
+  if (mma) return (int)launch_tree_mma(b, (uint8_t*)workspace, (cudaStream_t)stream);
+  tree_rows_kernel<<<dim3(b.rows, b.heads), kRowThreads, 0, (cudaStream_t)stream>>>(b);
   return (int)cudaGetLastError();
 }
 

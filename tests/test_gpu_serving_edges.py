@@ -94,3 +94,22 @@ def test_prompts_behind_a_long_one(S, lengths, heads, kv_heads, d, scaled, windo
             for h in range(heads):
                 c, g = slice(h * d, (h + 1) * d), slice(h * kv_heads // heads * d, (h * kv_heads // heads + 1) * d)
                 assert np.array_equal(got[a + i, c], ref.attend(q[a + i, c], k[lo:a + i + 1, g], v[lo:a + i + 1, g], scale)), i
+
+
+@pytest.mark.parametrize("d", [36, 64, 128])
+def test_a_window_past_every_position_hides_nothing(S, d):
+    rng = np.random.default_rng(d)
+    heads, kv_heads = 4, 2
+    for held, nodes in (([50, 3], [5, 2]), ([1500], [4]), ([400], [40])):
+        x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model")
+        want = tree_rows(x, heads, kv_heads, scale_of(d), 0)
+        for window in ((1 << 31) - 1, 1 << 31, (1 << 32) - 600, (1 << 32) - 1):
+            got = run_tree(S, x, heads, kv_heads, scale_of(d), window, max(nodes), max(held) + max(nodes))
+            assert np.array_equal(got, want), (held, window)
+    q, k, v = (values(rng, (150, w * d), "model") for w in (heads, kv_heads, kv_heads))
+    offsets = np.array([0, 20, 150], np.int32)
+    want = ref.prompts(q, k, v, offsets, heads, kv_heads, scale_of(d), 0)
+    for window in (1 << 31, (1 << 32) - 1):
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 130, heads=heads, kv_heads=kv_heads,
+                                 scale_q32=scale_of(d), window=window).cpu().numpy()
+        assert np.array_equal(got, want), window
