@@ -69,7 +69,6 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
   const uint32_t r0 = min(a.requests, tid * per), r1 = min(a.requests, r0 + per);
   uint64_t tok = 0, pg = 0;
   for (uint32_t r = r0; r < r1; ++r) tok += off[r], pg += base[r];
-  if (tok > (uint64_t)INT32_MAX) bad |= IRIS_PLAN_LENGTH;  // (then the offsets wrap; they stay below the tokens)
   const unsigned long long sum = ((unsigned long long)(uint32_t)tok << 32) | (uint32_t)pg;
   unsigned long long incl = sum;
 #pragma unroll
@@ -78,8 +77,7 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     if (lane >= d) incl += o;
   }
   if (lane == 31) part[warp] = incl;
-  const uint32_t faults = (__syncthreads_or(bad & IRIS_PLAN_LENGTH) ? IRIS_PLAN_LENGTH : 0) |
-                          (__syncthreads_or(bad & IRIS_PLAN_WIDTH) ? IRIS_PLAN_WIDTH : 0);
+  __syncthreads();
   unsigned long long before = incl - sum;
   for (uint32_t w = 0; w < warp; ++w) before += part[w];
   uint32_t t0 = (uint32_t)(before >> 32), p0 = (uint32_t)before;
@@ -89,12 +87,16 @@ __global__ void __launch_bounds__(kPlanThreads) page_plan_kernel(PlanArgs a) {
     base[r] = p0;
     t0 += f;
     p0 += n;
+    // (a request brings less than 2^31 tokens: the first sum past 31 bits shows; the
+    // offsets wrap then, and what they index is checked all the same)
+    if (t0 > (uint32_t)INT32_MAX) bad |= IRIS_PLAN_LENGTH;
   }
   if (r1 == a.requests && (r0 < r1 || (a.requests == 0 && tid == 0))) {
     off[a.requests] = t0;
     base[a.requests] = p0;
   }
-  __syncthreads();
+  const uint32_t faults = (__syncthreads_or(bad & IRIS_PLAN_LENGTH) ? IRIS_PLAN_LENGTH : 0) |
+                          (__syncthreads_or(bad & IRIS_PLAN_WIDTH) ? IRIS_PLAN_WIDTH : 0);
   const uint32_t total = off[a.requests], pages = base[a.requests];
 
   if (blockIdx.x == 0 && tid == 0) {

@@ -113,3 +113,17 @@ def test_a_window_past_every_position_hides_nothing(S, d):
         got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 130, heads=heads, kv_heads=kv_heads,
                                  scale_q32=scale_of(d), window=window).cpu().numpy()
         assert np.array_equal(got, want), window
+
+
+@pytest.mark.parametrize("fresh,fault", [([1 << 22] * 1024, True), ([1 << 30] * 3, True), ([1 << 30, 1 << 30], True),
+                                         ([0, 1 << 30] * 600, True), ([1 << 30, (1 << 30) - 1], False),
+                                         ([(1 << 31) - 1], False)])
+def test_page_plan_tells_when_the_fresh_tokens_pass_31_bits(S, fresh, fault):
+    """A sum of 2^31 tokens or more, over one request's run or many, is a fault of lengths."""
+    from iris_b200 import _lib
+    n, page = len(fresh), 1 << 20
+    table = np.full((n, 2048), -1, np.int32)
+    plan = S.page_plan(cuda(np.zeros(n, np.int32)), cuda(np.array(fresh, np.int32)), cuda(table),
+                       cuda(np.arange(8192, dtype=np.int32)), page, 8)
+    assert bool(plan.faults() & _lib.PLAN_LENGTH) == fault
+    assert plan.faults() & _lib.PLAN_TOKENS or fault
