@@ -72,6 +72,7 @@ __global__ void __launch_bounds__(kTcThreads) tree_cluster_kernel(IrisTreeAttent
   const uint32_t padded = (count + 31) / 32 * 32;
   const int32_t* table = a.table + (size_t)r * a.width;
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
+  const uint32_t stand_in = stand_in_row(a, q, table);
   for (uint32_t i = tid; i < padded; i += kTcThreads) {
     const int64_t row = i < count ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
     row_s[i] = row < 0 ? UINT32_MAX : (uint32_t)row;
@@ -185,8 +186,7 @@ __global__ void __launch_bounds__(kTcThreads) tree_cluster_kernel(IrisTreeAttent
     s.recip[tid] = sum_recip(sum);
     s.at[tid] = first;
   }
-  // hidden keys' weights are 0, whatever row stands for them
-  for (uint32_t i = tid; i < padded; i += kTcThreads) row_s[i] = row_s[i] == UINT32_MAX ? 0 : row_s[i];
+  for (uint32_t i = tid; i < padded; i += kTcThreads) row_s[i] = row_s[i] == UINT32_MAX ? stand_in : row_s[i];
   __syncthreads();
   // weights, over the query fragments
   for (uint32_t u = warp; u < NT * (padded / 32); u += kTcWarps) {

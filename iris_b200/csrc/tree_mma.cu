@@ -355,9 +355,10 @@ __global__ void __launch_bounds__(kValueThreads, 1) tree_values_kernel(IrisTreeA
   if (f0 >= rows || key0 >= q.keys) return;
   const uint32_t count = min(sc.vchunk, (q.keys - key0 + 31) / 32 * 32);
   const int32_t* table = a.table + (size_t)r * a.width;
+  const uint32_t stand_in = stand_in_row(a, q, table);
   for (uint32_t i = tid; i < (count + kValueKeys - 1) / kValueKeys * kValueKeys; i += kValueThreads) {
     const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
-    row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
+    row_s[i] = row < 0 ? stand_in : (uint32_t)row;
   }
   if (tid == 0) s.wide = 0;
   if (!sc.flags) pdl_wait();
@@ -432,9 +433,10 @@ __global__ void __launch_bounds__(kTreeThreads, 2)
   if (!rows || key0 >= q.keys) return;
   const uint32_t count = min(sc.vchunk, (q.keys - key0 + 31) / 32 * 32), steps = count / 32;
   const int32_t* table = a.table + (size_t)r * a.width;
+  const uint32_t stand_in = stand_in_row(a, q, table);
   for (uint32_t i = tid; i < count; i += kTreeThreads) {
     const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
-    row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
+    row_s[i] = row < 0 ? stand_in : (uint32_t)row;
   }
   if (tid < R) wsum_s[tid] = 0;
   pdl_wait();

@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const uint32_t count = min(sc.chunk, q.keys - key0), kts = (count + kTtKeys - 1) / kTtKeys;
   const int32_t* table = a.table + (size_t)r * a.width;
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
+  const uint32_t stand_in = stand_in_row(a, q, table);
   const bool used = 4 * lane < a.head_dim;  // the lane's four dims
   const int4 none = make_int4(0, 0, 0, 0);
 
@@ -156,8 +157,7 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   };
   auto load_keys = [&](uint32_t kt) {
     const uint32_t at = key0 + kt * kTtKeys + warp * 8 + (lane & 7);
-    // hidden keys are masked: any row will do
-    const int64_t row = id_key < 0 || (uint64_t)id_key >= a.pages ? 0 : (int64_t)id_key * a.page_size + at % a.page_size;
+    const int64_t row = id_key < 0 || (uint64_t)id_key >= a.pages ? stand_in : (int64_t)id_key * a.page_size + at % a.page_size;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
       const int32_t* src = a.k_pages + (size_t)__shfl_sync(0xffffffffu, row, i) * kvd + g * a.head_dim;
@@ -306,7 +306,6 @@ struct TtValues {
   uint64_t full[2];  // a stage's values and weights are in shared memory
   uint64_t sum[RB];
   uint32_t recip[RB], first[RB], id[RB];  // id: the row's place in the scratch, UINT32_MAX past the last
-  int32_t wsum[RB];
   uint32_t last;
 };
 
@@ -330,9 +329,10 @@ __global__ void __launch_bounds__(kTtThreads, 1)
   const uint32_t count = min(sc.tc_vchunk, (q.keys - key0 + 31) / 32 * 32), stages = (count + kTtKeys - 1) / kTtKeys;
   const int32_t* table = a.table + (size_t)r * a.width;
   const size_t kvd = (size_t)a.kv_heads * a.head_dim;
+  const uint32_t stand_in = stand_in_row(a, q, table);
   for (uint32_t i = tid; i < stages * kTtKeys; i += kTtThreads) {
     const int64_t row = key0 + i < q.keys ? page_row(table, a.width, a.page_size, a.pages, key0 + i) : -1;
-    row_s[i] = row < 0 ? 0 : (uint32_t)row;  // a hidden key's weight is 0, whatever the row
+    row_s[i] = row < 0 ? stand_in : (uint32_t)row;
   }
   if (tid == 0) {
     mbar_init(&s.done[0], 1);
@@ -386,7 +386,6 @@ __global__ void __launch_bounds__(kTtThreads, 1)
       s.recip[i] = sum_recip(sum);
       s.first[i] = first;
       s.id[i] = id;
-      s.wsum[i] = 0;
     }
   }
   tc_fence_before();

@@ -60,6 +60,13 @@ struct TreeRequest {
   __device__ uint32_t head_of(uint32_t f, uint32_t g) const { return g * group + f - node_of(f) * group; }
 };
 
+// The pool row that is read for keys that are not there (past the request's end or
+// off its table; they are masked, and their weights 0): the row of the request's
+// last key, so that only rows the call names choose its arithmetic.
+__device__ __forceinline__ uint32_t stand_in_row(const IrisTreeAttention& a, const TreeRequest& q, const int32_t* table) {
+  return (uint32_t)max(page_row(table, a.width, a.page_size, a.pages, q.keys - 1), (int64_t)0);
+}
+
 // head_dim up to 128 and trees of enough rows.
 bool tree_tc_usable(const IrisTreeAttention& a);
 // The scores and the value sums; flags are cleared before, terms run between.

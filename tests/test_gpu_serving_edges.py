@@ -127,3 +127,36 @@ def test_page_plan_tells_when_the_fresh_tokens_pass_31_bits(S, fresh, fault):
                        cuda(np.arange(8192, dtype=np.int32)), page, 8)
     assert bool(plan.faults() & _lib.PLAN_LENGTH) == fault
     assert plan.faults() & _lib.PLAN_TOKENS or fault
+
+
+def test_pages_that_no_request_names_do_not_choose_the_path(S):
+    """Keys past a request's end and holes in its table stand for no row: values
+    past 24 bits in the pool's first page, which no table names, leave the call on
+    the tensor cores (the scratch's last words tell of such values)."""
+    import ctypes as C
+
+    import torch
+    from iris_b200 import _lib
+    rng = np.random.default_rng(7)
+    heads, kv_heads, d, held, nodes = 4, 1, 128, [500, 130], [40, 11]
+    x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model", holes=[(0, 2, -1), (0, 5, 1 << 20)])
+    x["v_pages"] = values(rng, x["k_pages"].shape, "model")
+    x["table"][x["table"] == 0] = x["k_pages"].shape[0] - 1  # page 0 is nobody's
+    for where, flags in (((), [0, 0]), (("k_pages",), [1, 0]), (("v_pages",), [0, 1]), (("q",), [1, 0])):
+        for name in ("k_pages", "v_pages"):
+            x[name][0] = 1 << 30
+        y = {n: a.copy() for n, a in x.items()}
+        for name in where:  # one wide value that the call does see
+            y[name].reshape(-1)[0 if name == "q" else int(x["table"][0, 1]) * 16 * d] = 1 << 28
+        dev = {n: cuda(a) for n, a in y.items()}
+        out = torch.empty((sum(nodes), heads * d), dtype=torch.int32, device="cuda")
+        a = _lib.TreeAttention(*(dev[n].data_ptr() for n in ("q", "k_pages", "v_pages", "table", "held", "offsets",
+                                                             "masks")), None, out.data_ptr(), heads * d, heads * d,
+                               y["k_pages"].shape[0], len(held), sum(nodes), y["table"].shape[1], 16, max(nodes),
+                               max(h + n for h, n in zip(held, nodes)), heads, kv_heads, d, 0, scale_of(d))
+        need = _lib.lib().iris_tree_attention_workspace(C.byref(a))
+        work = torch.empty(need, dtype=torch.uint8, device="cuda")
+        _lib.check(_lib.lib().iris_tree_attention(C.byref(a), work.data_ptr(), need,
+                                                  torch.cuda.current_stream().cuda_stream), "iris_tree_attention")
+        assert np.array_equal(out.cpu().numpy(), tree_rows(y, heads, kv_heads, scale_of(d), 0))
+        assert work[need - 256:need - 248].view(torch.int32).ne(0).int().tolist() == flags, where
