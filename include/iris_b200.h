@@ -465,7 +465,9 @@ int iris_softmax_exp_terms(uint32_t first, uint32_t count, uint64_t* out);
  * stages). With release != 0 another thread completes the wait and the call
  * returns 0; with release == 0 nothing does, the wait gives up after about a
  * second and the call returns IRIS_ESTALL, the device staying usable.
- * Synchronous; clears the library's fault word before and after. */
+ * Synchronous; clears the library's fault word before and after. Kinds 2 and 3
+ * are 0 and 1 with the give-up left standing for the calls that report one
+ * (each once: the next pass of a session, the next iris_stall_check). */
 int iris_wait_probe(int kind, int release);
 
 /* ---------------------------------------------------------------------------
@@ -573,7 +575,8 @@ int iris_tree_accept(const int32_t* d_tokens, const int32_t* d_parents, const in
 /* The attentions above wait for their own copies and products with a bound. A
  * wait that gave up (about a second) leaves that call's output rows undefined.
  * Waits for `stream`, then IRIS_ESTALL if any kernel of the library on the
- * current device gave up since the last check (which clears it), else 0. */
+ * current device gave up since the last such check, else 0. Sessions report
+ * their own kernels' give-ups besides, and neither takes them from the other. */
 int iris_stall_check(void* stream);
 
 /* Message for any status this library returns. */

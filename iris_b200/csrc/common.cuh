@@ -125,15 +125,21 @@ __device__ __forceinline__ bool mbar_try_wait_suspend(uint64_t* bar, uint32_t pa
       : "memory");
   return ok != 0;
 }
+// A device's fault word has a bit for each that asks it, and each clears its own:
+// the calls that wait for their kernels (sessions, ranges), which report what the
+// library's other kernels gave up, and the serving check, which reports any.
+constexpr unsigned int kGaveUpLibrary = 1, kGaveUpServing = 2, kGaveUp = kGaveUpLibrary | kGaveUpServing;
+
 // Waits for the phase of `bar` with the given parity to complete, giving up
 // after about one second; a give-up is recorded in *fault.
-__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, unsigned int* fault) {
+__device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity, unsigned int* fault,
+                                                  unsigned int bits = kGaveUp) {
   if (mbar_try_wait(bar, parity)) return true;
   const uint64_t t0 = global_ns();
   for (uint32_t i = 1;; ++i) {
     if (mbar_try_wait_suspend(bar, parity)) return true;
     if ((i & 15) == 0 && global_ns() - t0 > 1000000000ull) {
-      atomicOr(fault, 1u);
+      atomicOr(fault, bits);
       return false;
     }
   }

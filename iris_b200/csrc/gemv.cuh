@@ -553,7 +553,7 @@ __device__ __forceinline__ bool ring_wait(uint64_t* bar, uint32_t parity, unsign
     if ((i & 15) == 0) {
       if (*(volatile unsigned int*)fault) return false;
       if (global_ns() - t0 > 1000000000ull) {
-        atomicOr(fault, 1u);
+        atomicOr(fault, kGaveUp);
         return false;
       }
     }

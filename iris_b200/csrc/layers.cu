@@ -566,7 +566,7 @@ __device__ __forceinline__ void group_barrier(unsigned int* bar, unsigned int ta
         __nanosleep(32);
         if (ld_acquire_u32(bar) >= target) break;
         if ((i & 255) == 0 && global_ns() - t0 > 1000000000ull) {
-          if (fault) atomicOr(fault, 1u);
+          if (fault) atomicOr(fault, kGaveUp);
           break;
         }
       }

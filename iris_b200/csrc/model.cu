@@ -804,7 +804,7 @@ cudaError_t run_pass(IrisSession* s, uint32_t tokens, const uint32_t* ids_dev, c
 // IRIS_ESTALL when a kernel recorded a given-up wait since the last check.
 int check_fault() {
   uint32_t fault = 0;
-  cudaError_t e = take_device_fault(&fault);
+  cudaError_t e = take_device_fault(&fault, kGaveUpLibrary);
   if (e != cudaSuccess) return (int)e;
   return fault ? IRIS_ESTALL : 0;
 }

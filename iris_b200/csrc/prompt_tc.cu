@@ -615,9 +615,9 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   }
   // every issued copy has landed, and every product is done, before the block exits
   if (warp == kPtEpiWarps && lane == 0) {
-    if (n_item) mbar_wait_bounded(&s.q_full, (n_item - 1) & 1, fault);
+    if (n_item) mbar_wait_bounded(&s.q_full, (n_item - 1) & 1, fault, kGaveUpServing);
     for (uint32_t i = 0; i < kPtSlots; ++i)
-      if (issued[i]) mbar_wait_bounded(&s.full[i], (issued[i] - 1) & 1, fault);
+      if (issued[i]) mbar_wait_bounded(&s.full[i], (issued[i] - 1) & 1, fault, kGaveUpServing);
   }
   if (warp == kPtEpiWarps + 1 && s.dead) tc_drain(&s.drained, leader, fault);
   tc_fence_before();

@@ -486,11 +486,15 @@ unsigned int* device_fault_word() {
   return addr[dev];
 }
 
-cudaError_t take_device_fault(uint32_t* fault) {
-  uint32_t zero = 0;
+__global__ void clear_fault_kernel(unsigned int bits) { atomicAnd(&g_fault, ~bits); }
+
+cudaError_t take_device_fault(uint32_t* fault, uint32_t bits) {
   cudaError_t e = cudaMemcpyFromSymbol(fault, g_fault, sizeof(uint32_t));
-  if (e == cudaSuccess && *fault) e = cudaMemcpyToSymbol(g_fault, &zero, sizeof(uint32_t));
-  return e;
+  *fault = e == cudaSuccess ? *fault & bits : 0;
+  if (!*fault) return e;
+  clear_fault_kernel<<<1, 1>>>(*fault);
+  e = cudaGetLastError();
+  return e == cudaSuccess ? cudaStreamSynchronize(nullptr) : e;
 }
 
 // ---------------------------------------------------------------------------

@@ -177,9 +177,9 @@ __host__ __device__ inline unsigned long long best_key(int32_t v, uint32_t idx) 
   return ((unsigned long long)((uint32_t)v ^ 0x80000000u) << 32) | (0xFFFFFFFFu - idx);
 }
 
-// Non-zero once a kernel gave up a bounded wait (a stalled pipeline); read and
-// cleared by the host.
-cudaError_t take_device_fault(uint32_t* fault);
+// Non-zero once a kernel gave up a bounded wait (a stalled pipeline); read by the
+// host, which clears the bits that it takes (kGaveUpLibrary, kGaveUpServing).
+cudaError_t take_device_fault(uint32_t* fault, uint32_t bits);
 // Device address of that fault word (kernels of other files record into it);
 // looked up once per device, before any stream capture.
 unsigned int* device_fault_word();

@@ -264,7 +264,7 @@ int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t wo
 int iris_stall_check(void* stream) {
   uint32_t fault = 0;
   cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
-  if (e == cudaSuccess) e = take_device_fault(&fault);
+  if (e == cudaSuccess) e = take_device_fault(&fault, kGaveUpServing);
   if (e != cudaSuccess) return (int)e;
   return fault ? IRIS_ESTALL : 0;
 }

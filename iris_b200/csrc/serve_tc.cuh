@@ -17,7 +17,7 @@ __device__ __forceinline__ bool tc_wait(uint64_t* bar, uint32_t parity, uint32_t
     if (*(volatile uint32_t*)dead) return false;
     if (global_ns() - t0 > 1000000000ull) {
       *(volatile uint32_t*)dead = 1;
-      atomicOr(fault, 1u);
+      atomicOr(fault, kGaveUpServing);
       return false;
     }
   }
@@ -44,7 +44,7 @@ __device__ __forceinline__ void tc_commit_by(uint64_t* bar, bool leader) {
 __device__ __forceinline__ void tc_drain(uint64_t* bar, bool leader, unsigned int* fault) {
   tc_commit_by(bar, leader);
   __syncwarp();
-  mbar_wait_bounded(bar, 0, fault);
+  mbar_wait_bounded(bar, 0, fault, kGaveUpServing);
 }
 // Shared-memory writes of this thread made visible to the tensor cores' reads.
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }

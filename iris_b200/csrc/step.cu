@@ -78,7 +78,7 @@ __device__ __forceinline__ void step_poll(const unsigned int* ctr, unsigned int 
     if ((i & 63) == 0) {
       if (*(volatile unsigned int*)fault) return;
       if (global_ns() - t0 > 1000000000ull) {
-        atomicOr(fault, 1u);
+        atomicOr(fault, kGaveUp);
         return;
       }
     }
@@ -268,7 +268,7 @@ __device__ __forceinline__ void step_exchange(const StepArgs& A, uint32_t k, uin
       if ((i & 63) == 0) {
         if (*(volatile unsigned int*)A.fault) break;
         if (global_ns() - t0 > 1000000000ull) {
-          atomicOr(A.fault, 1u);
+          atomicOr(A.fault, kGaveUp);
           break;
         }
       }
@@ -324,7 +324,7 @@ __device__ __forceinline__ void step_finish(const StepArgs& A, uint32_t p, uint3
       const uint64_t t0 = global_ns();
       for (uint32_t i = 1; ld_acquire_sys(mine + 2 * j + 1) < epoch; ++i) {
         if ((i & 63) == 0 && ((*(volatile unsigned int*)A.fault) || global_ns() - t0 > 1000000000ull)) {
-          atomicOr(A.fault, 1u);
+          atomicOr(A.fault, kGaveUp);
           break;
         }
       }
@@ -381,7 +381,7 @@ __device__ __forceinline__ void group_gather(const unsigned long long* slots, ui
     if ((it & 15) == 0) {
       const bool give_up = *(volatile unsigned int*)fault || global_ns() - t0 > 1000000000ull;
       if (__any_sync(0xffffffffu, give_up)) {
-        if (lane == 0) atomicOr(fault, 1u);
+        if (lane == 0) atomicOr(fault, kGaveUp);
         break;
       }
     }
@@ -1026,22 +1026,24 @@ __global__ void wait_probe_kernel(int kind, int release, unsigned int* ctr, unsi
 
 extern "C" int iris_wait_probe(int kind, int release) {
   using namespace iris;
-  if (kind != 0 && kind != 1) return IRIS_EINVAL;
+  if (kind < 0 || kind > 3) return IRIS_EINVAL;
+  const bool keep = kind >= 2;
   uint32_t stale = 0;
-  cudaError_t e = take_device_fault(&stale);  // start from a clear fault word
+  cudaError_t e = take_device_fault(&stale, kGaveUp);  // start from a clear fault word
   unsigned int* fault = device_fault_word();
   if (e == cudaSuccess && !fault) e = cudaErrorInvalidDevice;
   unsigned int* ctr = nullptr;
   if (e == cudaSuccess) e = cudaMalloc((void**)&ctr, sizeof(unsigned int));
   if (e == cudaSuccess) e = cudaMemset(ctr, 0, sizeof(unsigned int));
   if (e == cudaSuccess) {
-    wait_probe_kernel<<<1, 64>>>(kind, release, ctr, fault);
+    wait_probe_kernel<<<1, 64>>>(kind & 1, release, ctr, fault);
     e = cudaGetLastError();
   }
   if (e == cudaSuccess) e = cudaDeviceSynchronize();
   if (ctr) cudaFree(ctr);
   uint32_t gave_up = 0;
-  if (e == cudaSuccess) e = take_device_fault(&gave_up);
+  if (e == cudaSuccess && keep) e = cudaMemcpy(&gave_up, fault, sizeof(gave_up), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && !keep) e = take_device_fault(&gave_up, kGaveUp);
   if (e != cudaSuccess) return (int)e;
   return gave_up ? IRIS_ESTALL : 0;
 }

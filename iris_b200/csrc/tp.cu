@@ -107,7 +107,7 @@ __global__ void tp_p2p_finish_kernel(TpExchange x, uint32_t rows, const int32_t*
       for (uint32_t i = 1;; ++i) {  // the flag is in this GPU's memory: a tight poll stays in L2
         if (ld_acquire_sys(f) >= epoch) break;
         if ((i & 255) == 0 && ns_now() - t0 > 1000000000ull) {
-          if (x.fault) atomicOr(x.fault, 1u);
+          if (x.fault) atomicOr(x.fault, kGaveUp);
           break;
         }
       }
