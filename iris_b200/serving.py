@@ -55,20 +55,21 @@ class Accepted(NamedTuple):
 
 
 def _refuse(x: torch.Tensor, name: str, dtype: torch.dtype, dim: int, what: str) -> None:
-    raise ValueError(f"{name}: a CUDA tensor of {dtype} with {dim} axes, {what}, is needed; "
-                     f"got {x.dtype} {tuple(x.shape)} on {x.device} with strides {x.stride()}")
+    raise ValueError(f"{name}: a CUDA tensor of {dtype} with {dim} axes, {what}, on the device of the call's first "
+                     f"tensor, is needed; got {x.dtype} {tuple(x.shape)} on {x.device} with strides {x.stride()}")
 
 
-def _rows(x: torch.Tensor, name: str) -> int:
-    """The address of int32 rows whose last axis is dense (rows may lie apart)."""
-    if x.dtype != torch.int32 or not x.is_cuda or x.dim() != 2 or (x.stride(1) != 1 and x.numel()):
+def _rows(x: torch.Tensor, name: str, dev: int) -> int:
+    """The address of int32 rows on device `dev` whose last axis is dense (rows may lie apart)."""
+    if (x.dtype != torch.int32 or dev < 0 or x.get_device() != dev or x.dim() != 2
+            or (x.stride(1) != 1 and x.numel())):
         _refuse(x, name, torch.int32, 2, "the last one dense")
     return x.data_ptr()
 
 
-def _dense(x: torch.Tensor, name: str, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
-    """The address of a contiguous tensor."""
-    if x.dtype != dtype or not x.is_cuda or x.dim() != dim or not x.is_contiguous():
+def _dense(x: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int32, dim: int = 1) -> int:
+    """The address of a contiguous tensor on device `dev`."""
+    if x.dtype != dtype or dev < 0 or x.get_device() != dev or x.dim() != dim or not x.is_contiguous():
         _refuse(x, name, dtype, dim, "contiguous")
     return x.data_ptr()
 
@@ -78,11 +79,10 @@ def _same(count: int, want: int, name: str) -> None:
         raise ValueError(f"{name}: {count} entries, expected {want}")
 
 
-def _stream(x: torch.Tensor) -> int:
-    """torch's current stream on the tensor's device, which has to be the current one."""
-    index = x.get_device()
+def _stream(index: int) -> int:
+    """torch's current stream on the tensors' device, which has to be the current one."""
     if index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors are on {x.device}, but cuda:{torch.cuda.current_device()} is the current device")
+        raise ValueError(f"tensors are on cuda:{index}, but cuda:{torch.cuda.current_device()} is the current device")
     return torch._C._cuda_getCurrentRawStream(index)
 
 
@@ -94,22 +94,24 @@ def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free
     least the fresh tokens). With `parents` (each drafted node's parent in its
     request, -1 for a root) the plan has the nodes' visibility masks and their
     positions count ancestors only."""
+    dev = held.get_device()
     requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
-    ph, pf = _dense(held, "held"), _dense(fresh, "fresh")
-    pt, pp = _dense(table, "table", dim=2), _dense(free_pages, "free_pages")
+    ph, pf = _dense(held, "held", dev), _dense(fresh, "fresh", dev)
+    pt, pp = _dense(table, "table", dev, dim=2), _dense(free_pages, "free_pages", dev)
     _same(fresh.numel(), requests, "fresh")
     _same(table.shape[0], requests, "table")
-    counts, offsets, positions = held.new_empty(4), held.new_empty(requests + 1), held.new_empty(tokens)
-    slots = torch.empty(tokens, dtype=torch.int64, device=held.device)
     masks, pa, pm = None, None, None
     if parents is not None:
         if parents.numel() < tokens:
             raise ValueError(f"parents: {parents.numel()} entries, expected {tokens}")
-        pa = _dense(parents, "parents")
+        pa = _dense(parents, "parents", dev)
+    counts, offsets, positions = held.new_empty(4), held.new_empty(requests + 1), held.new_empty(tokens)
+    slots = torch.empty(tokens, dtype=torch.int64, device=held.device)
+    if parents is not None:
         masks = slots.new_empty(tokens)
         pm = masks.data_ptr()
     check(lib().iris_page_plan(ph, pf, requests, page_size, pt, width, pp, n_free, pa, tokens, offsets.data_ptr(),
-                               slots.data_ptr(), positions.data_ptr(), pm, counts.data_ptr(), _stream(held)),
+                               slots.data_ptr(), positions.data_ptr(), pm, counts.data_ptr(), _stream(dev)),
           "iris_page_plan")
     return PagePlan(offsets, slots, positions, table, counts, masks)
 
@@ -119,14 +121,15 @@ def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
     """K and V rows [tokens][kv_dim] into the pools [pages][page_size][kv_dim]
     at their slots; a slot outside the pools (-1) skips its row."""
     tokens, kv_dim = k.shape
-    pk, pv, ps = _rows(k, "k"), _rows(v, "v"), _dense(slots, "slots", torch.int64)
-    ck, cv = _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
+    dev = k.get_device()
+    pk, pv, ps = _rows(k, "k", dev), _rows(v, "v", dev), _dense(slots, "slots", dev, torch.int64)
+    ck, cv = _dense(k_pages, "k_pages", dev, dim=3), _dense(v_pages, "v_pages", dev, dim=3)
     if v.shape != k.shape or k_pages.shape != v_pages.shape or k_pages.shape[2] != kv_dim:
         raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
                          f"{tuple(v_pages.shape)} do not match")
     _same(slots.numel(), tokens, "slots")
     check(lib().iris_page_append(pk, pv, k.stride(0), v.stride(0), tokens, kv_dim, ps, ck, cv,
-                                 k_pages.shape[0] * k_pages.shape[1], _stream(k)), "iris_page_append")
+                                 k_pages.shape[0] * k_pages.shape[1], _stream(dev)), "iris_page_append")
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -141,7 +144,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     request r's rows are offsets[r] .. offsets[r + 1] - 1, the longest request
     at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense)."""
     tokens = q.shape[0]
-    pq, pk, pv, po = _rows(q, "q"), _rows(k, "k"), _rows(v, "v"), _dense(offsets, "offsets")
+    dev = q.get_device()
+    pq, pk, pv, po = _rows(q, "q", dev), _rows(k, "k", dev), _rows(v, "v", dev), _dense(offsets, "offsets", dev)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
     dim = q.shape[1] // heads
@@ -151,13 +155,13 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         out = q.new_empty((tokens, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out"), q.stride(0), k.stride(0), v.stride(0),
+    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), q.stride(0), k.stride(0), v.stride(0),
                              out.stride(0), offsets.numel() - 1, tokens, longest, heads, kv_heads, dim, window,
                              scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_prompt_attention_workspace(ref), q.device)
     check(L.iris_prompt_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-                                  _stream(q)), "iris_prompt_attention")
+                                  _stream(dev)), "iris_prompt_attention")
     return out
 
 
@@ -171,10 +175,11 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     cached tokens and the nodes of its mask. `longest`: the most cached tokens
     and nodes a request has together. A node that sees nothing gives zeros."""
     rows, requests = q.shape[0], held.numel()
-    pq, ck, cv = _rows(q, "q"), _dense(k_pages, "k_pages", dim=3), _dense(v_pages, "v_pages", dim=3)
-    pt, ph, po = _dense(table, "table", dim=2), _dense(held, "held"), _dense(offsets, "offsets")
-    pm = _dense(masks, "masks", torch.int64)
-    pp = _dense(positions, "positions") if positions is not None else None
+    dev = q.get_device()
+    pq, ck, cv = _rows(q, "q", dev), _dense(k_pages, "k_pages", dev, dim=3), _dense(v_pages, "v_pages", dev, dim=3)
+    pt, ph, po = _dense(table, "table", dev, dim=2), _dense(held, "held", dev), _dense(offsets, "offsets", dev)
+    pm = _dense(masks, "masks", dev, torch.int64)
+    pp = _dense(positions, "positions", dev) if positions is not None else None
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
     dim = q.shape[1] // heads
@@ -189,13 +194,13 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         out = q.new_empty((rows, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out"), q.stride(0), out.stride(0),
+    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out", dev), q.stride(0), out.stride(0),
                            k_pages.shape[0], requests, rows, table.shape[1], k_pages.shape[1], nodes, longest, heads,
                            kv_heads, dim, window, scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_tree_attention_workspace(ref), q.device)
     check(L.iris_tree_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
-                                _stream(q)), "iris_tree_attention")
+                                _stream(dev)), "iris_tree_attention")
     return out
 
 
@@ -207,24 +212,25 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     [layers][pages][page_size][kv_dim], their K/V rows moved after the cached
     ones, in place, in every layer."""
     rows, requests = tokens.numel(), held.numel()
-    pt, pa, pk = _dense(tokens, "tokens"), _dense(parents, "parents"), _dense(picks, "picks")
-    po, ph, tb = _dense(offsets, "offsets"), _dense(held, "held"), _dense(table, "table", dim=2)
+    dev = tokens.get_device()
+    pt, pa, pk = _dense(tokens, "tokens", dev), _dense(parents, "parents", dev), _dense(picks, "picks", dev)
+    po, ph, tb = _dense(offsets, "offsets", dev), _dense(held, "held", dev), _dense(table, "table", dev, dim=2)
     _same(parents.numel(), rows, "parents")
     _same(picks.numel(), rows, "picks")
     _same(offsets.numel(), requests + 1, "offsets")
     _same(table.shape[0], requests, "table")
-    accepted, after, now = held.new_empty(requests), held.new_empty(requests), held.new_empty(requests)
-    path = held.new_empty((requests, path_width))
     layers, stride, pages, page, kv_dim, ck, cv = 0, 0, 0, 0, 0, None, None
     if k_pages is not None or v_pages is not None:
         if k_pages is None or v_pages is None or k_pages.shape != v_pages.shape:
             raise ValueError("k_pages and v_pages are given together, of one shape")
-        ck, cv = _dense(k_pages, "k_pages", dim=4), _dense(v_pages, "v_pages", dim=4)
+        ck, cv = _dense(k_pages, "k_pages", dev, dim=4), _dense(v_pages, "v_pages", dev, dim=4)
         layers, pages, page, kv_dim = k_pages.shape
         stride = pages * page * kv_dim
+    accepted, after, now = held.new_empty(requests), held.new_empty(requests), held.new_empty(requests)
+    path = held.new_empty((requests, path_width))
     check(lib().iris_tree_accept(pt, pa, pk, po, requests, rows, ph, path_width, path.data_ptr(), accepted.data_ptr(),
                                  after.data_ptr(), now.data_ptr(), tb, table.shape[1], page, ck, cv, layers, stride,
-                                 pages, kv_dim, _stream(held)), "iris_tree_accept")
+                                 pages, kv_dim, _stream(dev)), "iris_tree_accept")
     return Accepted(path, accepted, after, now)
 
 

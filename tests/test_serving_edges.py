@@ -71,3 +71,69 @@ def test_a_place_that_was_not_found_is_read_inside_the_keys(edges):
         for first in (0, 1, count - 1, count, 0xFFFFFFFF):
             got = edges.edge_place_within(C.c_uint32(first), C.c_uint32(count))
             assert got == (first if first < count else count - 1)
+
+
+class Fake:
+    """What the wrappers look at of a contiguous CUDA tensor, without one."""
+
+    def __init__(self, *shape, dtype=None, device=0):
+        import torch
+        self.shape, self.dtype, self.index = shape, dtype or torch.int32, device
+        self.is_cuda, self.device = True, f"cuda:{device}"
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def stride(self, axis=None):
+        strides = [int(np.prod(self.shape[i + 1:])) for i in range(len(self.shape))]
+        return strides if axis is None else strides[axis]
+
+    def is_contiguous(self):
+        return True
+
+    def get_device(self):
+        return self.index
+
+    def data_ptr(self):
+        return 1 << 20
+
+
+def fakes(name):
+    """A call's tensors, and the call."""
+    import torch
+    from iris_b200 import serving as S
+    i64 = torch.int64
+    return {
+        "plan": (dict(held=Fake(2), fresh=Fake(2), table=Fake(2, 3), free_pages=Fake(4), parents=Fake(8)),
+                 lambda t: S.page_plan(t["held"], t["fresh"], t["table"], t["free_pages"], 16, 8, parents=t["parents"])),
+        "append": (dict(k=Fake(3, 64), v=Fake(3, 64), slots=Fake(3, dtype=i64), k_pages=Fake(2, 16, 64),
+                        v_pages=Fake(2, 16, 64)), lambda t: S.page_append(*t.values())),
+        "prompt": (dict(q=Fake(3, 64), k=Fake(3, 64), v=Fake(3, 64), offsets=Fake(2), out=Fake(3, 64)),
+                   lambda t: S.prompt_attention(t["q"], t["k"], t["v"], t["offsets"], 3, heads=1, kv_heads=1,
+                                                out=t["out"])),
+        "tree": (dict(q=Fake(3, 64), k_pages=Fake(2, 16, 64), v_pages=Fake(2, 16, 64), table=Fake(1, 2), held=Fake(1),
+                      offsets=Fake(2), masks=Fake(3, dtype=i64), positions=Fake(3), out=Fake(3, 64)),
+                 lambda t: S.tree_attention(t["q"], t["k_pages"], t["v_pages"], t["table"], t["held"], t["offsets"],
+                                            t["masks"], 3, 9, heads=1, kv_heads=1, positions=t["positions"],
+                                            out=t["out"])),
+        "accept": (dict(tokens=Fake(3), parents=Fake(3), picks=Fake(3), offsets=Fake(2), held=Fake(1), table=Fake(1, 2),
+                        k_pages=Fake(2, 2, 16, 64), v_pages=Fake(2, 2, 16, 64)),
+                   lambda t: S.tree_accept(t["tokens"], t["parents"], t["picks"], t["offsets"], t["held"], t["table"], 3,
+                                           k_pages=t["k_pages"], v_pages=t["v_pages"])),
+    }[name]
+
+
+CALLS = ["plan", "append", "prompt", "tree", "accept"]
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_the_wrappers_refuse_tensors_of_two_devices(call):
+    names = list(fakes(call)[0])
+    for name in names[1:]:
+        tensors, run = fakes(call)
+        tensors[name].index = 1
+        with pytest.raises(ValueError, match=f"^{name}: "):
+            run(tensors)
