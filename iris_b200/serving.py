@@ -79,6 +79,13 @@ def _same(count: int, want: int, name: str) -> None:
         raise ValueError(f"{name}: {count} entries, expected {want}")
 
 
+def _ranges(**values: int) -> None:
+    """Refuses what is no 32-bit count (ctypes would cut it to one)."""
+    for name, value in values.items():
+        if not 0 <= value < 1 << 32:
+            raise ValueError(f"{name}: {value} is not between 0 and 2^32 - 1")
+
+
 def _stream(index: int) -> int:
     """torch's current stream on the tensors' device, which has to be the current one."""
     if index != torch._C._cuda_getDevice():
@@ -98,6 +105,8 @@ def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free
     requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
     ph, pf = _dense(held, "held", dev), _dense(fresh, "fresh", dev)
     pt, pp = _dense(table, "table", dev, dim=2), _dense(free_pages, "free_pages", dev)
+    if (page_size | tokens) >> 32:
+        _ranges(page_size=page_size, tokens=tokens)
     _same(fresh.numel(), requests, "fresh")
     _same(table.shape[0], requests, "table")
     masks, pa, pm = None, None, None
@@ -146,6 +155,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     tokens = q.shape[0]
     dev = q.get_device()
     pq, pk, pv, po = _rows(q, "q", dev), _rows(k, "k", dev), _rows(v, "v", dev), _dense(offsets, "offsets", dev)
+    requests = offsets.numel() - 1
+    if (requests | longest | heads | kv_heads | window | scale_q32) >> 32:
+        _ranges(requests=requests, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
     dim = q.shape[1] // heads
@@ -156,7 +168,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
     a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), q.stride(0), k.stride(0), v.stride(0),
-                             out.stride(0), offsets.numel() - 1, tokens, longest, heads, kv_heads, dim, window,
+                             out.stride(0), requests, tokens, longest, heads, kv_heads, dim, window,
                              scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_prompt_attention_workspace(ref), q.device)
@@ -180,6 +192,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     pt, ph, po = _dense(table, "table", dev, dim=2), _dense(held, "held", dev), _dense(offsets, "offsets", dev)
     pm = _dense(masks, "masks", dev, torch.int64)
     pp = _dense(positions, "positions", dev) if positions is not None else None
+    if (nodes | longest | heads | kv_heads | window | scale_q32) >> 32:
+        _ranges(nodes=nodes, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
     dim = q.shape[1] // heads
@@ -215,6 +229,8 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     dev = tokens.get_device()
     pt, pa, pk = _dense(tokens, "tokens", dev), _dense(parents, "parents", dev), _dense(picks, "picks", dev)
     po, ph, tb = _dense(offsets, "offsets", dev), _dense(held, "held", dev), _dense(table, "table", dev, dim=2)
+    if path_width >> 32:
+        _ranges(path_width=path_width)
     _same(parents.numel(), rows, "parents")
     _same(picks.numel(), rows, "picks")
     _same(offsets.numel(), requests + 1, "offsets")

@@ -137,3 +137,28 @@ def test_the_wrappers_refuse_tensors_of_two_devices(call):
         tensors[name].index = 1
         with pytest.raises(ValueError, match=f"^{name}: "):
             run(tensors)
+
+
+@pytest.mark.parametrize("call,name", [
+    ("prompt", "longest"), ("prompt", "heads"), ("prompt", "kv_heads"), ("prompt", "window"), ("prompt", "scale_q32"),
+    ("tree", "nodes"), ("tree", "longest"), ("tree", "heads"), ("tree", "kv_heads"), ("tree", "window"),
+    ("tree", "scale_q32"), ("plan", "page_size"), ("plan", "tokens"), ("accept", "path_width")])
+def test_the_wrappers_refuse_numbers_that_are_no_32_bit_counts(call, name):
+    """Numbers past 32 bits, and negative ones, are not cut to some other count."""
+    from iris_b200 import serving as S
+    t, _ = fakes(call)
+    numbers = dict(prompt=dict(longest=3, heads=1, kv_heads=1, window=0, scale_q32=0),
+                   tree=dict(nodes=3, longest=9, heads=1, kv_heads=1, window=0, scale_q32=0),
+                   plan=dict(page_size=16, tokens=8), accept=dict(path_width=3))[call]
+    for bad in (-1, 1 << 32, (1 << 32) + numbers[name], -(1 << 40)):
+        with pytest.raises(ValueError, match=f"^{name}: .*2\\^32"):
+            run = dict(prompt=S.prompt_attention, tree=S.tree_attention, plan=S.page_plan, accept=S.tree_accept)[call]
+            run(**t, **{**numbers, name: bad})
+
+
+def test_offsets_have_an_end():
+    from iris_b200 import serving as S
+    t, _ = fakes("prompt")
+    t["offsets"] = Fake(0)
+    with pytest.raises(ValueError, match="^requests: -1"):
+        S.prompt_attention(**t, longest=3, heads=1, kv_heads=1)
