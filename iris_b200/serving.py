@@ -74,6 +74,11 @@ def _dense(x: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int3
     return x.data_ptr()
 
 
+def _stride(x: torch.Tensor) -> int:
+    """The values between two rows; of a single row torch may give any."""
+    return x.stride(0) if x.shape[0] != 1 else x.shape[1]
+
+
 def _same(count: int, want: int, name: str) -> None:
     if count != want:
         raise ValueError(f"{name}: {count} entries, expected {want}")
@@ -137,7 +142,7 @@ def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
         raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
                          f"{tuple(v_pages.shape)} do not match")
     _same(slots.numel(), tokens, "slots")
-    check(lib().iris_page_append(pk, pv, k.stride(0), v.stride(0), tokens, kv_dim, ps, ck, cv,
+    check(lib().iris_page_append(pk, pv, _stride(k), _stride(v), tokens, kv_dim, ps, ck, cv,
                                  k_pages.shape[0] * k_pages.shape[1], _stream(dev)), "iris_page_append")
 
 
@@ -167,8 +172,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         out = q.new_empty((tokens, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), q.stride(0), k.stride(0), v.stride(0),
-                             out.stride(0), requests, tokens, longest, heads, kv_heads, dim, window,
+    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), _stride(q), _stride(k), _stride(v),
+                             _stride(out), requests, tokens, longest, heads, kv_heads, dim, window,
                              scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_prompt_attention_workspace(ref), q.device)
@@ -208,7 +213,7 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         out = q.new_empty((rows, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out", dev), q.stride(0), out.stride(0),
+    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out", dev), _stride(q), _stride(out),
                            k_pages.shape[0], requests, rows, table.shape[1], k_pages.shape[1], nodes, longest, heads,
                            kv_heads, dim, window, scale_q32)
     L, ref = lib(), C.byref(a)

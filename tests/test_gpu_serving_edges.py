@@ -160,3 +160,29 @@ def test_pages_that_no_request_names_do_not_choose_the_path(S):
                                                   torch.cuda.current_stream().cuda_stream), "iris_tree_attention")
         assert np.array_equal(out.cpu().numpy(), tree_rows(y, heads, kv_heads, scale_of(d), 0))
         assert work[need - 256:need - 248].view(torch.int32).ne(0).int().tolist() == flags, where
+
+
+def test_a_single_row_of_any_stride(S):
+    """One row has no distance to the next: torch's number for it may be 1, or anything."""
+    import torch
+    rng = np.random.default_rng(1)
+    heads, kv_heads, d = 4, 2, 64
+
+    def one(width):
+        x = values(rng, (1, width), "model")
+        return x, cuda(x.reshape(-1, 1)).t()  # strides (1, 1)
+
+    (q, dq), (k, dk), (v, dv) = one(heads * d), one(kv_heads * d), one(kv_heads * d)
+    out = torch.zeros(heads * d, 1, dtype=torch.int32, device="cuda").t()
+    assert dq.stride() == out.stride() == (1, 1)
+    offsets = np.array([0, 1], np.int32)
+    S.prompt_attention(dq, dk, dv, cuda(offsets), 1, heads=heads, kv_heads=kv_heads, out=out)
+    assert np.array_equal(out.cpu().numpy(), ref.prompts(q, k, v, offsets, heads, kv_heads, 0, 0))
+    pools = [torch.zeros((1, 16, kv_heads * d), dtype=torch.int32, device="cuda") for _ in range(2)]
+    S.page_append(dk, dv, cuda(np.array([5])), *pools)
+    assert np.array_equal(pools[0][0, 5].cpu().numpy(), k[0]) and np.array_equal(pools[1][0, 5].cpu().numpy(), v[0])
+    pools[0][0, 0], pools[1][0, 0] = dk[0], dv[0]
+    out.zero_()
+    S.tree_attention(dq, *pools, cuda(np.zeros((1, 1), np.int32)), cuda(np.zeros(1, np.int32)), cuda(offsets),
+                     cuda(np.ones(1, np.int64)), 1, 1, heads=heads, kv_heads=kv_heads, out=out)
+    assert np.array_equal(out.cpu().numpy(), ref.prompts(q, k, v, offsets, heads, kv_heads, 0, 0))
