@@ -107,9 +107,9 @@ def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free
     request, -1 for a root) the plan has the nodes' visibility masks and their
     positions count ancestors only."""
     dev = held.get_device()
-    requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
     ph, pf = _dense(held, "held", dev), _dense(fresh, "fresh", dev)
     pt, pp = _dense(table, "table", dev, dim=2), _dense(free_pages, "free_pages", dev)
+    requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
     if (page_size | tokens) >> 32:
         _ranges(page_size=page_size, tokens=tokens)
     _same(fresh.numel(), requests, "fresh")
@@ -134,10 +134,10 @@ def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
                 v_pages: torch.Tensor) -> None:
     """K and V rows [tokens][kv_dim] into the pools [pages][page_size][kv_dim]
     at their slots; a slot outside the pools (-1) skips its row."""
-    tokens, kv_dim = k.shape
     dev = k.get_device()
     pk, pv, ps = _rows(k, "k", dev), _rows(v, "v", dev), _dense(slots, "slots", dev, torch.int64)
     ck, cv = _dense(k_pages, "k_pages", dev, dim=3), _dense(v_pages, "v_pages", dev, dim=3)
+    tokens, kv_dim = k.shape
     if v.shape != k.shape or k_pages.shape != v_pages.shape or k_pages.shape[2] != kv_dim:
         raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
                          f"{tuple(v_pages.shape)} do not match")
@@ -157,10 +157,9 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     [tokens][kv_heads * head_dim] (rows may be parts of a fused q|k|v row);
     request r's rows are offsets[r] .. offsets[r + 1] - 1, the longest request
     at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense)."""
-    tokens = q.shape[0]
     dev = q.get_device()
     pq, pk, pv, po = _rows(q, "q", dev), _rows(k, "k", dev), _rows(v, "v", dev), _dense(offsets, "offsets", dev)
-    requests = offsets.numel() - 1
+    tokens, requests = q.shape[0], offsets.numel() - 1
     if (requests | longest | heads | kv_heads | window | scale_q32) >> 32:
         _ranges(requests=requests, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
@@ -191,12 +190,12 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     .. offsets[r + 1] - 1 (at most `nodes` each), a node seeing the held[r]
     cached tokens and the nodes of its mask. `longest`: the most cached tokens
     and nodes a request has together. A node that sees nothing gives zeros."""
-    rows, requests = q.shape[0], held.numel()
     dev = q.get_device()
     pq, ck, cv = _rows(q, "q", dev), _dense(k_pages, "k_pages", dev, dim=3), _dense(v_pages, "v_pages", dev, dim=3)
     pt, ph, po = _dense(table, "table", dev, dim=2), _dense(held, "held", dev), _dense(offsets, "offsets", dev)
     pm = _dense(masks, "masks", dev, torch.int64)
     pp = _dense(positions, "positions", dev) if positions is not None else None
+    rows, requests = q.shape[0], held.numel()
     if (nodes | longest | heads | kv_heads | window | scale_q32) >> 32:
         _ranges(nodes=nodes, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:

@@ -162,3 +162,16 @@ def test_offsets_have_an_end():
     t["offsets"] = Fake(0)
     with pytest.raises(ValueError, match="^requests: -1"):
         S.prompt_attention(**t, longest=3, heads=1, kv_heads=1)
+
+
+@pytest.mark.parametrize("call", CALLS)
+@pytest.mark.parametrize("shape", [(), (3,), (1, 2), (1, 2, 16, 64), (0,)])
+def test_the_wrappers_name_the_tensor_of_a_wrong_shape(call, shape):
+    """A tensor with other axes than the call's is refused by its name, whatever they are."""
+    for name, x in fakes(call)[0].items():
+        if len(shape) == len(x.shape):
+            continue
+        tensors, run = fakes(call)
+        tensors[name] = Fake(*shape, dtype=x.dtype)
+        with pytest.raises(ValueError, match=name):
+            run(tensors)
