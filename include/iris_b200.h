@@ -513,8 +513,9 @@ int iris_page_append(const int32_t* d_k, const int32_t* d_v, uint64_t k_stride, 
                      uint32_t kv_dim, const int64_t* d_slots, int32_t* d_k_pages, int32_t* d_v_pages,
                      uint64_t pool_rows, void* stream);
 /* Causal attention of packed prompts: row i of request r (rows offsets[r] ..
- * offsets[r + 1] - 1, offsets[0] = 0, offsets[requests] = tokens) attends over
- * its request's rows up to i, the last `window` of them where window is not 0.
+ * offsets[r + 1] - 1, offsets[0] = 0, offsets[requests] at most tokens) attends
+ * over its request's rows up to i, the last `window` of them where window is not
+ * 0. Rows of out past the last request's are not written.
  * q and out [tokens][heads][head_dim], k and v [tokens][kv_heads][head_dim]
  * (a fused q|k|v row's parts may be passed with its stride). longest: no
  * request is longer (more than tokens counts as tokens). scale_q32: the score scale (mistral.rs:148-160), 0 for
@@ -536,10 +537,11 @@ int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_
 /* Attention of drafted trees over the paged cache (K/V of the nodes appended
  * already): request r's nodes are the packed rows offsets[r] .. offsets[r + 1]
  * - 1, at most `nodes` <= 64 of them; a node sees the held[r] cached tokens
- * and the nodes of its mask. With a window, only keys at positions above its own less the window
- * (positions: of the nodes, required then). A node that sees no key gives
- * zeros. longest: no request has more cached tokens and nodes together; at
- * most width * page_size. One node a request whose mask is 1 is plain decoding. */
+ * and the nodes of its mask. With a window, only keys at positions above its
+ * own less the window (positions: of the nodes, required then). A node that sees
+ * no key gives zeros; rows of out past the last request's nodes are not written.
+ * longest: no request has more cached tokens and nodes together; at most width *
+ * page_size. One node a request whose mask is 1 is plain decoding. */
 typedef struct {
   const int32_t* q;
   const int32_t *k_pages, *v_pages;

@@ -149,7 +149,8 @@ __device__ void attend_row(const Keys& keys, const int32_t* q, int32_t* out, uin
 __global__ void __launch_bounds__(kRowThreads) prompt_rows_kernel(IrisPromptAttention a) {
   const uint32_t i = blockIdx.x, h = blockIdx.y;
   const uint32_t r = request_of(a.offsets, a.requests, i);
-  const uint32_t begin = clamp_offset(a.offsets[r], i);
+  const uint32_t begin = clamp_offset(a.offsets[r], a.tokens), end = clamp_offset(a.offsets[r + 1], a.tokens);
+  if (i < begin || i >= end) return;  // of no request
   const uint32_t at = i - begin, lo = window_start(at, a.window);
   const PackedKeys keys{a.k, a.v, a.k_stride, a.v_stride, begin + lo, at + 1 - lo};
   attend_row(keys, a.q + (uint64_t)i * a.q_stride + h * a.head_dim, a.out + (uint64_t)i * a.out_stride + h * a.head_dim,
@@ -159,8 +160,9 @@ __global__ void __launch_bounds__(kRowThreads) prompt_rows_kernel(IrisPromptAtte
 __global__ void __launch_bounds__(kRowThreads) tree_rows_kernel(IrisTreeAttention a) {
   const uint32_t i = blockIdx.x, h = blockIdx.y;
   const uint32_t r = request_of(a.offsets, a.requests, i);
-  const uint32_t begin = clamp_offset(a.offsets[r], i), end = clamp_offset(a.offsets[r + 1], a.rows);
-  const uint32_t held = tree_held(a, r), nodes = end > begin ? min(end - begin, kTreeNodes) : 0;
+  const uint32_t begin = clamp_offset(a.offsets[r], a.rows), end = clamp_offset(a.offsets[r + 1], a.rows);
+  if (i < begin || i >= end) return;  // of no request
+  const uint32_t held = tree_held(a, r), nodes = min(end - begin, kTreeNodes);
   const uint32_t position = a.positions ? (uint32_t)a.positions[i] : 0;
   PagedKeys keys{a.k_pages, a.v_pages, (uint64_t)a.kv_heads * a.head_dim, (uint64_t)a.kv_heads * a.head_dim,
                  a.table + (uint64_t)r * a.width, a.positions ? a.positions + begin : nullptr, a.pages,

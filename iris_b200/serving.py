@@ -156,7 +156,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     """Causal attention of packed prompts: q [tokens][heads * head_dim], k and v
     [tokens][kv_heads * head_dim] (rows may be parts of a fused q|k|v row);
     request r's rows are offsets[r] .. offsets[r + 1] - 1, the longest request
-    at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense)."""
+    at most `longest` rows. scale_q32 0: unscaled scores (gemma-dense). Rows past
+    the last request's are left as `out` has them (undefined without it)."""
     dev = q.get_device()
     pq, pk, pv, po = _rows(q, "q", dev), _rows(k, "k", dev), _rows(v, "v", dev), _dense(offsets, "offsets", dev)
     tokens, requests = q.shape[0], offsets.numel() - 1
@@ -189,7 +190,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     already: q [rows][heads * head_dim], request r's nodes the rows offsets[r]
     .. offsets[r + 1] - 1 (at most `nodes` each), a node seeing the held[r]
     cached tokens and the nodes of its mask. `longest`: the most cached tokens
-    and nodes a request has together. A node that sees nothing gives zeros."""
+    and nodes a request has together. A node that sees nothing gives zeros; rows
+    past the last request's nodes are left as `out` has them (undefined without it)."""
     dev = q.get_device()
     pq, ck, cv = _rows(q, "q", dev), _dense(k_pages, "k_pages", dev, dim=3), _dense(v_pages, "v_pages", dev, dim=3)
     pt, ph, po = _dense(table, "table", dev, dim=2), _dense(held, "held", dev), _dense(offsets, "offsets", dev)

@@ -186,3 +186,28 @@ def test_a_single_row_of_any_stride(S):
     S.tree_attention(dq, *pools, cuda(np.zeros((1, 1), np.int32)), cuda(np.zeros(1, np.int32)), cuda(offsets),
                      cuda(np.ones(1, np.int64)), 1, 1, heads=heads, kv_heads=kv_heads, out=out)
     assert np.array_equal(out.cpu().numpy(), ref.prompts(q, k, v, offsets, heads, kv_heads, 0, 0))
+
+
+@pytest.mark.parametrize("d", [36, 64, 128])
+def test_rows_of_no_request_are_left_alone(S, d):
+    """Rows from the last request's end on (a step planned with room to spare) are not written, whichever kernel runs."""
+    rng = np.random.default_rng(d)
+    heads, kv_heads, spare = 4, 2, 5
+    for held, nodes in (([50, 3], [5, 2]), ([1500], [4]), ([400], [40])):
+        x = tree_inputs(rng, held, nodes, heads, kv_heads, d, 16, "model")
+        want = tree_rows(x, heads, kv_heads, scale_of(d), 0)
+        n = sum(nodes)
+        x["q"] = np.concatenate([x["q"], values(rng, (spare, heads * d), "model")])
+        x["masks"] = np.concatenate([x["masks"], np.zeros(spare, np.int64)])
+        out = cuda(np.full((n + spare, heads * d), 7, np.int32))
+        got = run_tree(S, x, heads, kv_heads, scale_of(d), 0, max(nodes), max(held) + max(nodes), out=out)
+        assert np.array_equal(got[:n], want) and (got[n:] == 7).all(), held
+    for lengths in ([20, 45], [150, 0, 33], [1030]):
+        n = sum(lengths)
+        q, k, v = (values(rng, (n + spare, w * d), "model") for w in (heads, kv_heads, kv_heads))
+        offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+        out = cuda(np.full((n + spare, heads * d), 7, np.int32))
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), max(lengths), heads=heads, kv_heads=kv_heads,
+                                 scale_q32=scale_of(d), out=out).cpu().numpy()
+        assert np.array_equal(got[:n], ref.prompts(q[:n], k[:n], v[:n], offsets, heads, kv_heads, scale_of(d), 0))
+        assert (got[n:] == 7).all(), lengths
