@@ -602,7 +602,7 @@ cudaError_t launch_values(const IrisTreeAttention& a, const TreeScratch& sc, dim
 
 bool tree_mma_usable(const IrisTreeAttention& a) {
   return a.head_dim % 32 == 0 && a.scale_q32 < 0x80000000u && a.requests <= 65535 && a.kv_heads <= 65535 &&
-         a.longest > 0 && a.pages > 0 && a.pages * a.page_size < 0xFFFFFFFFull &&
+         a.longest > 0 && a.longest <= 65535 * kTreeSegment && a.pages > 0 && a.pages * a.page_size < 0xFFFFFFFFull &&
          (uint64_t)a.rows * a.heads < 0xFFFFFFFFull && (uint64_t)a.heads * kTreeNodes <= 65535;
 }
 

@@ -211,3 +211,15 @@ def test_rows_of_no_request_are_left_alone(S, d):
                                  scale_q32=scale_of(d), out=out).cpu().numpy()
         assert np.array_equal(got[:n], ref.prompts(q[:n], k[:n], v[:n], offsets, heads, kv_heads, scale_of(d), 0))
         assert (got[n:] == 7).all(), lengths
+
+
+def test_trees_with_a_bound_past_67_million_keys(S):
+    """The widest table: the row kernel takes what the launches' grids cannot."""
+    rng = np.random.default_rng(9)
+    x = tree_inputs(rng, [20], [2], 2, 1, 64, 16, "model")
+    table = np.full((1, (1 << 27) // 16 - 1), -1, np.int32)
+    table[:, :x["table"].shape[1]] = x["table"]
+    x["table"] = table
+    for longest in (65535 * 1024, 65535 * 1024 + 1, (1 << 27) - 16):
+        got = run_tree(S, x, 2, 1, scale_of(64), 0, 2, longest)
+        assert np.array_equal(got, tree_rows(x, 2, 1, scale_of(64), 0)), longest

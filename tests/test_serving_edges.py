@@ -175,3 +175,16 @@ def test_the_wrappers_name_the_tensor_of_a_wrong_shape(call, shape):
         tensors[name] = Fake(*shape, dtype=x.dtype)
         with pytest.raises(ValueError, match=name):
             run(tensors)
+
+
+def test_trees_past_a_grid_of_segments_need_no_scratch(lib):
+    """Bounds past 65,535 segments of 1,024 keys are the row kernel's."""
+    a = 1 << 20
+
+    def need(longest):
+        t = lib.TreeAttention(a, a, a, a, a, a, a, None, a, 128, 128, 8, 1, 2, 1 << 23, 16, 2, longest, 2, 1, 64, 0, 1)
+        return lib.lib().iris_tree_attention_workspace(C.byref(t))
+
+    assert need(65535 * 1024) >= 65535 * 1024 * 16
+    for longest in (65535 * 1024 + 1, 1 << 27):
+        assert need(longest) == 0
