@@ -11,9 +11,10 @@
 //      epilogue adds them modulo 2^64, as the reference's wrapping sum.
 //   2. softmax on CUDA cores, one warp a (query, head): first maximum, exp
 //      terms and their sum, weights by one exact reciprocal, the residual
-//      1.0 - sum(weights) on the first maximum's weight; the weights
-//      (0..65536) are written as three byte planes, zero past the query's
-//      position (the causal mask).
+//      1.0 - sum(weights) on the first maximum's weight; the weights (0..65536;
+//      the first maximum's may be negative: 724 or more equal ones round up to more
+//      than 1.0 together) are written as three byte planes, the third signed, zero
+//      past the query's position (the causal mask).
 //   3. values: ctx[q][h][d] = requantize(sum_t w[q][t] v[t][d]): twelve MMAs
 //      (M = 128 dims from the transposed value planes, N = 64 queries, K = the
 //      positions) into six diagonals; a diagonal's true sum lies in
@@ -46,10 +47,13 @@ constexpr uint32_t kAtAPlane = kTcTileM * kTcTileK, kAtBPlane = kTcTileN * kTcTi
 constexpr uint32_t kAtStages = 2;
 constexpr uint32_t kAtMaxPositions = 22016;
 
-// Lower bound of one position's contribution to a value-sum diagonal s
-// (value planes i: 0-2 unsigned, 3 signed; weight planes j: 0-1 unsigned,
-// 2 holds 0 or 1).
-__host__ __device__ constexpr int64_t pv_diag_min(uint32_t s) { return s == 3 || s == 4 ? -32640 : s == 5 ? -128 : 0; }
+// Lower bound of a value-sum diagonal s over `positions` (value planes i: 0-2
+// unsigned, 3 signed; weight planes j: 0-1 unsigned, 2 holds 0 or 1, or -1 at one
+// position). Upper ones are below 130,305 a position: within 2^32 of it.
+__host__ __device__ constexpr int64_t pv_diag_min(uint32_t s, uint32_t positions) {
+  return (s == 3 || s == 4 ? -32640 : s == 5 ? -128 : 0) * (int64_t)positions - (s >= 2 ? 255 : 0);
+}
+static_assert((int64_t)kAtMaxPositions * 130305 - pv_diag_min(3, 0) < (int64_t)1 << 32, "diagonals of the value sums");
 
 struct ScoreTiles {  // tile = (head, query tile, key tile); one K stage (the 128 dims)
   uint32_t heads, group, qtiles, ktiles;
@@ -83,7 +87,8 @@ struct ValueTiles {  // tile = (head, query tile); K stages over the positions
 // (M = 128 rows) against NB planes of B (N = 64 columns), pair (i, j) into
 // diagonal i + j. Epi::value turns the diagonals' raw int32 values of one
 // (TMEM lane row, column) into the output, Epi::store writes it (after the
-// accumulators are released).
+// accumulators are released). The last plane of each operand is signed, the others
+// not.
 template <uint32_t NA, uint32_t NB, class Tiles, class Epi>
 __device__ __forceinline__ void at_pipeline(const Tiles& tiles, const Epi& epi, const CUtensorMap* amap,
                                             const CUtensorMap* bmap, unsigned int* fault, uint8_t* ring) {
@@ -173,7 +178,7 @@ __device__ __forceinline__ void at_pipeline(const Tiles& tiles, const Epi& epi, 
               for (uint32_t j = 0; j < NB; ++j) {
                 const uint64_t bd = tc_desc(base + NA * kAtAPlane + j * kAtBPlane + kk * 32);
                 const uint32_t d = i + j;
-                tc_mma(tmem + d * kTcTileN, ad, bd, tc_idesc(i == 3, Tiles::kBSigned && j == 3), (touched >> d) & 1u);
+                tc_mma(tmem + d * kTcTileN, ad, bd, tc_idesc(i == 3, j + 1 == NB), (touched >> d) & 1u);
                 touched |= 1u << d;
               }
             }
@@ -246,7 +251,7 @@ struct ValueEpi {
     uint64_t acc = 0;
 #pragma unroll
     for (uint32_t d = 0; d < 6; ++d) {
-      const int64_t lb = pv_diag_min(d) * (int64_t)pcap;
+      const int64_t lb = pv_diag_min(d, pcap);
       const int64_t T = lb + (int64_t)(uint32_t)(v[d] - (uint32_t)lb);
       acc += (uint64_t)T << (8 * d);
     }
@@ -261,15 +266,8 @@ struct ValueEpi {
   }
 };
 
-struct ScoreTilesS : ScoreTiles {
-  static constexpr bool kBSigned = true;
-};
-struct ValueTilesS : ValueTiles {
-  static constexpr bool kBSigned = false;  // weight planes are unsigned
-};
-
 __global__ void __launch_bounds__(kAtThreads, 1)
-    attn_tc_scores_kernel(ScoreTilesS tiles, ScoreEpi epi, const __grid_constant__ CUtensorMap kmap,
+    attn_tc_scores_kernel(ScoreTiles tiles, ScoreEpi epi, const __grid_constant__ CUtensorMap kmap,
                           const __grid_constant__ CUtensorMap qmap, unsigned int* fault) {
   extern __shared__ uint8_t at_raw[];
   uint8_t* ring = (uint8_t*)(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
@@ -277,7 +275,7 @@ __global__ void __launch_bounds__(kAtThreads, 1)
 }
 
 __global__ void __launch_bounds__(kAtThreads, 1)
-    attn_tc_values_kernel(ValueTilesS tiles, ValueEpi epi, const __grid_constant__ CUtensorMap vmap,
+    attn_tc_values_kernel(ValueTiles tiles, ValueEpi epi, const __grid_constant__ CUtensorMap vmap,
                           const __grid_constant__ CUtensorMap wmap, unsigned int* fault) {
   extern __shared__ uint8_t at_raw[];
   uint8_t* ring = (uint8_t*)(((uintptr_t)at_raw + 1023) & ~(uintptr_t)1023);
@@ -522,7 +520,7 @@ cudaError_t launch_attention_prefill_tc(const AttnArgs& a, uint32_t tokens, cons
       !make_map(&wmap, sc.wp, pcap, qcap, (uint64_t)a.heads * 3, pcap, (uint64_t)qcap * pcap, kTcTileN, 1))
     return cudaErrorInvalidValue;
   const uint32_t qtiles = qcap / kTcTileN, ktiles = pcap / kTcTileM, sms = (uint32_t)device_sms();
-  ScoreTilesS st;
+  ScoreTiles st;
   st.heads = a.heads, st.group = group, st.qtiles = qtiles, st.ktiles = ktiles;
   ScoreEpi se{sc.s, qtiles, ktiles, qcap, pcap, tokens, a.mode, a.scale_q32};
   const uint32_t sc_tiles = a.heads * qtiles * ktiles;
@@ -533,7 +531,7 @@ cudaError_t launch_attention_prefill_tc(const AttnArgs& a, uint32_t tokens, cons
                dim3(32 * kSoftRowsPerBlock), 0, stream, (int32_t*)sc.s, sc.wp, qcap, pcap, a.pos0, tokens,
                a.heads);
   if (e != cudaSuccess) return e;
-  ValueTilesS vt;
+  ValueTiles vt;
   vt.heads = a.heads, vt.group = group, vt.qtiles = qtiles, vt.kstages = pcap / kTcTileK;
   ValueEpi ve{a.ctx_planes, a.ctx, qtiles, tokens, qd, pcap};
   const uint32_t v_tiles = a.heads * qtiles;
