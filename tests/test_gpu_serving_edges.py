@@ -223,3 +223,35 @@ def test_trees_with_a_bound_past_67_million_keys(S):
     for longest in (65535 * 1024, 65535 * 1024 + 1, (1 << 27) - 16):
         got = run_tree(S, x, 2, 1, scale_of(64), 0, 2, longest)
         assert np.array_equal(got, tree_rows(x, 2, 1, scale_of(64), 0)), longest
+
+
+@pytest.mark.parametrize("n,heads,d,window,kind", [(16256, 1, 128, 0, "model"), (16257, 1, 64, 0, "model"),
+                                                   (17000, 2, 32, 0, "wide"), (17000, 1, 32, 16700, "model"),
+                                                   (33000, 1, 32, 0, "model")])
+def test_prompts_at_and_past_the_longest_of_the_tensor_cores(S, n, heads, d, window, kind):
+    """Rows past 16,256 keys, and past the 16,384 that one int32 accumulator holds, checked one by one."""
+    rng = np.random.default_rng(n + d)
+    q, k = (values(rng, (n, w * d), "model") for w in (heads, 1))
+    v = values(rng, (n, d), kind)
+    k[16200:16220] = k[3]              # ties far apart: the first maximum counts
+    v[100:] = np.abs(v[100:]) + 5000000  # large sums of one sign
+    got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(np.array([0, n], np.int32)), n, heads=heads, kv_heads=1,
+                             scale_q32=scale_of(d), window=window).cpu().numpy()
+    for i in [0, 5, 127, 128, 16127, n - 65, n - 2, n - 1]:
+        lo = max(0, i + 1 - window) if window else 0
+        for h in range(heads):
+            c = slice(h * d, (h + 1) * d)
+            assert np.array_equal(got[i, c], ref.attend(q[i, c], k[lo:i + 1], v[lo:i + 1], scale_of(d))), (i, h)
+
+
+@pytest.mark.parametrize("d", [32, 36, 256])
+def test_prompts_of_more_requests_than_are_sorted(S, d):
+    rng = np.random.default_rng(d)
+    lengths = rng.choice([0, 1, 2, 3, 9], 1100)
+    lengths[700] = 130
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int32)
+    n = int(offsets[-1])
+    q, k, v = (values(rng, (n, w * d), "model") for w in (2, 1, 1))
+    got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 130, heads=2, kv_heads=1,
+                             scale_q32=scale_of(d)).cpu().numpy()
+    assert np.array_equal(got, ref.prompts(q, k, v, offsets, 2, 1, scale_of(d), 0))
