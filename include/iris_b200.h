@@ -531,7 +531,9 @@ typedef struct {
 } IrisPromptAttention;
 /* Bytes of device scratch (16-byte aligned) the call needs, 0 for refused
  * arguments; a smaller workspace is refused with IRIS_ESCRATCH. Its contents
- * mean nothing between calls. */
+ * mean nothing between calls. About 38 KB for each key a row sees at most (the
+ * longest request, or the window), and three bytes a query, key and value of
+ * longer prompts. */
 uint64_t iris_prompt_attention_workspace(const IrisPromptAttention* a);
 int iris_prompt_attention(const IrisPromptAttention* a, void* workspace, uint64_t workspace_bytes, void* stream);
 /* Attention of drafted trees over the paged cache (K/V of the nodes appended
@@ -556,6 +558,10 @@ typedef struct {
   uint32_t heads, kv_heads, head_dim;
   uint32_t window, scale_q32;
 } IrisTreeAttention;
+/* As above. A call of more than a few rows keeps every score: 4 * rows * heads *
+ * longest bytes, the longest request's length for every row (24 nodes of each of
+ * 64 requests, 32 heads, 32,000 keys: 6.3 GB). Where one context is much longer
+ * than the others, a call for it and one for them need far less. */
 uint64_t iris_tree_attention_workspace(const IrisTreeAttention* a);
 int iris_tree_attention(const IrisTreeAttention* a, void* workspace, uint64_t workspace_bytes, void* stream);
 /* The drafted tokens that greedy decoding accepts: from a request's node 0

@@ -12,7 +12,7 @@
 // its item, which mostly stays in L2. Tiles are handed out longest first; few
 // tiles, a block each, are counted by the blocks themselves in one launch.
 // Bound by the chain of its phases on a few rows (five requests of up to 96 rows, 4
-// heads of 64, 27 us; with the list in a launch of its own 39 us) and by the products and the score and
+// heads of 64, 27 us on thirteen blocks; with the list in a launch of its own 39 us) and by the products and the score and
 // exponential arithmetic on many (512 rows, 32 heads of 128, 101 us; prompt_tc.cu
 // takes over there).
 #include <algorithm>

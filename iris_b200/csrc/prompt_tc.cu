@@ -27,12 +27,16 @@
 // a give-up ends the block and is recorded in the fault word.
 //
 // Requests of 4,096, 1,037, 711, 300 and 1 rows, 32 query heads over 8 of 128
-// values: 1,910 us (295 M pairs, 79 TFLOP/s of the plain products); 1,025, 640, 512
-// and 37 rows, 8 heads over one of 256: 135 us. Bound by the integer arithmetic of
-// the epilogue warps, not by the products: of a tile's cycles 38 % are scores (2,800
-// for 128 keys x 64 rows: a 64-bit product and rounding each), 30 % the exact
-// exponentials (3,300), 30 % weights and value sums, the wait for products a tenth
-// of each.
+// values: 1,897 us (295 M pairs, 79 TFLOP/s of the plain products); 1,025, 640, 512
+// and 37 rows, 8 heads over one of 256: 134 us. Bound by the epilogue warps, not by
+// the products (their unit is busy 12 %), and there by latency: half of the issue
+// slots stay empty and the integer pipes are 37 % busy, since a block's sixteen warps
+// take the three phases in strict turn and each waits for its loads of scores or
+// terms (the largest stall). Of a tile's cycles 38 % are scores (2,800 for 128 keys
+// x 64 rows: a 64-bit product and rounding each), 30 % the exact exponentials
+// (3,300), 30 % weights and value sums, the wait for products a tenth of each. One
+// value past 24 bits leaves the call to prompt_mma_kernel: 4,950 to 5,230 us and 264
+// to 292 us for these two calls in all, against 1,960 and 150.
 #include <algorithm>
 
 #include "../../include/iris_b200.h"

@@ -9,8 +9,9 @@
 // are read once, straight into the matrix instructions' operands, and nothing
 // goes through global memory but the outputs. Bound by latency on short
 // contexts (three exchanges, two dependent reads of the pages: one node over 777
-// keys, 32 query heads, 8 of 128 values, 14.6 us), by the reading of the pages on
-// long ones (four requests of one node over 12,000 keys 119 us, 3.3 TB/s).
+// keys, 32 query heads, 8 of 128 values, 14.7 us), by that of reading the pages on
+// long ones, a step ahead in registers (four requests of one node over 12,000 keys
+// 119 us, 3.3 TB/s of 6.46).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -16,8 +16,9 @@
 // K and V cross HBM once each; the scores (4 bytes a row and key, a fraction of
 // the keys' 512) stay in L2 between the launches while they fit.
 // One node of sixteen requests over 4,000 keys (32 query heads, 8 of 128 values,
-// 524 MB): 182 us, 2.9 TB/s, bound by the reading of K and V in the third launch
-// (114 us; eight rows leave a product of 16 x 8 half used) and in the first (66).
+// 524 MB): 182 us, 2.9 TB/s of 6.46, the third launch 114 us (eight rows leave a
+// product of 16 x 8 half used), the first 66: bound by the latency of reading K and
+// V, of which a warp has one step of 32 dimensions or positions in flight ahead.
 // 48 and 64 nodes over 20,011 and 32,001 keys: the second launch 184 us for 96 M
 // exponentials, bound by their arithmetic (the same a pair where the scores fit L2).
 #include <algorithm>

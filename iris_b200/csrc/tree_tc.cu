@@ -16,11 +16,15 @@
 // wait is bounded and a give-up ends the block and is recorded in the fault word.
 //
 // 64 and 48 nodes over 32,001 and 20,011 keys (32 query heads, 8 of 128 values): 251
-// us for the scores, 248 us for the values, of 701. The scores are bound by
-// their integer arithmetic and the splitting of the keys (without the score's
-// stores, the maxima, or three quarters of the products they take 1 to 5 % less), the
-// values by the reading of the terms (the scratch is 384 MB there) and the weights'
-// arithmetic; the products' unit is busy a tenth of the time.
+// us for the scores, 248 us for the values, of 700. The products' unit is busy a
+// tenth of the time, and the scores leave half of the issue slots empty (integer
+// pipes 41 % busy): bound by the latency of a block's one chain of loading and
+// splitting keys, waiting for products and finishing scores, with one block a
+// multiprocessor (without the score's stores, the maxima, or three quarters of the
+// products they take 1 to 5 % less); the values by the reading of the terms (the
+// scratch is 384 MB there) and the weights' arithmetic. A value past 24 bits that
+// the call names runs the launches of tree_mma.cu after these: 1,330 to 1,460 us in
+// all, and 513 to 527 for the trees of a batch that take 245.
 #include <algorithm>
 
 #include "../../include/iris_b200.h"

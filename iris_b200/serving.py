@@ -43,7 +43,7 @@ class PagePlan(NamedTuple):
     masks: Optional[torch.Tensor]  # [tokens] int64, with parents
 
     def faults(self) -> int:
-        """PLAN_* bits of this plan (0: every token has its slot)."""
+        """PLAN_* bits of this plan (0: the pages, the table and the rows sufficed)."""
         return int(self.counts[3])
 
 
