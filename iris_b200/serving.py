@@ -31,6 +31,7 @@ from . import _lib
 from ._lib import check, lib
 
 TREE_NODES = 64  # drafted nodes a request
+U32 = 1 << 32
 
 
 class PagePlan(NamedTuple):
@@ -74,9 +75,9 @@ def _dense(x: torch.Tensor, name: str, dev: int, dtype: torch.dtype = torch.int3
     return x.data_ptr()
 
 
-def _stride(x: torch.Tensor) -> int:
+def _stride(x: torch.Tensor, rows: int, width: int) -> int:
     """The values between two rows; of a single row torch may give any."""
-    return x.stride(0) if x.shape[0] != 1 else x.shape[1]
+    return x.stride(0) if rows != 1 else width
 
 
 def _same(count: int, want: int, name: str) -> None:
@@ -87,7 +88,7 @@ def _same(count: int, want: int, name: str) -> None:
 def _ranges(**values: int) -> None:
     """Refuses what is no 32-bit count (ctypes would cut it to one)."""
     for name, value in values.items():
-        if not 0 <= value < 1 << 32:
+        if not 0 <= value < U32:
             raise ValueError(f"{name}: {value} is not between 0 and 2^32 - 1")
 
 
@@ -110,7 +111,7 @@ def page_plan(held: torch.Tensor, fresh: torch.Tensor, table: torch.Tensor, free
     ph, pf = _dense(held, "held", dev), _dense(fresh, "fresh", dev)
     pt, pp = _dense(table, "table", dev, dim=2), _dense(free_pages, "free_pages", dev)
     requests, width, n_free = held.numel(), table.shape[1], free_pages.numel()
-    if (page_size | tokens) >> 32:
+    if not (0 <= page_size < U32 and 0 <= tokens < U32):
         _ranges(page_size=page_size, tokens=tokens)
     _same(fresh.numel(), requests, "fresh")
     _same(table.shape[0], requests, "table")
@@ -142,8 +143,8 @@ def page_append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: 
         raise ValueError(f"rows {tuple(k.shape)}, {tuple(v.shape)} and pools {tuple(k_pages.shape)}, "
                          f"{tuple(v_pages.shape)} do not match")
     _same(slots.numel(), tokens, "slots")
-    check(lib().iris_page_append(pk, pv, _stride(k), _stride(v), tokens, kv_dim, ps, ck, cv,
-                                 k_pages.shape[0] * k_pages.shape[1], _stream(dev)), "iris_page_append")
+    check(lib().iris_page_append(pk, pv, _stride(k, tokens, kv_dim), _stride(v, tokens, kv_dim), tokens, kv_dim, ps, ck,
+                                 cv, k_pages.shape[0] * k_pages.shape[1], _stream(dev)), "iris_page_append")
 
 
 def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
@@ -161,7 +162,8 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     dev = q.get_device()
     pq, pk, pv, po = _rows(q, "q", dev), _rows(k, "k", dev), _rows(v, "v", dev), _dense(offsets, "offsets", dev)
     tokens, requests = q.shape[0], offsets.numel() - 1
-    if (requests | longest | heads | kv_heads | window | scale_q32) >> 32:
+    if not (0 <= requests and 0 <= longest < U32 and 0 <= heads < U32 and 0 <= kv_heads < U32 and 0 <= window < U32
+            and 0 <= scale_q32 < U32):
         _ranges(requests=requests, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
@@ -172,9 +174,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         out = q.new_empty((tokens, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), _stride(q), _stride(k), _stride(v),
-                             _stride(out), requests, tokens, longest, heads, kv_heads, dim, window,
-                             scale_q32)
+    qd, kd = heads * dim, kv_heads * dim
+    a = _lib.PromptAttention(pq, pk, pv, po, _rows(out, "out", dev), _stride(q, tokens, qd), _stride(k, tokens, kd),
+                             _stride(v, tokens, kd), _stride(out, tokens, qd), requests, tokens, longest, heads,
+                             kv_heads, dim, window, scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_prompt_attention_workspace(ref), q.device)
     check(L.iris_prompt_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
@@ -198,7 +201,8 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     pm = _dense(masks, "masks", dev, torch.int64)
     pp = _dense(positions, "positions", dev) if positions is not None else None
     rows, requests = q.shape[0], held.numel()
-    if (nodes | longest | heads | kv_heads | window | scale_q32) >> 32:
+    if not (0 <= nodes < U32 and 0 <= longest < U32 and 0 <= heads < U32 and 0 <= kv_heads < U32 and 0 <= window < U32
+            and 0 <= scale_q32 < U32):
         _ranges(nodes=nodes, longest=longest, heads=heads, kv_heads=kv_heads, window=window, scale_q32=scale_q32)
     if heads < 1 or kv_heads < 1 or q.shape[1] % heads:
         raise ValueError(f"q rows of {q.shape[1]} values are not {heads} heads")
@@ -214,9 +218,9 @@ def tree_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         out = q.new_empty((rows, heads * dim))
     elif out.shape != q.shape:
         raise ValueError(f"out: {tuple(out.shape)}, expected {tuple(q.shape)}")
-    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out", dev), _stride(q), _stride(out),
-                           k_pages.shape[0], requests, rows, table.shape[1], k_pages.shape[1], nodes, longest, heads,
-                           kv_heads, dim, window, scale_q32)
+    a = _lib.TreeAttention(pq, ck, cv, pt, ph, po, pm, pp, _rows(out, "out", dev), _stride(q, rows, heads * dim),
+                           _stride(out, rows, heads * dim), k_pages.shape[0], requests, rows, table.shape[1],
+                           k_pages.shape[1], nodes, longest, heads, kv_heads, dim, window, scale_q32)
     L, ref = lib(), C.byref(a)
     ws = _workspace(L.iris_tree_attention_workspace(ref), q.device)
     check(L.iris_tree_attention(ref, ws.data_ptr() if ws is not None else None, ws.numel() if ws is not None else 0,
@@ -235,7 +239,7 @@ def tree_accept(tokens: torch.Tensor, parents: torch.Tensor, picks: torch.Tensor
     dev = tokens.get_device()
     pt, pa, pk = _dense(tokens, "tokens", dev), _dense(parents, "parents", dev), _dense(picks, "picks", dev)
     po, ph, tb = _dense(offsets, "offsets", dev), _dense(held, "held", dev), _dense(table, "table", dev, dim=2)
-    if path_width >> 32:
+    if not 0 <= path_width < U32:
         _ranges(path_width=path_width)
     _same(parents.numel(), rows, "parents")
     _same(picks.numel(), rows, "picks")

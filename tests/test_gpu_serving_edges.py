@@ -255,3 +255,16 @@ def test_prompts_of_more_requests_than_are_sorted(S, d):
     got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), 130, heads=2, kv_heads=1,
                              scale_q32=scale_of(d)).cpu().numpy()
     assert np.array_equal(got, ref.prompts(q, k, v, offsets, 2, 1, scale_of(d), 0))
+
+
+def test_numbers_may_be_numpys(S):
+    """Bounds taken from numpy's arrays, next to a scale of 2^31 (heads of four values)."""
+    rng = np.random.default_rng(2)
+    q, k, v = (values(rng, (9, w), "model") for w in (8, 4, 4))
+    offsets = np.array([0, 4, 9], np.int32)
+    want = ref.prompts(q, k, v, offsets, 2, 1, 1 << 31, 0)
+    assert scale_of(4) == 1 << 31
+    for number in (np.int32, np.uint32, np.int64, np.uint8):
+        got = S.prompt_attention(cuda(q), cuda(k), cuda(v), cuda(offsets), number(5), heads=number(2),
+                                 kv_heads=number(1), scale_q32=scale_of(4), window=number(0))
+        assert np.array_equal(got.cpu().numpy(), want)
